@@ -62,6 +62,10 @@ class accb_value_type(C.Structure):
     _fields_ = [("rank", C.c_int), ("ncomp", C.c_int), ("comp_bytes", C.c_int * MAX_COMP)]
 
 
+class accb_rows_array(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("type", C.c_int), ("cols", C.c_int), ("rows", C.c_longlong), ("pitch", C.c_longlong)]
+
+
 class InputArray(C.Structure):
     _fields_ = [("shape", C.POINTER(C.c_int)), ("adata", C.POINTER(C.c_void_p))]
 
@@ -81,7 +85,7 @@ def lib() -> C.CDLL:
             raise AccbError(ENOTFOUND, f"{LIBRARY_PATH} is missing: run `python accelerate-cuda_b200/build.py`")
         L = C.CDLL(LIBRARY_PATH)
         vp, ll, i32, u64, sz = C.c_void_p, C.c_longlong, C.c_int, C.c_uint64, C.c_size_t
-        arrp = C.POINTER(accb_array)
+        arrp, rowsp = C.POINTER(accb_array), C.POINTER(accb_rows_array)
         sigs = {
             "accb_init": [],
             "accb_device_count": [C.POINTER(i32)],
@@ -132,6 +136,10 @@ def lib() -> C.CDLL:
             "accb_stencil2": [vp, vp, vp, arrp, arrp, i32, vp, sz, arrp],
             "accb_stencil_iterate": [vp, vp, vp, arrp, arrp, i32, i32, vp, sz, C.POINTER(i32)],
             "accb_stencil_iterate_from": [vp, vp, vp, arrp, arrp, arrp, i32, i32, vp, sz, C.POINTER(i32)],
+            "accb_top_rows": [vp, vp, rowsp, C.c_double, i32, vp, vp, vp],
+            "accb_sample_rows": [vp, vp, rowsp, vp, ll] + [vp] * 7,
+            "accb_distill_rows": [vp, vp, rowsp, vp, i32, vp, i32, vp, vp, C.c_double, vp, vp, rowsp],
+            "accb_distill_rows_backward": [vp, vp, rowsp, vp, i32, vp, i32, vp, vp, C.c_double, vp, vp, rowsp],
             "accb_program_create": [vp, i32, C.POINTER(accb_value_type), C.POINTER(vp)],
             "accb_program_map": [vp, vp, C.POINTER(i32), i32, i32, C.POINTER(accb_value_type), vp, sz],
             "accb_program_fold": [vp, vp, C.POINTER(i32), i32, i32, i32, vp, sz, C.POINTER(accb_value_type)],
@@ -271,6 +279,16 @@ def _bytes_of(value, dtype=None):
     else:
         b = (np.asarray(value, dtype=dtype) if dtype is not None else np.asarray(value)).tobytes()
     return C.create_string_buffer(b, len(b)), len(b)
+
+
+ROWS_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+
+def _element_type(t) -> str:
+    """"float32", "bfloat16", ... of a tensor or a ``DeviceArray``."""
+    if not hasattr(t, "dtype"):
+        raise TypeError(f"not a device array: {type(t)!r}")
+    return str(t.dtype).rsplit(".", 1)[-1]
 
 
 class DeviceArray:
@@ -539,6 +557,116 @@ class Context:
                                                C.byref(ss) if ss is not None else None, C.byref(aa), C.byref(bb), iters,
                                                BOUNDARY[boundary], cb, cn, C.byref(in_b)), self.handle)
         return b if in_b.value else a
+
+    # -- rows of scores
+    def _on_device(self, name, t, kinds, shape):
+        """The address of an argument that must be a contiguous device array of this shape and one of these types."""
+        if t is None:
+            return None
+        kind = _element_type(t)
+        if kind not in kinds:
+            raise AccbError(EINVAL, f"{name}: elements of type {kind}, not {' or '.join(kinds)}")
+        if tuple(t.shape) != tuple(shape):
+            raise AccbError(EINVAL, f"{name}: shape {tuple(t.shape)}, not {tuple(shape)}")
+        if hasattr(t, "is_contiguous") and not t.is_contiguous():
+            raise AccbError(EINVAL, f"{name}: not contiguous")
+        self._check_device(name, t)
+        return C.c_void_p(_ptr(t))
+
+    def _check_device(self, name, t):
+        device = getattr(t, "device", None)
+        if device is not None and (device.type != "cuda" or device.index != self.device):
+            raise AccbError(EINVAL, f"{name}: on {device}, not on cuda:{self.device}")
+
+    def _rows(self, name, t) -> accb_rows_array:
+        """A matrix of scores: contiguous rows, any distance from row to row."""
+        kind = _element_type(t)
+        if kind not in ROWS_TYPES:
+            raise AccbError(EINVAL, f"{name}: elements of type {kind}, not {' or '.join(ROWS_TYPES)}")
+        if len(t.shape) != 2:
+            raise AccbError(EINVAL, f"{name}: rank {len(t.shape)}, not 2")
+        rows, cols = (int(e) for e in t.shape)
+        pitch = cols
+        if hasattr(t, "stride"):
+            if cols > 1 and t.stride(1) != 1:
+                raise AccbError(EINVAL, f"{name}: the entries of a row are not contiguous")
+            pitch = int(t.stride(0)) if rows > 1 else cols
+        if cols >= 1 << 31:
+            raise AccbError(EINVAL, f"{name}: rows of {cols} entries")
+        self._check_device(name, t)
+        return accb_rows_array(_ptr(t), ROWS_TYPES[kind], cols, rows, pitch)
+
+    def _own_stream(self, stream):
+        """The given stream, or the current one of this context's device."""
+        if stream is not None:
+            return C.c_void_p(int(stream))
+        try:
+            import torch
+        except ImportError:
+            return C.c_void_p(0)
+        return C.c_void_p(int(torch.cuda.current_stream(self.device).cuda_stream))
+
+    def top_rows(self, x, values, index, lse=None, temperature: float = 1.0, stream=None):
+        """The ``k`` largest scores of every row of ``x`` in falling order (equal ones by rising index) and where they
+        are: ``values`` and ``index`` have shape rows x k.  ``lse``: log-sum-exp of the whole row at ``temperature``.
+        See ``accb_top_rows`` in ``include/accb200.h``."""
+        a = self._rows("x", x)
+        if len(values.shape) != 2:
+            raise AccbError(EINVAL, f"values: rank {len(values.shape)}, not 2")
+        k = int(values.shape[1])
+        v = self._on_device("values", values, (_element_type(x),), (a.rows, k))
+        i = self._on_device("index", index, ("int32",), (a.rows, k))
+        s = self._on_device("lse", lse, ("float32",), (a.rows,))
+        _check(lib().accb_top_rows(self.handle, self._own_stream(stream), C.byref(a), temperature, k, v, i, s), self.handle)
+
+    def sample_rows(self, x, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                    allowed=None, stream=None):
+        """One index per row of ``x``, drawn by the random number ``uniform`` of the row among the entries that
+        ``top_k``, ``top_p`` and ``min_p`` keep (arrays of one value per row, or None).  ``allowed``: rows x
+        ceil(cols / 32) words of bits.  See ``accb_sample_rows`` in ``include/accb200.h``."""
+        a = self._rows("x", x)
+        each = [self._on_device(name, t, kinds, (a.rows,)) for name, t, kinds in (
+            ("uniform", uniform, ("float32",)), ("temperature", temperature, ("float32",)), ("top_k", top_k, ("int32",)),
+            ("top_p", top_p, ("float32",)), ("min_p", min_p, ("float32",)), ("token", token, ("int32",)),
+            ("logprob", logprob, ("float32",)))]
+        words = (a.cols + 31) // 32
+        bits = self._on_device("allowed", allowed, ("int32", "uint32"), (a.rows, words))
+        _check(lib().accb_sample_rows(self.handle, self._own_stream(stream), C.byref(a), bits, words, *each), self.handle)
+
+    def _teacher(self, a, teacher, index, teacher_lse, weight):
+        if len(teacher.shape) != 2:
+            raise AccbError(EINVAL, f"teacher: rank {len(teacher.shape)}, not 2")
+        k = int(teacher.shape[1])
+        t = self._on_device("teacher", teacher, tuple(ROWS_TYPES), (a.rows, k))
+        i = self._on_device("index", index, ("int32",), (a.rows, k))
+        s = self._on_device("teacher_lse", teacher_lse, ("float32",), (a.rows,))
+        w = self._on_device("weight", weight, ("float32",), (a.rows,))
+        return t, ROWS_TYPES[_element_type(teacher)], i, k, s, w
+
+    def distill_rows(self, student, teacher, index, loss, grad=None, stats=None, teacher_lse=None, weight=None,
+                     temperature: float = 1.0, stream=None):
+        """The divergence of every row of ``student`` from a teacher's scores ``teacher`` of the entries ``index``
+        (rows x k), into ``loss``; with ``grad`` its gradient in the same pass, with ``stats`` (rows x 4) what
+        ``distill_rows_backward`` needs.  See ``accb_distill_rows`` in ``include/accb200.h``."""
+        a = self._rows("student", student)
+        t = self._teacher(a, teacher, index, teacher_lse, weight)
+        lo = self._on_device("loss", loss, ("float32",), (a.rows,))
+        st = self._on_device("stats", stats, ("float32",), (a.rows, 4))
+        g = self._rows("grad", grad) if grad is not None else None
+        _check(lib().accb_distill_rows(self.handle, self._own_stream(stream), C.byref(a), *t, temperature, lo, st,
+                                       C.byref(g) if g is not None else None), self.handle)
+
+    def distill_rows_backward(self, student, teacher, index, stats, upstream, grad, teacher_lse=None, weight=None,
+                              temperature: float = 1.0, stream=None):
+        """The gradient of ``distill_rows`` from the statistics it left, for the gradient ``upstream`` of the rows'
+        losses (None: 1).  See ``accb_distill_rows_backward`` in ``include/accb200.h``."""
+        a = self._rows("student", student)
+        t = self._teacher(a, teacher, index, teacher_lse, weight)
+        st = self._on_device("stats", stats, ("float32",), (a.rows, 4))
+        up = self._on_device("upstream", upstream, ("float32",), (a.rows,))
+        g = self._rows("grad", grad)
+        _check(lib().accb_distill_rows_backward(self.handle, self._own_stream(stream), C.byref(a), *t, temperature, st, up,
+                                                C.byref(g)), self.handle)
 
     # -- synthetic inputs
     def gen_uniform_f32(self, dst, n, first, seed, stream_id, lo, hi, stream=None):

@@ -1,0 +1,899 @@
+/*
+ * rows.cu -- operators over rows of scores: the best entries of a row
+ * (accb_top_rows), one index drawn from a row (accb_sample_rows), and the
+ * divergence of a row from a teacher's best entries with its gradient
+ * (accb_distill_rows, accb_distill_rows_backward).
+ *
+ * They stand beside the folds over rows (fold.cuh): a matrix comes in, every
+ * row is reduced.  rows.cuh says how a row is held on chip.
+ */
+#include <algorithm>
+
+#include "common.h"
+#include "rows.cuh"
+
+namespace accb_rows {
+
+struct RowsIn {
+    const void *x;
+    long long rows, pitch; /* pitch in elements */
+    int cols;
+};
+
+/* ------------------------------------------------------------- sampling */
+struct SampleParams {
+    RowsIn in;
+    const unsigned *allowed; /* bit j % 32 of word j / 32: entry j may be drawn; or null */
+    long long allowed_pitch; /* words */
+    const float *uniform, *temperature, *top_p, *min_p;
+    const int *top_k;
+    int *token;
+    float *logprob;
+};
+
+/* the entries of vector v that `bits` (one per entry of the row) does not allow become -inf */
+template <class T, bool R> __device__ __forceinline__ uint4 only_allowed(const Share<T, R> &share, int v, uint4 w, const unsigned *bits) {
+    constexpr int E = Elem<T>::E;
+    float f[E];
+    Elem<T>::unpack(w, f);
+    const int e0 = share.entry(v);
+    unsigned m = 0;
+    if (share.whole(v)) {
+        const unsigned lo = bits[e0 >> 5], hi = (e0 & 31) + E > 32 ? bits[(e0 >> 5) + 1] : 0u;
+        m = __funnelshift_r(lo, hi, e0 & 31);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (e0 + i >= 0 && e0 + i < share.n) m |= ((bits[(e0 + i) >> 5] >> ((e0 + i) & 31)) & 1u) << i;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (!((m >> i) & 1u)) f[i] = neg_inf();
+    return Elem<T>::pack(f);
+}
+
+template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_rows(const SampleParams p) {
+    constexpr int E = Elem<T>::E;
+    extern __shared__ uint4 stage[];
+    __shared__ Exchange ex;
+    __shared__ Level lv;
+    const unsigned size = cluster_size(), rank = cluster_rank();
+    const long long row = blockIdx.x / size;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (size > 1) cluster_arrive(); /* every block of the row has started: waited for before the first message */
+
+    Share<T, R> share;
+    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    share.fetch();
+    const unsigned *bits = p.allowed ? p.allowed + row * p.allowed_pitch : nullptr;
+    float temperature = p.temperature ? p.temperature[row] : 1.0f;
+    const bool greedy = !(temperature > 0.0f);
+    if (greedy) temperature = 1.0f;
+    int k = p.top_k ? p.top_k[row] : 0;
+    if (greedy) k = 1;
+    const float top_p = p.top_p ? p.top_p[row] : 1.0f;
+    const float min_p = p.min_p ? p.min_p[row] : 0.0f;
+    const float uniform = p.uniform[row];
+    share.wait();
+
+    auto get = [&](int v, float *f) {
+        uint4 w = share.get(v);
+        if (!R && bits) w = only_allowed(share, v, w, bits);
+        Elem<T>::unpack(w, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = not_nan(f[i]);
+    };
+
+    /* the maximum, and the smallest of the threads' maxima: at least that many entries are as large */
+    float most = neg_inf();
+    for (int v = share.first; v < share.last; v += 32) {
+        if (R && bits) stage[v - share.v0] = only_allowed(share, v, stage[v - share.v0], bits);
+        float f[E];
+        get(v, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
+    }
+    const float warp_most = warp_max(most), warp_least = warp_min(most);
+    if (size > 1) cluster_wait();
+    auto tell = [&](int buffer, u64 a, u64 b) {
+        if (lane < (int)size) peer_store(peer_addr(shared_addr(&ex.word[buffer][rank * kWarps + warp][0]), lane), a, b);
+        cluster_sync(size);
+    };
+    tell(0, __float_as_uint(warp_most), __float_as_uint(warp_least));
+    float least = __uint_as_float(0x7f800000u);
+    most = neg_inf();
+    for (int i = lane; i < (int)size * kWarps; i += 32) {
+        most = fmaxf(most, __uint_as_float((unsigned)ex.word[0][i][0]));
+        least = fminf(least, __uint_as_float((unsigned)ex.word[0][i][1]));
+    }
+    most = warp_max(most), least = warp_min(least);
+    if (most == neg_inf()) { /* nothing may be drawn: the same in every block of the row */
+        if (rank == 0 && threadIdx.x == 0) {
+            p.token[row] = -1;
+            if (p.logprob) p.logprob[row] = neg_inf();
+        }
+        return;
+    }
+    const Scale scale{most, 1.4426950408889634 / (double)temperature};
+
+    /* the border of what is kept, beginning with every entry above -inf */
+    Border border{key_of(neg_inf()), 0, 0};
+    unsigned spare = 0;
+    bool cut = false;
+    if (k == 1) {
+        border = Border{key_of(most), 1, 1};
+    } else {
+        if (k > 0 && k < p.in.cols) {
+            const float from = k <= (int)size * kThreads ? least : neg_inf();
+            border = find_border<T, R, false>(share, get, lv, size, key_of(from), key_of(most), (u64)k, scale, 0.0, 0, 0);
+            spare = border.equals - border.ties;
+            cut = true;
+        }
+        if (top_p < 1.0f) {
+            u64 total = 0;
+            unsigned from = border.key;
+            if (!cut) {
+                u64 mine = 0;
+                for (int v = share.first; v < share.last; v += 32) {
+                    float f[E];
+                    get(v, f);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) mine += scale.weight(f[i]);
+                }
+                tell(1, warp_sum(mine), 0);
+                for (int i = lane; i < (int)size * kWarps; i += 32) total += ex.word[1][i][0];
+                total = warp_sum(total);
+                /* entries so far below the maximum that all of them together weigh less than what is cut off */
+                const double left = 1.0 - (double)top_p;
+                const double low = (double)most - (log((double)p.in.cols / left) + 1.0) * (double)temperature;
+                if (left > 1e-5 && low > -3.0e38) from = key_of(__double2float_rd(low));
+            }
+            const Border b = find_border<T, R, true>(share, get, lv, size, from, key_of(most), 0, scale, top_p > 0.0f ? (double)top_p : 0.0,
+                                                     total, spare);
+            if (b.ties != 0xffffffffu) border = b;
+        }
+        if (min_p > 0.0f) {
+            /* the lowest value whose share is min_p of the maximum's */
+            const double low = (double)most + log(fmin((double)min_p, 1.0)) * (double)temperature;
+            const unsigned below = key_of(low > -3.0e38 ? __double2float_ru(low) : neg_inf()) - 1u;
+            if (below >= border.key) border = Border{below, 0, 0};
+        }
+    }
+
+    /* weight above the border and number of entries on it, by warp; every warp then knows what precedes it */
+    u64 mass = 0;
+    unsigned ties = 0;
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        get(v, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const unsigned key = key_of(f[i]);
+            if (key > border.key) mass += scale.weight(f[i]);
+            ties += key == border.key;
+        }
+    }
+    mass = warp_sum(mass);
+    ties = warp_sum(ties);
+    tell(2, mass, ties);
+    const u64 tie_weight = border.ties ? scale.weight(value_of(border.key)) : 0;
+    const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
+    u64 total = 0, before = 0;
+    unsigned ties_seen = 0, ties_before = 0, quota = 0;
+    for (int i0 = 0; i0 < nwarps; i0 += 32) {
+        const int i = i0 + lane;
+        const u64 m = i < nwarps ? ex.word[2][i][0] : 0;
+        const unsigned n = i < nwarps ? (unsigned)ex.word[2][i][1] : 0;
+        const unsigned upto = ties_seen + warp_scan(n);
+        const unsigned kept = min(upto, border.ties) - min(upto - n, border.ties);
+        const u64 w = m + kept * tie_weight;
+        const u64 sum = total + warp_scan(w);
+        if (i == self) before = sum - w, ties_before = upto - n, quota = kept;
+        total = __shfl_sync(~0u, sum, 31);
+        ties_seen = __shfl_sync(~0u, upto, 31);
+    }
+    before = __shfl_sync(~0u, before, self & 31);
+    quota = __shfl_sync(~0u, quota, self & 31);
+    const u64 here = mass + quota * tie_weight;
+    /* the first entry whose running sum exceeds uniform * total */
+    const double want = floor((double)uniform * (double)total);
+    const u64 target = want > 0.0 ? min((u64)want, total - 1) : 0;
+    if (!(before <= target && target < before + here)) return;
+
+    unsigned left = quota;
+    u64 sum = before;
+    const int base = share.first - lane;
+    for (int v0 = base; v0 < share.last; v0 += 32) {
+        const int v = v0 + lane;
+        float f[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = neg_inf();
+        if (v < share.last) get(v, f);
+        unsigned n = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) n += key_of(f[i]) == border.key && v < share.last;
+        const unsigned upto = warp_scan(n);
+        unsigned may = left > upto - n ? left - (upto - n) : 0;
+        u64 w[E], mine = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const unsigned key = key_of(f[i]);
+            w[i] = 0;
+            if (key > border.key) {
+                w[i] = scale.weight(f[i]);
+            } else if (key == border.key && may) {
+                w[i] = tie_weight;
+                --may;
+            }
+            mine += w[i];
+        }
+        const u64 reach = sum + warp_scan(mine);
+        const unsigned hit = __ballot_sync(~0u, target < reach);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                u64 c = reach - mine;
+                int at = 0;
+                float value = 0.0f;
+                bool done = false;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    c += w[i];
+                    if (!done && target < c) at = share.entry(v) + i, value = f[i], done = true;
+                }
+                p.token[row] = at;
+                if (p.logprob) {
+                    const double share_log = value == most ? 0.0 : ((double)value - (double)most) / (double)temperature;
+                    p.logprob[row] = (float)(share_log - log((double)total * (1.0 / (double)(1ull << kUnitLog2))));
+                }
+            }
+            return;
+        }
+        sum = __shfl_sync(~0u, reach, 31);
+        const unsigned took = __shfl_sync(~0u, upto, 31);
+        left = left > took ? left - took : 0;
+    }
+}
+
+/* ---------------------------------------------------------- best entries */
+struct TopParams {
+    RowsIn in;
+    void *values;
+    int *index;
+    float *lse;
+    double temperature;
+    int k;
+};
+
+template <class T, bool R> __global__ void __launch_bounds__(kThreads) top_rows(const TopParams p) {
+    constexpr int E = Elem<T>::E;
+    extern __shared__ uint4 stage[];
+    __shared__ Exchange ex;
+    __shared__ union {
+        Level lv;
+        u64 list[kMaxK]; /* of the first block of the row: key of the value, and 2^32 - 1 - index, so that larger comes first */
+    } sh;
+    __shared__ unsigned taken;
+    const unsigned size = cluster_size(), rank = cluster_rank();
+    const long long row = blockIdx.x / size;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (size > 1) cluster_arrive();
+
+    Share<T, R> share;
+    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    share.fetch();
+    if (threadIdx.x == 0) taken = 0;
+    share.wait();
+    auto get = [&](int v, float *f) {
+        Elem<T>::unpack(share.get(v), f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = not_nan(f[i]);
+    };
+    float most = neg_inf();
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        get(v, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
+    }
+    const float warp_most = warp_max(most), warp_least = warp_min(most);
+    if (size > 1) cluster_wait();
+    auto tell = [&](int buffer, u64 a, u64 b) {
+        if (lane < (int)size) peer_store(peer_addr(shared_addr(&ex.word[buffer][rank * kWarps + warp][0]), lane), a, b);
+        cluster_sync(size);
+    };
+    tell(0, __float_as_uint(warp_most), __float_as_uint(warp_least));
+    float least = __uint_as_float(0x7f800000u);
+    most = neg_inf();
+    for (int i = lane; i < (int)size * kWarps; i += 32) {
+        most = fmaxf(most, __uint_as_float((unsigned)ex.word[0][i][0]));
+        least = fminf(least, __uint_as_float((unsigned)ex.word[0][i][1]));
+    }
+    most = warp_max(most), least = warp_min(least);
+    if (most == neg_inf()) {
+        if (rank == 0) {
+            for (int i = threadIdx.x; i < p.k; i += kThreads) {
+                static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(neg_inf());
+                p.index[row * p.k + i] = -1;
+            }
+            if (p.lse && threadIdx.x == 0) p.lse[row] = neg_inf();
+        }
+        return;
+    }
+    const float from = p.k <= (int)size * kThreads ? least : neg_inf();
+    const Scale scale{most, 0.0};
+    const Border border = find_border<T, R, false>(share, get, sh.lv, size, key_of(from), key_of(most), (u64)p.k, scale, 0.0, 0, 0);
+
+    /* entries on the border and the sum of exponentials, by warp */
+    const float c = (float)(1.4426950408889634 / p.temperature);
+    unsigned ties = 0;
+    float sum = 0.0f;
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        get(v, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            ties += key_of(f[i]) == border.key;
+            if (p.lse) sum += f[i] == most ? 1.0f : exp2f((f[i] - most) * c);
+        }
+    }
+    ties = warp_sum(ties);
+    tell(1, ties, (u64)__double_as_longlong(warp_sum((double)sum)));
+    double all = 0.0;
+    unsigned quota = 0, seen = 0;
+    const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
+    for (int i0 = 0; i0 < nwarps; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned n = i < nwarps ? (unsigned)ex.word[1][i][0] : 0;
+        const unsigned upto = seen + warp_scan(n);
+        if (i == self) quota = min(upto, border.ties) - min(upto - n, border.ties);
+        seen = __shfl_sync(~0u, upto, 31);
+        if (i < nwarps) all += __longlong_as_double((long long)ex.word[1][i][1]);
+    }
+    quota = __shfl_sync(~0u, quota, self & 31);
+    all = warp_sum(all);
+    if (p.lse && rank == 0 && threadIdx.x == 0) p.lse[row] = (float)((double)most / p.temperature + log(all));
+
+    /* what is above the border, and the first of what is on it, goes to the first block of the row */
+    const unsigned lowest = key_of(neg_inf()), list = peer_addr(shared_addr(sh.list), 0), count = peer_addr(shared_addr(&taken), 0);
+    for (int v0 = share.first - lane; v0 < share.last; v0 += 32) {
+        const int v = v0 + lane;
+        float f[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = neg_inf();
+        if (v < share.last) get(v, f);
+        unsigned on = 0, above = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const unsigned key = key_of(f[i]);
+            if (key > lowest && v < share.last) on |= (unsigned)(key == border.key) << i, above |= (unsigned)(key > border.key) << i;
+        }
+        if (!__any_sync(~0u, on | above)) continue;
+        const unsigned n = __popc(on), upto = warp_scan(n);
+        unsigned may = quota > upto - n ? quota - (upto - n) : 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            bool take = (above >> i) & 1u;
+            if (((on >> i) & 1u) && may) take = true, --may;
+            if (take) {
+                const unsigned at = peer_count(count, 1);
+                if (at < (unsigned)p.k) peer_store1(list + at * 8, (u64)key_of(f[i]) << 32 | (0xffffffffu - (unsigned)(share.entry(v) + i)));
+            }
+        }
+        const unsigned took = __shfl_sync(~0u, upto, 31);
+        quota = quota > took ? quota - took : 0;
+    }
+    cluster_sync(size);
+    if (rank != 0) return;
+
+    /* bitonic sort of the next power of two, largest first; unused places hold 0, below every entry */
+    int m = 32;
+    while (m < p.k) m *= 2;
+    for (int i = (int)taken + threadIdx.x; i < m; i += kThreads) sh.list[i] = 0;
+    for (int len = 2; len <= m; len *= 2)
+        for (int d = len / 2; d; d /= 2) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < m / 2; i += kThreads) {
+                const int a = (i / d) * 2 * d + i % d, b = a + d;
+                const u64 u = sh.list[a], w = sh.list[b];
+                if ((u < w) == ((a & len) == 0)) sh.list[a] = w, sh.list[b] = u;
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.k; i += kThreads) {
+        const u64 e = sh.list[i];
+        static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(e ? value_of((unsigned)(e >> 32)) : neg_inf());
+        p.index[row * p.k + i] = e ? (int)(0xffffffffu - (unsigned)e) : -1;
+    }
+}
+
+/* ---------------------------------------------------------- distillation */
+struct DistillParams {
+    RowsIn in;
+    const void *teacher; /* rows x k, element type teacher_type */
+    const int *index;
+    const float *teacher_lse, *weight, *upstream;
+    float *loss, *stats; /* stats: rows x 4, see accb_distill_rows */
+    void *grad;          /* element type of the scores */
+    long long grad_pitch;
+    double temperature;
+    int k, teacher_type;
+    int map_words; /* 32-bit words of the map of named entries of a block's share */
+};
+
+__device__ __forceinline__ float teacher_value(const DistillParams &p, long long i) {
+    if (p.teacher_type == ACCB_ROWS_F32) return static_cast<const float *>(p.teacher)[i];
+    if (p.teacher_type == ACCB_ROWS_F16) return __half2float(static_cast<const __half *>(p.teacher)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p.teacher)[i]);
+}
+
+__device__ __forceinline__ double block_sum(double v, double *scratch) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int w = 0; w < kWarps; ++w) s += scratch[w];
+    return s;
+}
+__device__ __forceinline__ float block_max(float v, double *scratch) {
+    v = warp_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double s = scratch[0];
+    for (int w = 1; w < kWarps; ++w) s = fmax(s, scratch[w]);
+    return (float)s;
+}
+
+/* What a row's teacher says, the same in every block of the row.  Thread t holds entries t, t + 256, ... */
+struct Teacher {
+    static constexpr int M = kMaxK / kThreads;
+    int at[M];       /* index of the entry, -1 for one that says nothing */
+    double logp[M];
+    double p[M];
+    double named;    /* sum of p */
+    bool any;
+    __device__ __forceinline__ void read(const DistillParams &q, long long row, double *scratch) {
+        const double inv = 1.0 / q.temperature;
+        float z[M], top = neg_inf();
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int j = threadIdx.x + i * kThreads;
+            at[i] = -1;
+            z[i] = neg_inf();
+            if (j < q.k) {
+                const int e = q.index[row * q.k + j];
+                const float v = teacher_value(q, row * q.k + j);
+                if (e >= 0 && e < q.in.cols && v > neg_inf()) at[i] = e, z[i] = v;
+            }
+            top = fmaxf(top, z[i]);
+        }
+        top = block_max(top, scratch);
+        any = top > neg_inf();
+        double norm;
+        if (q.teacher_lse) {
+            norm = (double)q.teacher_lse[row];
+        } else {
+            double s = 0.0;
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+                if (at[i] >= 0) s += exp(((double)z[i] - (double)top) * inv);
+            norm = (double)top * inv + log(block_sum(s, scratch));
+        }
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            logp[i] = (double)z[i] * inv - norm;
+            p[i] = at[i] >= 0 ? exp(logp[i]) : 0.0;
+            s += p[i];
+        }
+        named = block_sum(s, scratch);
+    }
+};
+
+/* gradient vectors: 16-byte stores where gradient and scores start at the same place of a 16-byte word */
+template <class T, bool R> __device__ __forceinline__ void put(const Share<T, R> &share, T *grad, bool same, int v, const float *d) {
+    constexpr int E = Elem<T>::E;
+    T *to = grad + share.entry(v);
+    if (same && share.whole(v)) {
+        *reinterpret_cast<uint4 *>(to) = Elem<T>::pack(d);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (share.entry(v) + i >= 0 && share.entry(v) + i < share.n) to[i] = Elem<T>::down(d[i]);
+    }
+}
+
+/* A (maximum, sum of exponentials below it) pair; the sum of two is taken at the larger maximum. */
+struct LogSum {
+    float top;
+    double sum;
+    __device__ __forceinline__ void add(float t, double s, double c) {
+        if (t == neg_inf() && s == 0.0) return; /* no entry; -inf with another sum: entries that are NaN */
+        if (top == neg_inf()) {
+            top = t, sum = s;
+        } else if (t <= top) {
+            sum += s * exp2(((double)t - (double)top) * c);
+        } else {
+            sum = sum * exp2(((double)top - (double)t) * c) + s;
+            top = t;
+        }
+    }
+};
+
+/* BACKWARD: the statistics are given, and no block needs the others. */
+template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads) distill_rows(const DistillParams p) {
+    constexpr int E = Elem<T>::E;
+    extern __shared__ uint4 dynamic[];
+    __shared__ double scratch[kWarps];
+    __shared__ Exchange ex;
+    __shared__ int twice;
+    unsigned *map = reinterpret_cast<unsigned *>(dynamic);
+    float *named_p = reinterpret_cast<float *>(map + p.map_words);
+    int *named_at = reinterpret_cast<int *>(named_p + kMaxK);
+    uint4 *stage = dynamic + (p.map_words + 2 * kMaxK) / 4;
+    const unsigned size = cluster_size(), rank = cluster_rank();
+    const long long row = blockIdx.x / size;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    Share<T, R> share;
+    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    T *grad = p.grad ? static_cast<T *>(p.grad) + row * p.grad_pitch : nullptr;
+    const bool same = grad && (((reinterpret_cast<unsigned long long>(grad) ^ (reinterpret_cast<unsigned long long>(share.base) + share.lead * sizeof(T))) & 15u) == 0);
+    const float weight = p.weight ? p.weight[row] : 1.0f;
+    float st[4];
+    if (BACKWARD)
+        for (int i = 0; i < 4; ++i) st[i] = p.stats[row * 4 + i];
+    bool live = BACKWARD ? weight != 0.0f && st[1] != 0.0f : weight != 0.0f;
+    if (live) share.fetch();
+    if (!BACKWARD && size > 1) cluster_arrive();
+
+    Teacher teacher;
+    if (live) {
+        teacher.read(p, row, scratch);
+        live = teacher.any;
+    }
+    /* rows that do not count: nothing of the scores is looked at */
+    auto nothing = [&] {
+        share.wait();
+        if (grad) {
+            float d[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) d[i] = 0.0f;
+            for (int v = share.first; v < share.last; v += 32) put(share, grad, same, v, d);
+        }
+        if (!BACKWARD && rank == 0 && threadIdx.x < 4) {
+            if (threadIdx.x == 0) p.loss[row] = 0.0f;
+            if (p.stats) p.stats[row * 4 + threadIdx.x] = 0.0f;
+        }
+    };
+    if (!live) {
+        if (!BACKWARD && size > 1) cluster_wait();
+        nothing();
+        return;
+    }
+
+    /* which entries of the share the teacher names; an entry named twice is counted once */
+    const int origin = share.entry(share.v0), width = (share.v1 - share.v0) * E;
+    for (int i = threadIdx.x; i < p.map_words; i += kThreads) map[i] = 0;
+    if (threadIdx.x == 0) twice = 0;
+    share.wait();
+    __syncthreads();
+    const float c = (float)(1.4426950408889634 / p.temperature);
+    const double cd = 1.4426950408889634 / p.temperature;
+    float z[Teacher::M];
+    bool counts[Teacher::M], first[Teacher::M]; /* in this share; the first of its index */
+#pragma unroll
+    for (int i = 0; i < Teacher::M; ++i) {
+        const int e = teacher.at[i] - origin;
+        counts[i] = teacher.at[i] >= 0 && e >= 0 && e < width;
+        first[i] = false;
+        z[i] = neg_inf();
+        const int j = threadIdx.x + i * kThreads;
+        if (j < p.k) named_at[j] = counts[i] ? teacher.at[i] : -1, named_p[j] = (float)teacher.p[i];
+        if (counts[i]) {
+            first[i] = !((atomicOr(&map[e >> 5], 1u << (e & 31)) >> (e & 31)) & 1u);
+            if (!first[i]) twice = 1;
+            z[i] = R ? Elem<T>::up(reinterpret_cast<const T *>(stage)[e]) : Elem<T>::up(share.base[share.lead + teacher.at[i]]);
+        }
+    }
+    __syncthreads();
+
+    float top, inverse, at_named, elsewhere;
+    if (!BACKWARD) {
+        /* the rest of the row (all of it without teacher_lse) and the named entries, each as maximum and sum */
+        const bool rest = p.teacher_lse != nullptr;
+        float most = neg_inf(), most_named = neg_inf();
+        auto get = [&](int v, float *f) {
+            Elem<T>::unpack(share.get(v), f);
+            if (rest) {
+                const int e = (v - share.v0) * E;
+                const unsigned m = map[e >> 5] >> (e & 31);
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if ((m >> i) & 1u) f[i] = neg_inf();
+            }
+        };
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
+        }
+        most = warp_max(most);
+        const float base = most > neg_inf() ? most : 0.0f;
+        float sum = 0.0f;
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum += exp2f((f[i] - base) * c);
+        }
+        double named_sum = 0.0, cross = 0.0;
+        if (rest) {
+#pragma unroll
+            for (int i = 0; i < Teacher::M; ++i)
+                if (first[i]) most_named = fmaxf(most_named, z[i]);
+            most_named = warp_max(most_named);
+            const float named_base = most_named > neg_inf() ? most_named : 0.0f;
+#pragma unroll
+            for (int i = 0; i < Teacher::M; ++i)
+                if (first[i]) named_sum += exp2(((double)z[i] - (double)named_base) * cd);
+        }
+        /* sum of p (log p - z / tau): what is left of the loss is the student's log-sum-exp */
+#pragma unroll
+        for (int i = 0; i < Teacher::M; ++i)
+            if (counts[i] && teacher.p[i] > 0.0) cross += teacher.p[i] * (teacher.logp[i] - (double)z[i] / p.temperature);
+        const double s0 = warp_sum((double)sum), s1 = warp_sum(named_sum), s2 = warp_sum(cross);
+        if (size > 1) cluster_wait();
+        if (lane < (int)size) {
+            const unsigned to = peer_addr(shared_addr(&ex.word[0][rank * kWarps + warp][0]), lane);
+            peer_store(to, __double_as_longlong(s0), __double_as_longlong(s1));
+            peer_store(to + 16, __double_as_longlong(s2), (u64)__float_as_uint(most) << 32 | __float_as_uint(most_named));
+        }
+        cluster_sync(size);
+        LogSum others{neg_inf(), 0.0}, all{neg_inf(), 0.0};
+        cross = 0.0;
+        for (int i = 0; i < (int)size * kWarps; ++i) {
+            const u64 *w = ex.word[0][i];
+            others.add(__uint_as_float((unsigned)(w[3] >> 32)), __longlong_as_double((long long)w[0]), cd);
+            all.add(__uint_as_float((unsigned)w[3]), __longlong_as_double((long long)w[1]), cd);
+            cross += __longlong_as_double((long long)w[2]);
+        }
+        all.add(others.top, others.sum, cd);
+        if (all.top == neg_inf() && all.sum == 0.0) { /* the student excludes every entry: the same in every block of the row */
+            nothing();
+            return;
+        }
+        const double lse = (double)all.top / p.temperature + log(all.sum);
+        double loss = cross + teacher.named * lse, factor = teacher.named, other = teacher.named;
+        if (rest) {
+            const double r = 1.0 - teacher.named;
+            if (r > 0.0 && others.top > neg_inf()) {
+                const double log_share = (double)others.top / p.temperature + log(others.sum) - lse;
+                loss += r * (log(r) - log_share);
+                factor += r;
+                other = factor - r * exp(-log_share);
+            }
+        }
+        top = all.top, inverse = (float)(1.0 / all.sum), at_named = (float)factor, elsewhere = (float)other;
+        if (rank == 0 && threadIdx.x == 0) {
+            p.loss[row] = weight * (float)loss;
+            if (p.stats) {
+                float *s = p.stats + row * 4;
+                s[0] = top, s[1] = inverse, s[2] = at_named, s[3] = elsewhere;
+            }
+        }
+        if (!grad) return;
+    } else {
+        top = st[0], inverse = st[1], at_named = st[2], elsewhere = st[3];
+    }
+
+    /* gradient: elsewhere * q everywhere, then the named entries once more with their own value */
+    float g = (float)((double)weight / p.temperature);
+    if (BACKWARD && p.upstream) g *= p.upstream[row];
+    const float factor = g * elsewhere * inverse;
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        Elem<T>::unpack(share.get(v), f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = factor * exp2f((f[i] - top) * c);
+        put(share, grad, same, v, f);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Teacher::M; ++i) {
+        if (!counts[i]) continue;
+        double named = teacher.p[i];
+        if (twice) { /* the first entry of an index in the list writes the sum of all of them, in the list's order */
+            const int j = threadIdx.x + i * kThreads;
+            bool earlier = false;
+            named = 0.0;
+            for (int o = 0; o < p.k; ++o)
+                if (named_at[o] == teacher.at[i]) {
+                    if (o < j) earlier = true;
+                    named += (double)named_p[o];
+                }
+            if (earlier) continue;
+        }
+        const float q = inverse * exp2f((z[i] - top) * c);
+        grad[teacher.at[i]] = Elem<T>::down(g * (float)((double)at_named * q - named));
+    }
+}
+
+/* ----------------------------------------------------------------- host */
+constexpr size_t kSharedMost = 200u << 10; /* dynamic shared memory a block may ask for (227 KB less what it declares) */
+constexpr long long kShareBytes = 64 << 10; /* the share of a row a block aims to hold */
+
+/* Blocks per row: as few as hold the row in shares of 64 KB (two or three blocks of an SM then overlap one another's
+ * phases), more while rows are too few to give every SM a block, as long as a share stays worth a block. */
+static int cluster_for(long long rows, long long row_bytes, int sm_count) {
+    int size = 1;
+    while (size < kMaxCluster && row_bytes > kShareBytes * size) size *= 2;
+    while (size < kMaxCluster && rows * size < sm_count && row_bytes > (8 << 10) * size) size *= 2;
+    return size;
+}
+
+}  // namespace accb_rows
+
+using namespace accb_rt;
+using namespace accb_rows;
+
+#define LOCK(ctx)                                                   \
+    if (!(ctx)) return fail(nullptr, ACCB_EINVAL, "null context"); \
+    std::lock_guard<std::recursive_mutex> lock_((ctx)->mu);         \
+    CtxGuard guard_(ctx)
+#define TRY(expr)                     \
+    do {                              \
+        int st_ = (expr);             \
+        if (st_ != ACCB_OK) return st_; \
+    } while (0)
+
+static size_t size_of(int type) { return type == ACCB_ROWS_F32 ? 4 : 2; }
+
+static int check_rows(accb_context *ctx, const accb_rows_array *a, const char *what) {
+    if (!a) return fail(ctx, ACCB_EINVAL, "%s: null array", what);
+    if (a->type != ACCB_ROWS_F32 && a->type != ACCB_ROWS_F16 && a->type != ACCB_ROWS_BF16)
+        return fail(ctx, ACCB_EINVAL, "%s: unknown element type %d", what, a->type);
+    if (a->rows < 0 || a->rows > 0x7fffffffLL / kMaxCluster) return fail(ctx, ACCB_EINVAL, "%s: bad number of rows %lld", what, a->rows);
+    if (a->cols < 1) return fail(ctx, ACCB_EBOUNDS, "%s: rows without entries", what);
+    if (a->cols > kMaxCols) return fail(ctx, ACCB_EINVAL, "%s: rows of %d entries (at most %lld)", what, a->cols, kMaxCols);
+    if (a->rows > 1 && a->pitch < a->cols) return fail(ctx, ACCB_EINVAL, "%s: rows of %d entries every %lld entries overlap", what, a->cols, a->pitch);
+    if (a->rows > 0 && a->pitch > (1LL << 62) / (a->rows * 4)) return fail(ctx, ACCB_EINVAL, "%s: row pitch %lld too large", what, a->pitch);
+    if (a->rows > 0 && !a->ptr) return fail(ctx, ACCB_EINVAL, "%s: null pointer", what);
+    if (reinterpret_cast<uintptr_t>(a->ptr) % size_of(a->type)) return fail(ctx, ACCB_EINVAL, "%s: misaligned pointer", what);
+    return ACCB_OK;
+}
+
+static RowsIn rows_in(const accb_rows_array *a) { return RowsIn{a->ptr, a->rows, a->pitch, a->cols}; }
+
+/* one launch with `size` blocks per row; `fixed` bytes of dynamic shared memory besides the share */
+template <class P>
+static int launch_rows(accb_context *ctx, void (*resident)(const P), void (*streaming)(const P), const P &p, const accb_rows_array *a, int size,
+                       size_t fixed, cudaStream_t stream, const char *name) {
+    const long long per16 = 16 / (long long)size_of(a->type);
+    const long long nvec = (a->cols + 2 * per16 - 2) / per16; /* of the worst placed row */
+    const size_t share = (size_t)((nvec + size - 1) / size) * 16;
+    const bool fits = fixed + share <= kSharedMost;
+    void (*kernel)(const P) = fits ? resident : streaming;
+    const size_t smem = fixed + (fits ? share : 0);
+    if (!std::count(ctx->rows_ready, ctx->rows_ready + ctx->rows_ready_count, (const void *)kernel)) {
+        int st = check_cuda(ctx, cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedMost), name);
+        if (st == ACCB_OK)
+            st = check_cuda(ctx, cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100), name);
+        if (st != ACCB_OK) return st;
+        ctx->rows_ready[ctx->rows_ready_count++] = (const void *)kernel;
+    }
+    if (ctx->trace_exec)
+        fprintf(stderr, "[accb exec] %s<<<%lld,%d,%zu>>> rows=%lld cols=%d\n", name, a->rows * size, kThreads, smem, a->rows, a->cols);
+    cudaLaunchAttribute attr;
+    memset(&attr, 0, sizeof attr);
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3((unsigned)(a->rows * size));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    void *args[] = {const_cast<P *>(&p)};
+    const int st = check_cuda(ctx, cudaLaunchKernelExC(&cfg, (const void *)kernel, args), name);
+    if (st == ACCB_OK) ctx->launches++;
+    return st;
+}
+
+#define BY_TYPE(type, call)                                        \
+    ((type) == ACCB_ROWS_F32   ? call(float)                       \
+     : (type) == ACCB_ROWS_F16 ? call(__half)                      \
+                               : call(__nv_bfloat16))
+
+extern "C" {
+
+int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *x, double temperature, int k, void *values, int32_t *index,
+                  float *lse) {
+    LOCK(ctx);
+    TRY(check_rows(ctx, x, "top_rows"));
+    if (k < 1 || k > kMaxK || k > x->cols) return fail(ctx, ACCB_EINVAL, "top_rows: %d entries of rows of %d (at most %d)", k, x->cols, kMaxK);
+    if (!(temperature > 1e-30) || temperature > 1e30) return fail(ctx, ACCB_EINVAL, "top_rows: bad temperature %g", temperature);
+    if (x->rows == 0) return ACCB_OK;
+    if (!values || !index) return fail(ctx, ACCB_EINVAL, "top_rows: null result");
+    const TopParams p{rows_in(x), values, index, lse, temperature, k};
+    const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
+#define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, 0, (cudaStream_t)stream, "top_rows")
+    return BY_TYPE(x->type, CALL);
+#undef CALL
+}
+
+int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *x, const uint32_t *allowed, long long allowed_pitch,
+                     const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                     int32_t *token, float *logprob) {
+    LOCK(ctx);
+    TRY(check_rows(ctx, x, "sample_rows"));
+    if (allowed && allowed_pitch < (x->cols + 31) / 32)
+        return fail(ctx, ACCB_EINVAL, "sample_rows: %lld words of allowed bits for rows of %d entries", allowed_pitch, x->cols);
+    if (x->rows == 0) return ACCB_OK;
+    if (!uniform || !token) return fail(ctx, ACCB_EINVAL, "sample_rows: null random numbers or result");
+    const SampleParams p{rows_in(x), allowed, allowed_pitch, uniform, temperature, top_p, min_p, top_k, token, logprob};
+    const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
+#define CALL(T) launch_rows(ctx, sample_rows<T, true>, sample_rows<T, false>, p, x, size, 0, (cudaStream_t)stream, "sample_rows")
+    return BY_TYPE(x->type, CALL);
+#undef CALL
+}
+
+static int distill(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const accb_rows_array *grad, DistillParams &p,
+                   bool backward) {
+    const char *what = backward ? "distill_rows_backward" : "distill_rows";
+    TRY(check_rows(ctx, student, what));
+    if (p.k < 1 || p.k > kMaxK) return fail(ctx, ACCB_EINVAL, "%s: %d entries of the teacher (1 to %d)", what, p.k, kMaxK);
+    if (p.teacher_type != ACCB_ROWS_F32 && p.teacher_type != ACCB_ROWS_F16 && p.teacher_type != ACCB_ROWS_BF16)
+        return fail(ctx, ACCB_EINVAL, "%s: unknown element type %d of the teacher", what, p.teacher_type);
+    if (!(p.temperature > 1e-30) || p.temperature > 1e30) return fail(ctx, ACCB_EINVAL, "%s: bad temperature %g", what, p.temperature);
+    if (grad) {
+        TRY(check_rows(ctx, grad, what));
+        if (grad->rows != student->rows || grad->cols != student->cols || grad->type != student->type)
+            return fail(ctx, ACCB_EINVAL, "%s: the gradient has another shape or type than the scores", what);
+        p.grad = grad->ptr;
+        p.grad_pitch = grad->pitch;
+    }
+    if (student->rows == 0) return ACCB_OK;
+    if (!p.teacher || !p.index) return fail(ctx, ACCB_EINVAL, "%s: null teacher", what);
+    if (backward ? !p.stats || !grad : !p.loss) return fail(ctx, ACCB_EINVAL, "%s: null result or statistics", what);
+    p.in = rows_in(student);
+    const int size = cluster_for(student->rows, (long long)student->cols * size_of(student->type), ctx->sm_count);
+    const long long e = 16 / (long long)size_of(student->type);
+    const long long share = ((student->cols + 2 * e - 2) / e + size - 1) / size * e; /* entries of a block's share, at most */
+    p.map_words = (int)((share + 31) / 32 + 3) & ~3;
+    const size_t fixed = (size_t)p.map_words * 4 + 8 * kMaxK;
+#define CALL(T)                                                                                                                       \
+    (backward ? launch_rows(ctx, distill_rows<T, true, true>, distill_rows<T, false, true>, p, student, size, fixed, (cudaStream_t)stream, what) \
+              : launch_rows(ctx, distill_rows<T, true, false>, distill_rows<T, false, false>, p, student, size, fixed, (cudaStream_t)stream, what))
+    return BY_TYPE(student->type, CALL);
+#undef CALL
+}
+
+int accb_distill_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const void *teacher, int teacher_type,
+                      const int32_t *index, int k, const float *teacher_lse, const float *weight, double temperature, float *loss,
+                      float *stats, const accb_rows_array *grad) {
+    LOCK(ctx);
+    DistillParams p;
+    memset(&p, 0, sizeof p);
+    p.teacher = teacher, p.index = index, p.teacher_lse = teacher_lse, p.weight = weight;
+    p.loss = loss, p.stats = stats, p.temperature = temperature, p.k = k, p.teacher_type = teacher_type;
+    return distill(ctx, stream, student, grad, p, false);
+}
+
+int accb_distill_rows_backward(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const void *teacher,
+                               int teacher_type, const int32_t *index, int k, const float *teacher_lse, const float *weight,
+                               double temperature, const float *stats, const float *upstream, const accb_rows_array *grad) {
+    LOCK(ctx);
+    DistillParams p;
+    memset(&p, 0, sizeof p);
+    p.teacher = teacher, p.index = index, p.teacher_lse = teacher_lse, p.weight = weight, p.upstream = upstream;
+    p.stats = const_cast<float *>(stats), p.temperature = temperature, p.k = k, p.teacher_type = teacher_type;
+    return distill(ctx, stream, student, grad, p, true);
+}
+
+} /* extern "C" */

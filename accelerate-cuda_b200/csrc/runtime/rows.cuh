@@ -1,0 +1,397 @@
+/*
+ * rows.cuh -- what the operators over rows of scores (rows.cu) share: a row
+ * held on chip by a cluster of blocks, exchanges between its warps, and the
+ * search for the border of a row's best entries.
+ *
+ * A row of scores is longer than what the folds over rows see (10^4 to 10^6
+ * entries) and has to be looked at several times: for its maximum, its sum of
+ * exponentials, the value of its k-th entry, and once more for what is written.
+ * So a row belongs to a cluster of 1 to 8 blocks.  Every block copies its
+ * share of the row to shared memory once (cp.async, 16 bytes a thread), all
+ * passes read that copy, and the blocks tell one another what they found
+ * through distributed shared memory.  HBM sees the row once.  No scratch
+ * memory is used at all: launches on different streams or in captured graphs
+ * share nothing.
+ *
+ * Inside a block every warp owns a contiguous piece of the share, so that
+ * sums over warps in order are sums over the row in order; a thread reads the
+ * same vectors in every pass, which makes its own copies visible to it
+ * without a barrier.
+ *
+ * accelerate-cuda has no counterpart: its folds reduce a row with one block in
+ * one pass (Data/Array/Accelerate/CUDA/CodeGen/Reduction.hs:221-367).
+ */
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace accb_rows {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kBins = 4 * kThreads;    /* bins of one level of the border search: four per thread */
+constexpr int kMaxK = 1024;            /* most entries of a top list */
+constexpr long long kMaxCols = 1 << 20;
+
+typedef unsigned long long u64;
+
+/* ------------------------------------------------------- element types */
+template <class T> struct Elem;
+template <> struct Elem<float> {
+    static constexpr int E = 4;
+    static constexpr int kShift = 0; /* low bits of key_of() that never tell two values apart */
+    static constexpr unsigned kLowest = 0xff800000u; /* -inf, as often as it fits into 32 bits */
+    static __device__ __forceinline__ void unpack(const uint4 &w, float *f) {
+        f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float *f) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct Elem<__half> {
+    static constexpr int E = 8;
+    static constexpr int kShift = 13;
+    static constexpr unsigned kLowest = 0xfc00fc00u;
+    static __device__ __forceinline__ void unpack(const uint4 &w, float *f) {
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float *f) {
+        unsigned u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static constexpr int kShift = 16;
+    static constexpr unsigned kLowest = 0xff80ff80u;
+    static __device__ __forceinline__ void unpack(const uint4 &w, float *f) {
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ uint4 pack(const float *f) {
+        unsigned u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+__device__ __forceinline__ float neg_inf() { return __uint_as_float(0xff800000u); }
+/* a NaN is an entry that cannot be chosen, like -inf (fmaxf returns the operand that is a number) */
+__device__ __forceinline__ float not_nan(float f) { return fmaxf(f, neg_inf()); }
+
+/* unsigned keys in the order of the values; -0 and +0 are equal */
+__device__ __forceinline__ unsigned key_of(float f) {
+    const unsigned b = __float_as_uint(f + 0.0f);
+    return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); }
+
+/* ------------------------------------------------------------- clusters */
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync(unsigned size) {
+    if (size == 1) {
+        __syncthreads();
+    } else {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+}
+__device__ __forceinline__ unsigned shared_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+/* the address of this block's shared variable in the block of the given rank */
+__device__ __forceinline__ unsigned peer_addr(unsigned addr, unsigned rank) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void peer_store(unsigned addr, u64 a, u64 b) {
+    asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(addr), "l"(a), "l"(b) : "memory");
+}
+__device__ __forceinline__ void peer_store1(unsigned addr, u64 a) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(a) : "memory");
+}
+__device__ __forceinline__ uint4 peer_load(unsigned addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned peer_count(unsigned addr, unsigned n) {
+    unsigned old;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(n) : "memory");
+    return old;
+}
+
+/* What every warp of a row tells every other: four 64-bit words per warp and exchange.  A kernel uses every buffer
+ * once, so none is overwritten while it is read. */
+struct Exchange {
+    alignas(16) u64 word[3][kMaxCluster * kWarps][4];
+};
+
+/* ----------------------------------------------------------------- rows */
+/* A block's share of one row, in vectors of 16 bytes counted from the row's address rounded down to 16 bytes.
+ * Entries of an edge vector that lie outside the row read as -inf. */
+template <class T, bool RESIDENT> struct Share {
+    static constexpr int E = Elem<T>::E;
+    const T *base;   /* the row's address rounded down to 16 bytes */
+    int lead;        /* entries between base and the row's first */
+    int n;           /* entries of the row */
+    int v0, v1;      /* this block's vectors */
+    int first, last; /* this thread's: first, first + 32, ... below last */
+    uint4 *stage;
+
+    __device__ __forceinline__ void init(const T *row, int cols, unsigned rank, unsigned size, uint4 *smem) {
+        lead = (int)((reinterpret_cast<unsigned long long>(row) & 15u) / sizeof(T));
+        base = row - lead;
+        n = cols;
+        const int nvec = (lead + cols + E - 1) / E;
+        const int per = (nvec + (int)size - 1) / (int)size;
+        v0 = min(nvec, (int)rank * per);
+        v1 = min(nvec, v0 + per);
+        const int piece = ((v1 - v0 + kWarps - 1) / kWarps + 31) & ~31;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        first = v0 + warp * piece + lane;
+        last = min(v1, v0 + (warp + 1) * piece);
+        stage = smem;
+    }
+    __device__ __forceinline__ int entry(int v) const { return v * E - lead; } /* index of a vector's first entry */
+    __device__ __forceinline__ bool whole(int v) const { return entry(v) >= 0 && entry(v) + E <= n; }
+
+    __device__ __forceinline__ uint4 edge(int v) const {
+        uint4 w = make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+        float f[E];
+        Elem<T>::unpack(w, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (entry(v) + i >= 0 && entry(v) + i < n) f[i] = Elem<T>::up(base[(long long)v * E + i]);
+        return Elem<T>::pack(f);
+    }
+    __device__ __forceinline__ uint4 from_memory(int v) const {
+        return whole(v) ? reinterpret_cast<const uint4 *>(base)[v] : edge(v);
+    }
+    /* start the copies of this thread's vectors; wait() before the first get() */
+    __device__ __forceinline__ void fetch() const {
+        if (!RESIDENT) return;
+        for (int v = first; v < last; v += 32) {
+            if (whole(v))
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(stage + (v - v0))),
+                             "l"(reinterpret_cast<const uint4 *>(base) + v)
+                             : "memory");
+            else
+                stage[v - v0] = edge(v);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void wait() const {
+        if (RESIDENT) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __device__ __forceinline__ uint4 get(int v) const { return RESIDENT ? stage[v - v0] : from_memory(v); }
+};
+
+/* --------------------------------------------------------- reductions */
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, d));
+    return v;
+}
+__device__ __forceinline__ float warp_min(float v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = fminf(v, __shfl_xor_sync(~0u, v, d));
+    return v;
+}
+template <class V> __device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+    return v;
+}
+template <class V> __device__ __forceinline__ V warp_scan(V v) { /* inclusive */
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const V o = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+/* ------------------------------------------------- weights and borders */
+/* The share of an entry is exp((x - max) / T).  It is held as a whole number in units of 2^-43, so that sums do not
+ * depend on their order -- on how a row is split over warps and blocks -- and a million entries (kMaxCols) still fit
+ * into 64 bits.  Computed in 64 bits: two indices are told apart by a sum, and an error of 2^-24 in a row of 10^5
+ * like entries would pick the wrong one every few thousand rows. */
+constexpr int kUnitLog2 = 43;
+struct Scale {
+    float top;  /* the row's maximum */
+    double c;   /* log2(e) / T */
+    __device__ __forceinline__ u64 weight(float f) const {
+        if (f == top) return 1ull << kUnitLog2;
+        const double y = ((double)f - (double)top) * c;
+        if (!(y > -(kUnitLog2 + 2.0))) return 0; /* also f = -inf with T = inf, a NaN here */
+        return __double2ull_rn(exp2(y) * (double)(1ull << kUnitLog2));
+    }
+};
+
+/* The best entries of a row, in the order of falling value and, among equals, rising index: every entry whose key is
+ * above `key`, and the first `ties` of those whose key it is. */
+struct Border {
+    unsigned key;
+    unsigned ties;
+    unsigned equals; /* entries with that key */
+};
+
+struct Level { /* one level of the border search */
+    alignas(16) u64 mass[kBins];
+    alignas(16) unsigned count[kBins];
+    u64 warp_total[kWarps], warp_mass[kWarps];
+    u64 before;
+    unsigned bin, bin_count;
+    int found;
+};
+
+/* Finds the border of the shortest run of best entries, among those with klo <= key <= khi (khi >= every key of the
+ * row), that holds `target` entries (BY_MASS false) or the given fraction of a total weight (BY_MASS true; total 0:
+ * what the range holds, less the weight of `spare` entries of key klo).
+ *
+ * Every level lays 1024 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
+ * the border lies and goes on with that bin's range; when a bin is one key, the rest is arithmetic.  For 16-bit
+ * scores one level usually does, for 32-bit ones three.  Bins are summed over the cluster by reading the other
+ * blocks' bins, four per thread; every block does that for itself and so learns the result without another message.
+ * All threads of the cluster call it with the same arguments. */
+template <class T, bool RESIDENT, bool BY_MASS, class Get>
+__device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &lv, unsigned size, unsigned klo, unsigned khi,
+                              u64 target, const Scale &scale, double fraction, u64 total, unsigned spare) {
+    constexpr int E = Elem<T>::E, S0 = Elem<T>::kShift;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const unsigned bottom = klo;
+    bool have_target = !BY_MASS || total != 0;
+    if (BY_MASS && have_target) target = max(1ull, (u64)ceil(fraction * (double)total));
+    for (;;) {
+        const unsigned span = khi - klo;
+        const int shift = max(S0, 22 - __clz(span)); /* span >> shift < 1024 */
+        const bool weigh = BY_MASS && shift > S0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lv.count[t + i * kThreads] = 0, lv.mass[t + i * kThreads] = 0;
+        if (t == 0) lv.found = 0;
+        __syncthreads();
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const unsigned k = key_of(f[i]);
+                if (k - klo <= span) {
+                    const unsigned b = (khi - k) >> shift;
+                    atomicAdd(&lv.count[b], 1u);
+                    if (weigh) atomicAdd(&lv.mass[b], scale.weight(f[i]));
+                }
+            }
+        }
+        cluster_sync(size);
+        unsigned count[4] = {0, 0, 0, 0};
+        u64 mass[4] = {0, 0, 0, 0};
+        for (unsigned r = 0; r < size; ++r) {
+            const uint4 c = peer_load(peer_addr(shared_addr(&lv.count[4 * t]), r));
+            count[0] += c.x, count[1] += c.y, count[2] += c.z, count[3] += c.w;
+            if (weigh) {
+                const uint4 a = peer_load(peer_addr(shared_addr(&lv.mass[4 * t]), r));
+                const uint4 b = peer_load(peer_addr(shared_addr(&lv.mass[4 * t + 2]), r));
+                mass[0] += (u64)a.y << 32 | a.x, mass[1] += (u64)a.w << 32 | a.z;
+                mass[2] += (u64)b.y << 32 | b.x, mass[3] += (u64)b.w << 32 | b.z;
+            }
+        }
+        /* the one key of a bin once a bin is one key: keys of 16-bit types end in zeros above zero and in ones below */
+        auto key_at = [&](unsigned bin) {
+            const unsigned hi = khi - (bin << shift), low = (1u << S0) - 1u;
+            return (hi & 0x80000000u) ? (hi & ~low) : ((hi + 1u) & ~low) - 1u;
+        };
+        u64 sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (BY_MASS && !weigh && count[i]) mass[i] = count[i] * scale.weight(value_of(key_at(4 * t + i)));
+            if (!BY_MASS) mass[i] = count[i];
+            sum += mass[i];
+        }
+        u64 upto = warp_scan(sum);
+        if (lane == 31) lv.warp_total[warp] = upto;
+        __syncthreads();
+        u64 all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) upto += lv.warp_total[w];
+            all += lv.warp_total[w];
+        }
+        if (!have_target) { /* the weight of the range is the total that the fraction is of */
+            all -= spare * scale.weight(value_of(bottom));
+            target = max(1ull, (u64)ceil(fraction * (double)all));
+            have_target = true;
+        }
+        u64 before = upto - sum;
+        if (before < target && target <= upto) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (before < target && target <= before + mass[i]) {
+                    lv.bin = 4 * t + i;
+                    lv.bin_count = count[i];
+                    lv.before = before;
+                    lv.found = 1;
+                }
+                before += mass[i];
+            }
+        }
+        cluster_sync(size); /* the result is there, and no block reads the bins any more */
+        if (!lv.found) return Border{klo, 0xffffffffu, 0xffffffffu}; /* less than was asked for: all of the range */
+        const unsigned bin = lv.bin, bin_count = lv.bin_count;
+        target -= lv.before;
+        if (shift == S0) {
+            const unsigned key = key_at(bin);
+            u64 ties = target;
+            if (BY_MASS) {
+                const u64 w = scale.weight(value_of(key));
+                ties = (target + w - 1) / w; /* w > 0: the bin held some of the weight that was looked for */
+            }
+            __syncthreads(); /* lv is used again */
+            return Border{key, (unsigned)min(ties, (u64)bin_count), bin_count};
+        }
+        khi -= bin << shift;
+        const unsigned width = (1u << shift) - 1u;
+        if (khi - klo > width) klo = khi - width;
+        __syncthreads();
+    }
+}
+
+}  // namespace accb_rows

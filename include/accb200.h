@@ -235,6 +235,81 @@ ACCB_API int accb_permute_at(accb_context *ctx, accb_kernel *k, accb_stream stre
                              int nenv, long long n_src, const void *scalars, size_t scalar_bytes,
                              const accb_array *out, long long index_base);
 
+/* ------------------------------------------------- rows of scores
+ * Reductions along long rows that a fold cannot express: the best entries of a row, one entry drawn from a row, and
+ * the divergence of a row from a teacher's best entries.  A row holds one score (logit) per entry of a vocabulary.
+ * No counterpart in the reference, whose row folds see every element once (mkFoldDim,
+ * CUDA/CodeGen/Reduction.hs:221-367).
+ *   - Scores are 32- or 16-bit floats; all arithmetic is done in 32 bits or more.  Rows start every `pitch` elements
+ *     and need only the alignment of an element.  A row has 1 to 2^20 entries (none: ACCB_EBOUNDS).
+ *   - Entries are ranked by falling value, equal values by rising index; -0 equals +0.
+ *   - A temperature that is an argument lies between 1e-30 and 1e30.
+ *   - No scratch memory is used and nothing is allocated: launches may overlap on several streams and be captured.
+ *   - Device arrays must not overlap one another, except where it is said.                                       */
+enum { ACCB_ROWS_F32 = 0, ACCB_ROWS_F16 = 1, ACCB_ROWS_BF16 = 2 };
+typedef struct accb_rows_array {
+    void *ptr;       /* device pointer to the first row */
+    int type;        /* ACCB_ROWS_* */
+    int cols;        /* entries of a row */
+    long long rows;
+    long long pitch; /* elements from one row to the next, at least cols */
+} accb_rows_array;
+
+/* The k largest scores of every row, 1 <= k <= min(cols, 1024): values (rows x k, the type of x) in ranked order and
+ * their index (rows x k).  lse (rows, or NULL): log of the sum over the whole row of exp(score / temperature).  -inf
+ * and NaN are entries that are not there: a row with fewer than k others ends in (-inf, -1), a row with none has
+ * lse = -inf. */
+ACCB_API int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *x, double temperature, int k,
+                           void *values, int32_t *index, float *lse);
+
+/* One index per row, drawn by a random number in [0, 1) that the caller supplies.  The settings are device arrays of
+ * one value per row; NULL is off.  Entries have the weight exp(score / temperature); of the ranked entries are kept
+ *   top_k   the first top_k (0 and below: off),
+ *   top_p   of those, the shortest run from the top that holds the share top_p of their weight (1 and above: off;
+ *           0 and below: the first),
+ *   min_p   of those, the ones whose weight is at least min_p of the best one's (0 and below: off; above 1 as 1),
+ * and the row's token is the first kept index, in index order, at which the running sum of the kept weights exceeds
+ * uniform times their total.  A temperature that is not above 0 takes the best entry.  `allowed` (or NULL) holds bits
+ * for the entries, bit j % 32 of word j / 32 for entry j, rows every allowed_pitch words: the others are not there,
+ * whatever their score; nor are -inf and NaN.  A row with no entry gives token -1.  logprob (or NULL): log of the
+ * token's share of the kept weight; -inf with token -1.
+ * Weights are added as whole multiples of 2^-43 of the best entry's: sums are exact, and the token does not depend
+ * on how a row is split over the GPU. */
+ACCB_API int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *x, const uint32_t *allowed,
+                              long long allowed_pitch, const float *uniform, const float *temperature,
+                              const int32_t *top_k, const float *top_p, const float *min_p, int32_t *token,
+                              float *logprob);
+
+/* The Kullback-Leibler divergence of a student's rows from a teacher of which the scores of k entries per row are
+ * known (what accb_top_rows gives).  With q = softmax(student / temperature) over the row and the teacher's
+ * probabilities p over the entries it names,
+ *   teacher_lse NULL:  p = softmax(teacher / temperature) over the named entries;
+ *                      loss = weight * sum p (log p - log q)
+ *   else:              p = exp(teacher / temperature - teacher_lse), and what they leave, r = max(0, 1 - sum p), is
+ *                      one more class that the student meets with its probability q_r of all entries not named:
+ *                      loss = weight * (sum p (log p - log q) + r (log r - log q_r))
+ * teacher and index: rows x k, 1 <= k <= 1024.  An index outside the row, and a score of -inf or NaN, names nothing;
+ * an index named twice has both probabilities.  weight: one per row, or NULL for 1.  A row with weight 0, one whose
+ * teacher names nothing, and one of a student with only -inf has loss 0 and gradient 0, and the scores of a row with
+ * weight 0 are not read.  r counts for nothing where the student leaves nothing to the others.  A NaN of the student
+ * in a row that counts makes its loss and gradient NaN.
+ *   loss   rows
+ *   stats  rows x 4, or NULL: what the backward pass needs -- the row's maximum, 1 / sum exp((x - maximum) /
+ *          temperature), and the two factors of q in the gradient, at named entries (sum p + r) and elsewhere
+ *          (sum p + r - r / q_r).  All 0 for rows that do not count.
+ *   grad   NULL, or the gradient of sum(loss) in the student's shape and type, written in the same pass:
+ *          weight / temperature * (factor * q - p).  It may be the student's own memory (same pointer and pitch). */
+ACCB_API int accb_distill_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const void *teacher,
+                               int teacher_type, const int32_t *index, int k, const float *teacher_lse,
+                               const float *weight, double temperature, float *loss, float *stats,
+                               const accb_rows_array *grad);
+/* The gradient from the statistics of the forward pass: upstream (rows, or NULL for 1) is the gradient with respect to
+ * `loss`; everything else as given to the forward pass.  grad may be the student's own memory. */
+ACCB_API int accb_distill_rows_backward(accb_context *ctx, accb_stream stream, const accb_rows_array *student,
+                                        const void *teacher, int teacher_type, const int32_t *index, int k,
+                                        const float *teacher_lse, const float *weight, double temperature,
+                                        const float *stats, const float *upstream, const accb_rows_array *grad);
+
 /* Int32 `scanl (+) seed` for callers that cannot allocate device memory.  It has
  * no counterpart in the reference, whose every scan allocates its block-sum
  * array (scanCore, CUDA/Execute.hs:364-392).  Meant for code that runs with a

@@ -1,0 +1,606 @@
+"""The operators over rows of scores (accb_top_rows, accb_sample_rows, accb_distill_rows[_backward]) against their
+definitions in 64 bits (rows_reference.py).
+
+Tolerances.  Values and indices are exact.  A log-sum-exp is m / T + log(sum): the sum's terms carry the error of a
+32-bit exponential (exponent |y| <= 150 rounded to 2^-24 of itself and a base-2 exponential good to 2 units in the last place), which
+is at most 150 * ln 2 * 2^-24 + 2^-22 < 1e-5 for one term; terms that far down weigh nothing, and for the terms that
+count (|y| <= 20) it is 20 * ln 2 * 2^-24 + 2^-22 + 64 * 2^-24 (a thread's running sum of at most 128 terms, each
+addition half a step) < 6e-6.  The result is rounded once, 2^-24 of itself.  A loss of weight w inherits sum p = 1
+times that.  A gradient entry is w / T times (sum p + r) q - p or (sum p + r - r / q_r) q: q and 1 / q_r are within the
+same 6e-6 of themselves plus 2^-22, the rest is computed in 64 bits and rounded once; so every part is off by at most
+twice 6e-6 of itself, and the whole is rounded to the element type."""
+import numpy as np
+import pytest
+
+from rows_reference import clean, distill, sample, top
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["float32", "float16", "bfloat16"]
+EPS = {"float32": 2.0**-24, "float16": 2.0**-11, "bfloat16": 2.0**-8}
+SUM_ERROR = 6e-6
+
+
+def scores(torch, rng, rows, cols, kind, pitch=None, offset=0, spread=2.0, peaks=True):
+    """Rows of scores in memory of their own: `pitch` elements apart, the first one `offset` elements into it."""
+    x = rng.normal(0, spread, (rows, cols)).astype(np.float32)
+    if peaks and cols > 4:
+        for r in range(rows):
+            at = rng.choice(cols, min(8, cols), replace=False)
+            x[r, at] = rng.uniform(4, 14, at.size)
+    return place(torch, x, kind, pitch, offset)
+
+
+def place(torch, x, kind, pitch=None, offset=0):
+    rows, cols = x.shape
+    pitch = pitch or cols
+    memory = torch.full((offset + rows * pitch + 64,), 77.0, dtype=getattr(torch, kind), device="cuda")
+    view = memory[offset:].as_strided((rows, cols), (pitch, 1), storage_offset=offset)
+    view.copy_(torch.from_numpy(x))
+    return view
+
+
+def numbers(t):
+    return t.double().cpu().numpy()
+
+
+# ------------------------------------------------------------------ top
+def run_top(ctx, torch, x, k, temperature=1.0, lse=True):
+    rows = x.shape[0]
+    values = torch.full((rows, k), 7.0, dtype=x.dtype, device="cuda")
+    index = torch.full((rows, k), -7, dtype=torch.int32, device="cuda")
+    out = torch.full((rows,), 7.0, device="cuda") if lse else None
+    ctx.top_rows(x, values, index, lse=out, temperature=temperature)
+    ctx.sync()
+    return numbers(values), index.cpu().numpy(), numbers(out) if lse else None
+
+
+def check_top(ctx, torch, x, k, temperature=1.0):
+    values, index, lse = run_top(ctx, torch, x, k, temperature)
+    for r, row in enumerate(numbers(x)):
+        v, i, s = top(row, k, temperature)
+        assert np.array_equal(values[r], v), (r, values[r], v)
+        assert np.array_equal(index[r], i), (r, index[r], i)
+        assert lse[r] == s or abs(lse[r] - s) <= SUM_ERROR + 2.0**-24 * abs(s), (r, lse[r], s)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (3, 2, 2), (5, 7, 3), (2, 33, 33), (4, 1000, 50), (2, 1024, 1024), (3, 4099, 1000),
+                                         (2, 32768, 64), (5, 50257, 20), (1, 131072, 1024), (2, 151001, 7)])
+def test_top(ctx, torch_cuda, rng, kind, rows, cols, k):
+    check_top(ctx, torch_cuda, scores(torch_cuda, rng, rows, cols, kind), k, 1.0 if k % 2 else 2.5)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset,pitch", [(1, 1013), (3, 1001), (7, 1024), (8, 1009), (0, 1003)])
+def test_top_of_rows_anywhere(ctx, torch_cuda, rng, kind, offset, pitch):
+    check_top(ctx, torch_cuda, scores(torch_cuda, rng, 9, 1001, kind, pitch, offset), 17)
+
+
+def test_top_of_rows_too_long_for_shared_memory(ctx, torch_cuda, rng):
+    check_top(ctx, torch_cuda, scores(torch_cuda, rng, 2, (1 << 20) - 3, "float32", (1 << 20) + 5, 1), 300)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_top_settles_ties_by_index(ctx, torch_cuda, rng, kind):
+    t = torch_cuda
+    x = rng.integers(-3, 4, (6, 5000)).astype(np.float32)
+    x[0] = 0.0
+    x[1] = np.where(rng.random(5000) < 0.5, 0.0, -0.0)  # equal values
+    x[2, ::3] = -0.0
+    for k in (1, 2, 100, 1024):
+        check_top(ctx, t, place(t, x, kind), k)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_top_of_rows_with_little_in_them(ctx, torch_cuda, rng, kind):
+    t = torch_cuda
+    x = rng.normal(0, 1, (8, 3000)).astype(np.float32)
+    x[0] = -np.inf
+    x[1, 5:] = -np.inf
+    x[2] = np.nan
+    x[3, ::2] = np.nan
+    x[4] = np.finfo(np.float32).min if kind == "float32" else float(t.finfo(getattr(t, kind)).min)
+    x[5, 7] = np.inf
+    x[6, 1:] = -np.inf
+    x[7] = np.nan
+    x[7, 2999] = -1.0
+    values, index, lse = run_top(ctx, t, place(t, x, kind), 40)
+    for r, row in enumerate(numbers(place(t, x, kind))):
+        v, i, s = top(row, 40, 1.0)
+        assert np.array_equal(values[r], v) and np.array_equal(index[r], i), r
+        if r != 5:  # an infinite score: inf - inf in the reference's formula
+            assert lse[r] == s or abs(lse[r] - s) <= SUM_ERROR + 2.0**-24 * abs(s)
+    assert lse[5] == np.inf
+
+
+# --------------------------------------------------------------- sampling
+def settings(torch, rows, **values):
+    kinds = dict(temperature=torch.float32, top_p=torch.float32, min_p=torch.float32, top_k=torch.int32, uniform=torch.float32)
+    return {k: torch.as_tensor(np.broadcast_to(np.asarray(v), (rows,)).copy()).to(kinds[k]).cuda() for k, v in values.items() if v is not None}
+
+
+def bits_of(torch, allowed):
+    rows, cols = allowed.shape
+    padded = np.zeros((rows, (cols + 31) // 32 * 32), bool)
+    padded[:, :cols] = allowed
+    words = np.packbits(padded.reshape(rows, -1, 32), axis=2, bitorder="little").view(np.uint32)[:, :, 0]
+    return torch.from_numpy(words.view(np.int32).copy()).cuda()
+
+
+def run_sample(ctx, torch, x, allowed=None, **s):
+    rows = x.shape[0]
+    token = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+    logprob = torch.full((rows,), 7.0, device="cuda")
+    ctx.sample_rows(x, s.pop("uniform"), token, logprob=logprob, allowed=allowed, **s)
+    ctx.sync()
+    return token.cpu().numpy(), numbers(logprob)
+
+
+def check_sample(ctx, torch, x, allowed=None, **values):
+    rows = x.shape[0]
+    s = settings(torch, rows, **values)
+    host = {k: v.double().cpu().numpy() for k, v in s.items()}
+    token, logprob = run_sample(ctx, torch, x, bits_of(torch, allowed) if allowed is not None else None, **s)
+    for r, row in enumerate(numbers(x)):
+        want, log_share, distance = sample(row, allowed=None if allowed is None else allowed[r], **{k: v[r] for k, v in host.items()})
+        # sums are exact up to 2^-43 for each entry; the reference's own are good to 2^-52 for each
+        assert token[r] == want or distance < row.size * 2.0**-43, (r, token[r], want, distance)
+        if token[r] == want:
+            # computed in 64 bits from exact sums, rounded once; near a border of top_p the reference may keep one more
+            assert logprob[r] == log_share or abs(logprob[r] - log_share) <= 2.0**-24 * abs(log_share) + row.size * 2.0**-43
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [1, 2, 31, 33, 1000, 4099, 32768, 50257, 131072, 151001])
+def test_sample_without_cuts(ctx, torch_cuda, rng, kind, cols):
+    check_sample(ctx, torch_cuda, scores(torch_cuda, rng, 4, cols, kind), uniform=rng.random(4), temperature=[1.0, 0.5, 3.0, 100.0])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cuts", [dict(top_k=1), dict(top_k=5), dict(top_k=300), dict(top_k=3000), dict(top_p=0.5), dict(top_p=0.9),
+                                  dict(top_p=0.999), dict(top_p=0.0), dict(min_p=0.1), dict(min_p=1.0), dict(min_p=7.0),
+                                  dict(top_k=50, top_p=0.9), dict(top_k=50, top_p=0.9, min_p=0.05), dict(top_k=4000, min_p=0.01),
+                                  dict(top_p=0.99999994), dict(top_k=10**9), dict(top_k=-3), dict(top_p=1.5, min_p=-1.0)])
+@pytest.mark.parametrize("cols,temperature", [(4099, 0.7), (40000, 1.0), (100003, 2.0)])
+def test_sample_with_cuts(ctx, torch_cuda, rng, kind, cols, temperature, cuts):
+    check_sample(ctx, torch_cuda, scores(torch_cuda, rng, 6, cols, kind), uniform=rng.random(6), temperature=temperature, **cuts)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_flat_rows(ctx, torch_cuda, rng, kind):
+    """Rows without a peak: every entry is near the border, and there are many ties in 16 bits."""
+    x = scores(torch_cuda, rng, 8, 70001, kind, spread=0.3, peaks=False)
+    for cuts in (dict(top_p=0.9), dict(top_k=1000), dict(top_k=40000, top_p=0.7), dict(min_p=0.5), dict()):
+        check_sample(ctx, torch_cuda, x, uniform=rng.random(8), **cuts)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_equal_scores(ctx, torch_cuda, kind):
+    """All scores equal: the weights are exact in the reference too, so that borders can be met exactly."""
+    t = torch_cuda
+    x = place(t, np.full((9, 4096), 1.5, np.float32), kind)
+    u = np.arange(9) / 8 * 0.9999999
+    u[:8] = np.arange(8) / 8
+    check_sample(ctx, t, x, uniform=u)
+    check_sample(ctx, t, x, uniform=u, top_p=0.5)
+    check_sample(ctx, t, x, uniform=u, top_k=8)
+    check_sample(ctx, t, x, uniform=u, top_k=1000, top_p=0.25)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset,pitch", [(1, 5003), (5, 5001), (8, 5008)])
+def test_sample_allowed(ctx, torch_cuda, rng, kind, offset, pitch):
+    t = torch_cuda
+    x = scores(t, rng, 12, 5001, kind, pitch, offset)
+    allowed = rng.random((12, 5001)) < 0.3
+    allowed[0] = False
+    allowed[1] = False
+    allowed[1, 5000] = True
+    allowed[2] = False
+    allowed[2, 0] = True
+    allowed[3] = True
+    host = numbers(x)
+    host[~allowed] = rng.choice([np.nan, np.inf, -np.inf, 60000.0], (~allowed).sum())  # whatever a masked place holds
+    x.copy_(t.from_numpy(host))
+    check_sample(ctx, t, x, allowed, uniform=rng.random(12))
+    check_sample(ctx, t, x, allowed, uniform=rng.random(12), temperature=0.8, top_k=40, top_p=0.9, min_p=0.01)
+
+
+def test_sample_every_row_with_settings_of_its_own(ctx, torch_cuda, rng):
+    n = 200
+    check_sample(ctx, torch_cuda, scores(torch_cuda, rng, n, 3001, "bfloat16"), uniform=rng.random(n),
+                 temperature=rng.choice([0.0, -1.0, np.nan, 0.3, 1.0, 2.0], n), top_k=rng.choice([0, 1, 2, 30, 3001, 5000], n),
+                 top_p=rng.choice([1.0, 0.3, 0.9, np.nan], n), min_p=rng.choice([0.0, 0.1, np.nan], n))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_rows_with_little_in_them(ctx, torch_cuda, rng, kind):
+    t = torch_cuda
+    x = rng.normal(0, 1, (8, 3000)).astype(np.float32)
+    x[0] = -np.inf
+    x[1, 5:] = -np.inf
+    x[2] = np.nan
+    x[3, ::2] = np.nan
+    x[4] = np.finfo(np.float32).min if kind == "float32" else float(t.finfo(getattr(t, kind)).min)
+    x[5, 7] = x[5, 1234] = np.inf
+    x[6, 1:] = -np.inf
+    x[7] = np.nan
+    x[7, 2999] = -1.0
+    for cuts in (dict(), dict(top_k=20), dict(top_p=0.9), dict(min_p=0.1), dict(top_k=20, top_p=0.5), dict(temperature=0.0),
+                 dict(temperature=1e-30), dict(temperature=np.inf), dict(temperature=np.inf, top_p=0.5)):
+        check_sample(ctx, t, place(t, x, kind), uniform=rng.random(8), **cuts)
+
+
+def test_sample_random_numbers_at_the_ends(ctx, torch_cuda, rng):
+    t = torch_cuda
+    x = scores(t, rng, 6, 5000, "float32")
+    for u in (0.0, 1.0 - 2.0**-24, 1.0, 2.0):
+        check_sample(ctx, t, x, uniform=u)
+    token, _ = run_sample(ctx, t, x, **settings(t, 6, uniform=np.nan))
+    assert ((token >= 0) & (token < 5000)).all()
+
+
+def test_sample_of_rows_too_long_for_shared_memory(ctx, torch_cuda, rng):
+    n = (1 << 20) - 1
+    x = scores(torch_cuda, rng, 2, n, "float32", n + 2, 3)
+    allowed = rng.random((2, n)) < 0.5
+    for cuts in (dict(), dict(top_k=100, top_p=0.9), dict(top_p=0.8, min_p=1e-4)):
+        check_sample(ctx, torch_cuda, x, uniform=rng.random(2), **cuts)
+        check_sample(ctx, torch_cuda, x, allowed, uniform=rng.random(2), **cuts)
+
+
+def test_sample_draws_by_the_shares(ctx, torch_cuda):
+    """4096 evenly spaced random numbers over one row draw every index as often as its share says, give or take one."""
+    t = torch_cuda
+    n = 4096
+    row = t.linspace(-3, 3, 50, device="cuda")
+    x = row.expand(n, 50).contiguous()
+    u = (t.arange(n, device="cuda") + 0.5) / n
+    token = t.empty(n, dtype=t.int32, device="cuda")
+    ctx.sample_rows(x, u, token)
+    ctx.sync()
+    share = t.softmax(row.double(), 0).cpu().numpy()
+    assert np.abs(np.bincount(token.cpu().numpy(), minlength=50) - n * share).max() <= 1.0
+
+
+# ----------------------------------------------------------- distillation
+def teacher_of(torch, rng, x, k, kind, temperature, rest):
+    """A teacher's k best scores of rows like the student's, some entries missing."""
+    rows, cols = x.shape
+    z = np.nan_to_num(numbers(x), nan=0.0, posinf=5.0, neginf=-5.0) + rng.normal(0, 0.7, (rows, cols))
+    at = np.stack([rng.permutation(np.argsort(-row)[:k]) for row in z])
+    values = np.take_along_axis(z, at, 1)
+    lse = np.array([np.log(np.exp(row / temperature - (row / temperature).max()).sum()) + (row / temperature).max() for row in z])
+    at = at.astype(np.int32)
+    if k > 3:
+        at[::3, k // 2] = -1
+        at[1::3, 0] = cols
+        values[2::3, 1] = -np.inf
+    return (torch.from_numpy(values).to(getattr(torch, kind)).cuda(), torch.from_numpy(at).cuda(),
+            torch.from_numpy(lse).float().cuda() if rest else None)
+
+
+def check_gradient(got, x, teacher, index, lse, weight, upstream, temperature, kind):
+    t, i = numbers(teacher), index.cpu().numpy()
+    for r, row in enumerate(numbers(x)):
+        _, d, parts = distill(row, t[r], i[r], None if lse is None else float(lse[r]), float(weight[r]), temperature)
+        d = d * upstream[r]
+        # (sum p + r) q - p, (sum p + r - r / q_r) q: every part is off by its own share, however small the difference
+        parts = parts * abs(upstream[r])
+        small = 2.0**-24 if kind == "float16" else 2.0**-126  # half a step of subnormal numbers
+        bad = np.abs(got[r] - d) > EPS[kind] * np.abs(d) + 2 * SUM_ERROR * parts + small
+        assert not bad.any(), (r, np.nonzero(bad)[0][:5], got[r][bad][:5], d[bad][:5])
+
+
+def check_distill(ctx, torch, rng, x, k, temperature=1.0, rest=False, teacher_kind="float32", in_place=False, weight=None, teacher=None,
+                  grad_pitch=None, grad_offset=0):
+    rows, cols = x.shape
+    kind = str(x.dtype)[6:]
+    tv, ti, lse = teacher or teacher_of(torch, rng, x, k, teacher_kind, temperature, rest)
+    if weight is None:
+        weight = rng.uniform(0.1, 2, rows).astype(np.float32)
+        weight[rows // 2:rows // 2 + 1] = 0.0 if rows > 2 else weight[0]
+    w = torch.from_numpy(weight).cuda()
+    host = x.clone()
+    want = [distill(row, numbers(tv)[r], ti.cpu().numpy()[r], None if lse is None else float(lse[r]), float(weight[r]), temperature)[0]
+            for r, row in enumerate(numbers(host))]
+    new = lambda *shape: torch.full(shape, 7.0, device="cuda")  # noqa: E731
+    loss, stats = new(rows), new(rows, 4)
+    ctx.distill_rows(x, tv, ti, loss, stats=stats, teacher_lse=lse, weight=w, temperature=temperature)
+    ctx.sync()
+    allowance = np.abs(weight) * SUM_ERROR * 2 + 2.0**-23 * np.abs(want)
+    assert (np.abs(numbers(loss) - want) <= allowance).all(), (numbers(loss), want)
+    # backward from the statistics
+    upstream = rng.uniform(-2, 2, rows).astype(np.float32)
+    fresh = lambda: place(torch, np.zeros((rows, cols), np.float32), kind, grad_pitch, grad_offset)  # noqa: E731
+    grad = fresh()
+    ctx.distill_rows_backward(x, tv, ti, stats, torch.from_numpy(upstream).cuda(), grad, teacher_lse=lse, weight=w, temperature=temperature)
+    ctx.sync()
+    check_gradient(numbers(grad), host, tv, ti, lse, weight, upstream, temperature, kind)
+    # both in one pass
+    both, grad = new(rows), x if in_place else fresh()
+    ctx.distill_rows(x, tv, ti, both, grad=grad, teacher_lse=lse, weight=w, temperature=temperature)
+    ctx.sync()
+    assert torch.equal(both, loss)
+    check_gradient(numbers(grad), host, tv, ti, lse, weight, np.ones(rows), temperature, kind)
+    if in_place:
+        x.copy_(host)
+        ctx.distill_rows_backward(x, tv, ti, stats, None, x, teacher_lse=lse, weight=w, temperature=temperature)
+        ctx.sync()
+        check_gradient(numbers(x), host, tv, ti, lse, weight, np.ones(rows), temperature, kind)
+        x.copy_(host)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,cols,k", [(1, 1, 1), (3, 2, 1), (5, 7, 7), (2, 33, 5), (4, 1000, 50), (2, 1024, 1024), (3, 4099, 300),
+                                         (2, 32768, 64), (5, 50257, 20), (2, 131072, 100), (2, 151001, 7)])
+def test_distill(ctx, torch_cuda, rng, kind, rows, cols, k, rest):
+    check_distill(ctx, torch_cuda, rng, scores(torch_cuda, rng, rows, cols, kind), k, 1.0 if cols % 2 else 2.0, rest)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("teacher_kind", TYPES)
+def test_distill_types_of_the_teacher(ctx, torch_cuda, rng, kind, teacher_kind):
+    check_distill(ctx, torch_cuda, rng, scores(torch_cuda, rng, 3, 3001, kind), 20, 0.7, True, teacher_kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("offset,pitch,grad_offset,grad_pitch", [(1, 1013, 1, 1013), (3, 1001, 0, 1008), (0, 1008, 5, 1003), (7, 1003, 7, 1011)])
+def test_distill_of_rows_anywhere(ctx, torch_cuda, rng, kind, offset, pitch, grad_offset, grad_pitch):
+    x = scores(torch_cuda, rng, 6, 1001, kind, pitch, offset)
+    check_distill(ctx, torch_cuda, rng, x, 12, rest=True, grad_pitch=grad_pitch, grad_offset=grad_offset)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [1001, 100003])
+def test_distill_in_place(ctx, torch_cuda, rng, kind, cols):
+    check_distill(ctx, torch_cuda, rng, scores(torch_cuda, rng, 4, cols, kind, cols + 2, 1), 16, rest=True, in_place=True)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_of_rows_too_long_for_shared_memory(ctx, torch_cuda, rng, rest):
+    n = (1 << 20) - 5
+    check_distill(ctx, torch_cuda, rng, scores(torch_cuda, rng, 2, n, "float32", n + 2, 1), 40, rest=rest, in_place=True)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("kind", TYPES)
+def test_distill_an_index_named_twice(ctx, torch_cuda, rng, kind, rest):
+    t = torch_cuda
+    x = scores(t, rng, 3, 2000, kind)
+    tv, ti, lse = teacher_of(t, rng, x, 300, "float32", 1.0, rest)
+    ti[0, 5] = ti[0, 299] = ti[0, 100]
+    ti[1, :] = 17
+    ti[2, 290] = ti[2, 0]
+    if rest:
+        lse = lse + 1.5  # what is named twice must not add up to more than there is
+        lse[1] += 5.0
+    check_distill(ctx, t, rng, x, 300, teacher=(tv, ti, lse))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("kind", TYPES)
+def test_distill_rows_that_do_not_count(ctx, torch_cuda, rng, kind, rest):
+    t = torch_cuda
+    x = scores(t, rng, 6, 3001, kind)
+    tv, ti, lse = teacher_of(t, rng, x, 9, "float32", 1.0, rest)
+    x[0] = float("nan")           # weight 0
+    x[1] = -float("inf")          # a student that excludes everything
+    ti[2] = -1                    # a teacher that names nothing
+    tv[3] = -float("inf")
+    x[4, 5::2] = -float("inf")    # a student that excludes half
+    ti[4] = t.arange(0, 18, 2, dtype=t.int32, device="cuda")
+    weight = np.array([0, 1, 1, 1, 1, 1], np.float32)
+    check_distill(ctx, t, rng, x, 9, weight=weight, teacher=(tv, ti, lse), in_place=True)
+
+
+def test_distill_the_rest_alone_far_below(ctx, torch_cuda, rng):
+    """The student leaves the unnamed entries less than 32 bits can hold next to the named ones."""
+    t = torch_cuda
+    x = rng.normal(0, 1, (2, 2000)).astype(np.float32)
+    x[:, :4] += 150.0
+    tv = t.tensor([[1.0, 0.5, 0.2, 0.1]] * 2, device="cuda")
+    ti = t.arange(4, dtype=t.int32, device="cuda").repeat(2, 1)
+    lse = t.tensor([2.0, 3.0], device="cuda")
+    loss = t.empty(2, device="cuda")
+    ctx.distill_rows(place(t, x, "float32"), tv, ti, loss, teacher_lse=lse)
+    ctx.sync()
+    want = [distill(x[r], tv[r].cpu().numpy(), ti[r].cpu().numpy(), float(lse[r]), 1.0, 1.0)[0] for r in range(2)]
+    assert np.abs(numbers(loss) - want).max() <= 2.0**-23 * max(want) + 2 * SUM_ERROR
+
+
+def test_distill_nan_in_a_row_that_counts(ctx, torch_cuda, rng):
+    t = torch_cuda
+    for rest in (False, True):
+        x = scores(t, rng, 3, 1000, "bfloat16")
+        tv, ti, lse = teacher_of(t, rng, x, 5, "float32", 1.0, rest)
+        x[0, 999] = float("nan")
+        x[1, int(ti[1, 4])] = float("nan")
+        loss, stats, grad = t.zeros(3, device="cuda"), t.zeros(3, 4, device="cuda"), t.zeros_like(x)
+        ctx.distill_rows(x, tv, ti, loss, stats=stats, grad=grad, teacher_lse=lse)
+        ctx.sync()
+        assert loss.isnan().tolist() == [True, True, False]
+        assert grad[:2].isnan().all() and not grad[2].isnan().any()
+        grad.zero_()
+        ctx.distill_rows_backward(x, tv, ti, stats, None, grad, teacher_lse=lse)
+        ctx.sync()
+        assert grad[:2].isnan().all() and not grad[2].isnan().any()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_gradient_against_differences(ctx, torch_cuda, rng, rest):
+    """Central differences of the loss, 32 bits: h = 2^-3, the third derivative of a log-sum-exp is below 1, so the
+    difference is off by h^2 / 6 at most, plus the loss's own error over 2 h."""
+    t = torch_cuda
+    n, k, h = 40, 6, 0.125
+    x = rng.normal(0, 1, n).astype(np.float32)
+    at = rng.choice(n, k, replace=False).astype(np.int32)
+    rows = np.repeat(x[None], 2 * n + 1, 0)
+    for j in range(n):
+        rows[2 * j, j] += h
+        rows[2 * j + 1, j] -= h
+    tv = t.from_numpy(rng.normal(1, 1, k).astype(np.float32)).cuda().repeat(2 * n + 1, 1)
+    ti = t.from_numpy(at).cuda().repeat(2 * n + 1, 1)
+    lse = t.full((2 * n + 1,), float(np.log(np.exp(numbers(tv)[0]).sum()) + 0.5), device="cuda") if rest else None
+    loss, grad = t.empty(2 * n + 1, device="cuda"), t.empty(2 * n + 1, n, device="cuda")
+    ctx.distill_rows(place(t, rows, "float32"), tv, ti, loss, grad=grad, teacher_lse=lse, temperature=1.0)
+    ctx.sync()
+    loss = numbers(loss)
+    d = (loss[0:2 * n:2] - loss[1:2 * n:2]) / (2 * h)
+    assert np.abs(d - numbers(grad)[2 * n]).max() <= h * h / 6 + (2 * SUM_ERROR + 2.0**-23 * loss.max()) / h
+
+
+# ------------------------------------------------------------- in use
+def test_rows_nobody_asked_for_stay_as_they_were(ctx, torch_cuda, rng):
+    t = torch_cuda
+    x = scores(t, rng, 4, 1001, "bfloat16", 1008, 0)
+    tv, ti, _ = teacher_of(t, rng, x, 4, "float32", 1.0, False)
+    memory = t.full((6, 1008), 5.0, dtype=t.bfloat16, device="cuda")
+    loss = t.full((6,), 5.0, device="cuda")
+    ctx.distill_rows(x, tv, ti, loss[1:5], grad=memory[1:5, 3:1004])
+    token = t.full((6,), 5, dtype=t.int32, device="cuda")
+    ctx.sample_rows(x, t.rand(4, device="cuda"), token[1:5])
+    ctx.sync()
+    assert (memory[0] == 5).all() and (memory[5] == 5).all() and (memory[:, :3] == 5).all() and (memory[:, 1004:] == 5).all()
+    assert loss[0] == 5 and loss[5] == 5 and token[0] == 5 and token[5] == 5
+
+
+def test_no_rows(ctx, torch_cuda):
+    t = torch_cuda
+    x = t.empty(0, 100, device="cuda")
+    e = lambda *shape, kind=t.float32: t.empty(shape, dtype=kind, device="cuda")  # noqa: E731
+    ctx.top_rows(x, e(0, 5), e(0, 5, kind=t.int32), lse=e(0))
+    ctx.sample_rows(x, e(0), e(0, kind=t.int32))
+    ctx.distill_rows(x, e(0, 5), e(0, 5, kind=t.int32), e(0), grad=e(0, 100), stats=e(0, 4))
+    ctx.distill_rows_backward(x, e(0, 5), e(0, 5, kind=t.int32), e(0, 4), None, e(0, 100))
+    ctx.sync()
+
+
+def test_teacher_to_student_to_answer_on_a_stream_and_as_a_graph(accb, ctx, torch_cuda, rng):
+    """The operators as they are used together: a teacher's best scores, the student's loss and gradient, a step along
+    it, and a token of the new scores; eagerly on a stream of its own, and replayed as a graph with new inputs."""
+    t = torch_cuda
+    rows, cols, k = 6, 20011, 32
+    teacher, student = scores(t, rng, rows, cols, "bfloat16"), scores(t, rng, rows, cols, "float32")
+    u = t.from_numpy(rng.random(rows).astype(np.float32)).cuda()
+    top_k = t.full((rows,), 20, dtype=t.int32, device="cuda")
+    values, index, lse = t.empty(rows, k, dtype=t.bfloat16, device="cuda"), t.empty(rows, k, dtype=t.int32, device="cuda"), t.empty(rows, device="cuda")
+    loss, grad, token = t.empty(rows, device="cuda"), t.empty(rows, cols, device="cuda"), t.empty(rows, dtype=t.int32, device="cuda")
+
+    def run(stream):
+        ctx.top_rows(teacher, values, index, lse=lse, stream=stream)
+        ctx.distill_rows(student, values, index, loss, grad=grad, teacher_lse=lse, stream=stream)
+        ctx.sample_rows(student, u, token, top_k=top_k, stream=stream)
+
+    s = t.cuda.Stream()
+    s.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(s):
+        run(None)  # the current stream
+    s.synchronize()
+    for r in range(rows):
+        v, i, m = top(numbers(teacher)[r], k, 1.0)
+        assert np.array_equal(numbers(values)[r], v) and np.array_equal(index.cpu().numpy()[r], i)
+        want = distill(numbers(student)[r], v, i, float(lse[r]), 1.0, 1.0)[0]
+        assert abs(float(loss[r]) - want) <= 2 * SUM_ERROR + 2.0**-23 * abs(want)
+        assert int(token[r]) == sample(numbers(student)[r], float(u[r]), top_k=20)[0]
+    eager = [a.clone() for a in (values, index, lse, loss, grad, token)]
+    graph, second = t.cuda.CUDAGraph(), t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        run(None)
+    with t.cuda.graph(second):
+        run(None)
+    other = scores(t, rng, rows, cols, "bfloat16")
+    kept, was = teacher.clone(), student.clone()
+    for g in (graph, second, graph):
+        teacher.copy_(other)
+        student.copy_(other)
+        g.replay()
+        teacher.copy_(kept)
+        student.copy_(was)
+        for a in (values, index, lse, loss, grad, token):
+            a.zero_()
+        g.replay()
+        t.cuda.synchronize()
+        for a, b in zip((values, index, lse, loss, grad, token), eager):
+            assert t.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(ctx, torch_cuda, rng):
+    t = torch_cuda
+    x = scores(t, rng, 300, 30011, "bfloat16")
+    u = t.from_numpy(rng.random(300).astype(np.float32)).cuda()
+    p = t.full((300,), 0.9, device="cuda")
+    streams = [t.cuda.Stream() for _ in range(4)]
+    out = [t.empty(300, dtype=t.int32, device="cuda") for _ in range(5)]
+    ctx.sample_rows(x, u, out[4], top_p=p)
+    t.cuda.synchronize()
+    for _ in range(20):
+        for s, o in zip(streams, out):
+            ctx.sample_rows(x, u, o, top_p=p, stream=s.cuda_stream)
+    t.cuda.synchronize()
+    assert all(t.equal(o, out[4]) for o in out)
+
+
+def test_same_rows_alone_and_in_a_batch(ctx, torch_cuda, rng):
+    """How many blocks hold a row depends on how many rows there are; what is drawn does not."""
+    t = torch_cuda
+    x = scores(t, rng, 400, 40000, "bfloat16")
+    u = t.from_numpy(rng.random(400).astype(np.float32)).cuda()
+    p = t.full((400,), 0.95, device="cuda")
+    batch, one = t.empty(400, dtype=t.int32, device="cuda"), t.empty(1, dtype=t.int32, device="cuda")
+    lp, lp1 = t.empty(400, device="cuda"), t.empty(1, device="cuda")
+    ctx.sample_rows(x, u, batch, logprob=lp, top_p=p)
+    for r in (0, 1, 7, 399):
+        ctx.sample_rows(x[r:r + 1], u[r:r + 1], one, logprob=lp1, top_p=p[r:r + 1])
+        ctx.sync()
+        assert t.equal(one, batch[r:r + 1]) and t.equal(lp1, lp[r:r + 1])
+
+
+def test_offsets_past_32_bits(ctx, torch_cuda, rng):
+    """Rows that start more than 2^32 elements into the matrix."""
+    t = torch_cuda
+    rows, cols, pitch = 5, 1000, (1 << 30) + 8
+    memory = t.empty((rows - 1) * pitch + cols, dtype=t.bfloat16, device="cuda")
+    x = memory.as_strided((rows, cols), (pitch, 1))
+    x.copy_(t.from_numpy(rng.normal(0, 2, (rows, cols)).astype(np.float32)))
+    check_top(ctx, t, x, 10)
+    check_sample(ctx, t, x, uniform=rng.random(rows), top_p=0.9)
+    tv, ti, _ = teacher_of(t, rng, x, 5, "float32", 1.0, False)
+    host, loss = x.contiguous(), t.empty(rows, device="cuda")
+    ctx.distill_rows(x, tv, ti, loss, grad=x)
+    ctx.sync()
+    check_gradient(numbers(x), host, tv, ti, None, np.ones(rows), np.ones(rows), 1.0, "bfloat16")
+
+
+# ------------------------------------------------------------ refusals
+def test_refusals_of_the_library(accb, ctx, torch_cuda):
+    t = torch_cuda
+    L = accb.lib()
+    import ctypes as C
+    x, out = t.zeros(2, 8, device="cuda"), t.zeros(64, device="cuda")
+    p, q = C.c_void_p(x.data_ptr()), C.c_void_p(out.data_ptr())
+    array = lambda ptr=x.data_ptr(), kind=0, cols=8, rows=2, pitch=8: C.byref(accb.accb_rows_array(ptr, kind, cols, rows, pitch))  # noqa: E731
+    top_call = lambda a, tau=1.0, k=2, v=q, i=q: L.accb_top_rows(ctx.handle, None, a, tau, k, v, i, None)  # noqa: E731
+    for bad in (array(kind=3), array(rows=-1), array(cols=(1 << 20) + 1, pitch=1 << 21), array(pitch=7), array(ptr=None),
+                array(ptr=x.data_ptr() + 2), array(rows=1 << 40), array(rows=1 << 20, pitch=1 << 50), None):
+        assert top_call(bad) == accb.EINVAL
+        assert L.accb_last_error(ctx.handle)
+        assert L.accb_sample_rows(ctx.handle, None, bad, None, 0, p, None, None, None, None, q, None) == accb.EINVAL
+        assert L.accb_distill_rows(ctx.handle, None, bad, p, 0, p, 2, None, None, 1.0, q, None, None) == accb.EINVAL
+    assert top_call(array(cols=0)) == accb.EBOUNDS
+    for bad in (dict(k=0), dict(k=9), dict(tau=0.0), dict(tau=-1.0), dict(tau=float("nan")), dict(tau=float("inf")), dict(v=None), dict(i=None)):
+        assert top_call(array(), **bad) == accb.EINVAL
+    assert L.accb_top_rows(None, None, array(), 1.0, 1, q, q, None) == accb.EINVAL
+    assert L.accb_sample_rows(ctx.handle, None, array(), None, 0, None, None, None, None, None, q, None) == accb.EINVAL
+    assert L.accb_sample_rows(ctx.handle, None, array(), None, 0, p, None, None, None, None, None, None) == accb.EINVAL
+    assert L.accb_sample_rows(ctx.handle, None, array(), p, 0, p, None, None, None, None, q, None) == accb.EINVAL
+    d = lambda teacher=p, kind=0, index=p, k=2, tau=1.0, loss=q, grad=None: L.accb_distill_rows(  # noqa: E731
+        ctx.handle, None, array(), teacher, kind, index, k, None, None, tau, loss, None, grad)
+    for bad in (dict(teacher=None), dict(kind=9), dict(index=None), dict(k=0), dict(k=1025), dict(tau=0.0), dict(loss=None),
+                dict(grad=array(cols=7)), dict(grad=array(rows=1)), dict(grad=array(kind=2)), dict(grad=array(ptr=None))):
+        assert d(**bad) == accb.EINVAL
+    b = lambda stats=p, grad=array(): L.accb_distill_rows_backward(ctx.handle, None, array(), p, 0, p, 2, None, None, 1.0, stats, None, grad)  # noqa: E731
+    assert b(stats=None) == accb.EINVAL and b(grad=None) == accb.EINVAL
+    ctx.sync()  # and nothing was launched that could have failed
