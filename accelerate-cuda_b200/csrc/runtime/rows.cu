@@ -458,6 +458,7 @@ struct Teacher {
         float z[M], top = neg_inf();
 #pragma unroll
         for (int i = 0; i < M; ++i) {
+            logp[i] = p[i] = 0.0;
             const int j = threadIdx.x + i * kThreads;
             at[i] = -1;
             z[i] = neg_inf();
@@ -483,8 +484,9 @@ struct Teacher {
         double s = 0.0;
 #pragma unroll
         for (int i = 0; i < M; ++i) {
+            if (at[i] < 0) continue;
             logp[i] = (double)z[i] * inv - norm;
-            p[i] = at[i] >= 0 ? exp(logp[i]) : 0.0;
+            p[i] = exp(logp[i]);
             s += p[i];
         }
         named = block_sum(s, scratch);
@@ -504,34 +506,24 @@ template <class T, bool R> __device__ __forceinline__ void put(const Share<T, R>
     }
 }
 
-/* A (maximum, sum of exponentials below it) pair; the sum of two is taken at the larger maximum. */
-struct LogSum {
-    float top;
-    double sum;
-    __device__ __forceinline__ void add(float t, double s, double c) {
-        if (t == neg_inf() && s == 0.0) return; /* no entry; -inf with another sum: entries that are NaN */
-        if (top == neg_inf()) {
-            top = t, sum = s;
-        } else if (t <= top) {
-            sum += s * exp2(((double)t - (double)top) * c);
-        } else {
-            sum = sum * exp2(((double)top - (double)t) * c) + s;
-            top = t;
-        }
-    }
+/* What the blocks of a row know together, told to all threads of a block by its first warp. */
+struct RowSums {
+    float top, others_top;          /* maximum of the row, and of the entries not named (-inf: none) */
+    double sum, others_sum, cross;  /* sums of exponentials below those maxima */
 };
 
 /* BACKWARD: the statistics are given, and no block needs the others. */
-template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads) distill_rows(const DistillParams p) {
+template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const DistillParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 dynamic[];
     __shared__ double scratch[kWarps];
-    __shared__ Exchange ex;
+    __shared__ alignas(16) u64 told[kMaxCluster * kWarps][4];
+    __shared__ RowSums row_sums;
     __shared__ int twice;
     unsigned *map = reinterpret_cast<unsigned *>(dynamic);
     float *named_p = reinterpret_cast<float *>(map + p.map_words);
-    int *named_at = reinterpret_cast<int *>(named_p + kMaxK);
-    uint4 *stage = dynamic + (p.map_words + 2 * kMaxK) / 4;
+    int *named_at = reinterpret_cast<int *>(named_p + p.k);
+    uint4 *stage = dynamic + (p.map_words + 2 * p.k + 3) / 4;
     const unsigned size = cluster_size(), rank = cluster_rank();
     const long long row = blockIdx.x / size;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -603,32 +595,42 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
     if (!BACKWARD) {
         /* the rest of the row (all of it without teacher_lse) and the named entries, each as maximum and sum */
         const bool rest = p.teacher_lse != nullptr;
-        float most = neg_inf(), most_named = neg_inf();
-        auto get = [&](int v, float *f) {
-            Elem<T>::unpack(share.get(v), f);
-            if (rest) {
+        if (R && rest) { /* named entries leave the staged row; their scores are in z */
+#pragma unroll
+            for (int i = 0; i < Teacher::M; ++i)
+                if (first[i]) reinterpret_cast<T *>(stage)[teacher.at[i] - origin] = Elem<T>::down(neg_inf());
+            __syncthreads();
+        }
+        auto get = [&](int v) {
+            uint4 w = share.get(v);
+            if (!R && rest) {
                 const int e = (v - share.v0) * E;
                 const unsigned m = map[e >> 5] >> (e & 31);
+                float f[E];
+                Elem<T>::unpack(w, f);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     if ((m >> i) & 1u) f[i] = neg_inf();
+                w = Elem<T>::pack(f);
             }
+            return w;
         };
+        typename Elem<T>::Max largest;
+#pragma unroll 4
+        for (int v = share.first; v < share.last; v += 32) largest.add(get(v));
+        const float most = warp_max(largest.get()), base = most > neg_inf() ? most : 0.0f;
+        const Pair less(-base, -base), by(c, c);
+        Pair part[2] = {Pair(0.0f, 0.0f), Pair(0.0f, 0.0f)};
+#pragma unroll 2
         for (int v = share.first; v < share.last; v += 32) {
             float f[E];
-            get(v, f);
+            Elem<T>::unpack(get(v), f);
 #pragma unroll
-            for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
+            for (int i = 0; i < E / 2; ++i) part[i & 1] = part[i & 1] + fast_exp2((Pair(f[2 * i], f[2 * i + 1]) + less) * by);
         }
-        most = warp_max(most);
-        const float base = most > neg_inf() ? most : 0.0f;
-        float sum = 0.0f;
-        for (int v = share.first; v < share.last; v += 32) {
-            float f[E];
-            get(v, f);
-#pragma unroll
-            for (int i = 0; i < E; ++i) sum += exp2f((f[i] - base) * c);
-        }
+        float part_a, part_b;
+        (part[0] + part[1]).get(part_a, part_b);
+        float most_named = neg_inf();
         double named_sum = 0.0, cross = 0.0;
         if (rest) {
 #pragma unroll
@@ -644,33 +646,47 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
 #pragma unroll
         for (int i = 0; i < Teacher::M; ++i)
             if (counts[i] && teacher.p[i] > 0.0) cross += teacher.p[i] * (teacher.logp[i] - (double)z[i] / p.temperature);
-        const double s0 = warp_sum((double)sum), s1 = warp_sum(named_sum), s2 = warp_sum(cross);
+        const double s0 = warp_sum((double)part_a + (double)part_b), s1 = warp_sum(named_sum), s2 = warp_sum(cross);
         if (size > 1) cluster_wait();
         if (lane < (int)size) {
-            const unsigned to = peer_addr(shared_addr(&ex.word[0][rank * kWarps + warp][0]), lane);
+            const unsigned to = peer_addr(shared_addr(&told[rank * kWarps + warp][0]), lane);
             peer_store(to, __double_as_longlong(s0), __double_as_longlong(s1));
             peer_store(to + 16, __double_as_longlong(s2), (u64)__float_as_uint(most) << 32 | __float_as_uint(most_named));
         }
         cluster_sync(size);
-        LogSum others{neg_inf(), 0.0}, all{neg_inf(), 0.0};
-        cross = 0.0;
-        for (int i = 0; i < (int)size * kWarps; ++i) {
-            const u64 *w = ex.word[0][i];
-            others.add(__uint_as_float((unsigned)(w[3] >> 32)), __longlong_as_double((long long)w[0]), cd);
-            all.add(__uint_as_float((unsigned)w[3]), __longlong_as_double((long long)w[1]), cd);
-            cross += __longlong_as_double((long long)w[2]);
+        if (warp == 0) {
+            const int n = (int)size * kWarps;
+            float others_top = neg_inf(), row_top = neg_inf();
+            for (int i = lane; i < n; i += 32) {
+                others_top = fmaxf(others_top, __uint_as_float((unsigned)(told[i][3] >> 32)));
+                row_top = fmaxf(row_top, __uint_as_float((unsigned)told[i][3]));
+            }
+            others_top = warp_max(others_top), row_top = fmaxf(others_top, warp_max(row_top));
+            double others_sum = 0.0, sum = 0.0, crosses = 0.0;
+            for (int i = lane; i < n; i += 32) {
+                /* a sum that is 0 belongs to no entry; one that is not, at a maximum of -inf, to entries that are NaN */
+                const double a = __longlong_as_double((long long)told[i][0]), b = __longlong_as_double((long long)told[i][1]);
+                const double at_a = __uint_as_float((unsigned)(told[i][3] >> 32)), at_b = __uint_as_float((unsigned)told[i][3]);
+                if (a != 0.0) others_sum += a * exp2((at_a - (double)others_top) * cd);
+                if (b != 0.0) sum += b * exp2((at_b - (double)row_top) * cd);
+                crosses += __longlong_as_double((long long)told[i][2]);
+            }
+            others_sum = warp_sum(others_sum), sum = warp_sum(sum), crosses = warp_sum(crosses);
+            if (others_sum != 0.0) sum += others_sum * exp2(((double)others_top - (double)row_top) * cd);
+            if (lane == 0) row_sums = RowSums{row_top, others_top, sum, others_sum, crosses};
         }
-        all.add(others.top, others.sum, cd);
+        __syncthreads();
+        const RowSums all = row_sums;
         if (all.top == neg_inf() && all.sum == 0.0) { /* the student excludes every entry: the same in every block of the row */
             nothing();
             return;
         }
         const double lse = (double)all.top / p.temperature + log(all.sum);
-        double loss = cross + teacher.named * lse, factor = teacher.named, other = teacher.named;
+        double loss = all.cross + teacher.named * lse, factor = teacher.named, other = teacher.named;
         if (rest) {
             const double r = 1.0 - teacher.named;
-            if (r > 0.0 && others.top > neg_inf()) {
-                const double log_share = (double)others.top / p.temperature + log(others.sum) - lse;
+            if (r > 0.0 && all.others_top > neg_inf()) {
+                const double log_share = (double)all.others_top / p.temperature + log(all.others_sum) - lse;
                 loss += r * (log(r) - log_share);
                 factor += r;
                 other = factor - r * exp(-log_share);
@@ -693,11 +709,14 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
     float g = (float)((double)weight / p.temperature);
     if (BACKWARD && p.upstream) g *= p.upstream[row];
     const float factor = g * elsewhere * inverse;
+    const Pair times(factor, factor), less(-top, -top), by(c, c);
+#pragma unroll 2
     for (int v = share.first; v < share.last; v += 32) {
         float f[E];
         Elem<T>::unpack(share.get(v), f);
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = factor * exp2f((f[i] - top) * c);
+        for (int i = 0; i < E / 2; ++i)
+            (times * fast_exp2((Pair(f[2 * i], f[2 * i + 1]) + less) * by)).get(f[2 * i], f[2 * i + 1]);
         put(share, grad, same, v, f);
     }
     __syncthreads();
@@ -716,7 +735,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
                 }
             if (earlier) continue;
         }
-        const float q = inverse * exp2f((z[i] - top) * c);
+        const float q = inverse * fast_exp2((z[i] - top) * c);
         grad[teacher.at[i]] = Elem<T>::down(g * (float)((double)at_named * q - named));
     }
 }
@@ -791,8 +810,7 @@ static int launch_rows(accb_context *ctx, void (*resident)(const P), void (*stre
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)size;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof cfg);
+    cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a->rows * size));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
@@ -866,7 +884,7 @@ static int distill(accb_context *ctx, accb_stream stream, const accb_rows_array 
     const long long e = 16 / (long long)size_of(student->type);
     const long long share = ((student->cols + 2 * e - 2) / e + size - 1) / size * e; /* entries of a block's share, at most */
     p.map_words = (int)((share + 31) / 32 + 3) & ~3;
-    const size_t fixed = (size_t)p.map_words * 4 + 8 * kMaxK;
+    const size_t fixed = (size_t)(p.map_words + 2 * p.k + 3) / 4 * 16;
 #define CALL(T)                                                                                                                       \
     (backward ? launch_rows(ctx, distill_rows<T, true, true>, distill_rows<T, false, true>, p, student, size, fixed, (cudaStream_t)stream, what) \
               : launch_rows(ctx, distill_rows<T, true, false>, distill_rows<T, false, false>, p, student, size, fixed, (cudaStream_t)stream, what))

@@ -50,6 +50,15 @@ template <> struct Elem<float> {
     }
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
+    /* running maximum of whole vectors; a NaN is passed over */
+    struct Max {
+        float m;
+        __device__ __forceinline__ Max() : m(-__builtin_huge_valf()) {}
+        __device__ __forceinline__ void add(const uint4 &w) {
+            m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w.x), __uint_as_float(w.y))), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+        }
+        __device__ __forceinline__ float get() const { return m; }
+    };
 };
 template <> struct Elem<__half> {
     static constexpr int E = 8;
@@ -74,6 +83,18 @@ template <> struct Elem<__half> {
     }
     static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+    struct Max {
+        unsigned m = 0xfc00fc00u;
+        static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+            const __half2 r = __hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+            return *reinterpret_cast<const unsigned *>(&r);
+        }
+        __device__ __forceinline__ void add(const uint4 &w) { m = larger(larger(m, larger(w.x, w.y)), larger(w.z, w.w)); }
+        __device__ __forceinline__ float get() const {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&m));
+            return fmaxf(p.x, p.y);
+        }
+    };
 };
 template <> struct Elem<__nv_bfloat16> {
     static constexpr int E = 8;
@@ -95,7 +116,50 @@ template <> struct Elem<__nv_bfloat16> {
     }
     static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+    struct Max {
+        unsigned m = 0xff80ff80u;
+        static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+            const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+            return *reinterpret_cast<const unsigned *>(&r);
+        }
+        __device__ __forceinline__ void add(const uint4 &w) { m = larger(larger(m, larger(w.x, w.y)), larger(w.z, w.w)); }
+        __device__ __forceinline__ float get() const {
+            const float2 p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&m));
+            return fmaxf(p.x, p.y);
+        }
+    };
 };
+
+/* ------------------------------------------- two 32-bit floats at a time
+ * Blackwell adds, multiplies and fuses pairs of 32-bit floats in one instruction; the passes over a row are bound by
+ * instruction issue, so they use them. */
+struct Pair {
+    u64 v;
+    __device__ __forceinline__ Pair() {}
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+/* 2^x by the special function unit (relative error 2^-22, results below 2^-126 are 0) */
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ Pair fast_exp2(Pair x) {
+    float a, b;
+    x.get(a, b);
+    return Pair(fast_exp2(a), fast_exp2(b));
+}
 
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xff800000u); }
 /* a NaN is an entry that cannot be chosen, like -inf (fmaxf returns the operand that is a number) */
@@ -206,8 +270,7 @@ template <class T, bool RESIDENT> struct Share {
     }
     /* start the copies of this thread's vectors; wait() before the first get() */
     __device__ __forceinline__ void fetch() const {
-        if (!RESIDENT) return;
-        for (int v = first; v < last; v += 32) {
+        for (int v = RESIDENT ? first : last; v < last; v += 32) {
             if (whole(v))
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(stage + (v - v0))),
                              "l"(reinterpret_cast<const uint4 *>(base) + v)
