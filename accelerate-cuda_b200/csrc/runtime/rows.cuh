@@ -228,6 +228,33 @@ struct Exchange {
 };
 
 /* ----------------------------------------------------------------- rows */
+/* A block runs most of its code once per row, so what counts of rarely run code is its size: every instruction that
+ * is not in the SM's instruction cache is waited for.  Edges and 64-bit functions are therefore calls. */
+template <class T> __device__ __noinline__ uint4 edge(const T *base, int v, int lead, int n) {
+    constexpr int E = Elem<T>::E;
+    T f[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int e = v * E - lead + i;
+        f[i] = e >= 0 && e < n ? base[v * E + i] : Elem<T>::down(neg_inf());
+    }
+    uint4 w;
+    memcpy(&w, f, sizeof w);
+    return w;
+}
+template <class T> __device__ __noinline__ void put_edge(T *row, int v, int lead, int n, uint4 w) {
+    constexpr int E = Elem<T>::E;
+    T f[E];
+    memcpy(f, &w, sizeof w);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int e = v * E - lead + i;
+        if (e >= 0 && e < n) row[e] = f[i];
+    }
+}
+static __device__ __noinline__ double exp_64(double x) { return exp(x); }
+static __device__ __noinline__ double log_64(double x) { return log(x); }
+
 /* A block's share of one row, in vectors of 16 bytes counted from the row's address rounded down to 16 bytes.
  * Entries of an edge vector that lie outside the row read as -inf. */
 template <class T, bool RESIDENT> struct Share {
@@ -256,17 +283,8 @@ template <class T, bool RESIDENT> struct Share {
     __device__ __forceinline__ int entry(int v) const { return v * E - lead; } /* index of a vector's first entry */
     __device__ __forceinline__ bool whole(int v) const { return entry(v) >= 0 && entry(v) + E <= n; }
 
-    __device__ __forceinline__ uint4 edge(int v) const {
-        uint4 w = make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
-        float f[E];
-        Elem<T>::unpack(w, f);
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (entry(v) + i >= 0 && entry(v) + i < n) f[i] = Elem<T>::up(base[(long long)v * E + i]);
-        return Elem<T>::pack(f);
-    }
     __device__ __forceinline__ uint4 from_memory(int v) const {
-        return whole(v) ? reinterpret_cast<const uint4 *>(base)[v] : edge(v);
+        return whole(v) ? reinterpret_cast<const uint4 *>(base)[v] : edge<T>(base, v, lead, n);
     }
     /* start the copies of this thread's vectors; wait() before the first get() */
     __device__ __forceinline__ void fetch() const {
@@ -276,7 +294,7 @@ template <class T, bool RESIDENT> struct Share {
                              "l"(reinterpret_cast<const uint4 *>(base) + v)
                              : "memory");
             else
-                stage[v - v0] = edge(v);
+                stage[v - v0] = edge<T>(base, v, lead, n);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -285,6 +303,15 @@ template <class T, bool RESIDENT> struct Share {
     }
     __device__ __forceinline__ uint4 get(int v) const { return RESIDENT ? stage[v - v0] : from_memory(v); }
 };
+
+/* a vector of a result row laid out like the share's row; 16-byte stores where both start at the same place of a
+ * 16-byte word */
+template <class T, bool R> __device__ __forceinline__ void put(const Share<T, R> &share, T *row, bool same, int v, const uint4 &w) {
+    if (same && share.whole(v))
+        *reinterpret_cast<uint4 *>(row + share.entry(v)) = w;
+    else
+        put_edge<T>(row, v, share.lead, share.n, w);
+}
 
 /* --------------------------------------------------------- reductions */
 __device__ __forceinline__ float warp_max(float v) {
