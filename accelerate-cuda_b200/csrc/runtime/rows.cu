@@ -20,6 +20,104 @@ struct RowsIn {
     int cols;
 };
 
+/* ----------------------------------------------------- finding candidates */
+/* A vector of a row as this block sees it: entries that `bits` does not allow are -inf. */
+template <class T> __device__ __noinline__ uint4 only_allowed(uint4 w, int e0, int n, const unsigned *bits) {
+    constexpr int E = Elem<T>::E;
+    float f[E];
+    Elem<T>::unpack(w, f);
+    unsigned m = 0;
+    if (e0 >= 0 && e0 + E <= n) {
+        const unsigned lo = bits[e0 >> 5], hi = (e0 & 31) + E > 32 ? bits[(e0 >> 5) + 1] : 0u;
+        m = __funnelshift_r(lo, hi, e0 & 31);
+    } else {
+        for (int i = 0; i < E; ++i)
+            if (e0 + i >= 0 && e0 + i < n) m |= ((bits[(e0 + i) >> 5] >> ((e0 + i) & 31)) & 1u) << i;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (!((m >> i) & 1u)) f[i] = neg_inf();
+    return Elem<T>::pack(f);
+}
+
+/* Where a row's candidates are gathered: in the first block of its cluster. */
+struct Gather {
+    unsigned own;   /* entries of this block */
+    unsigned count; /* in the first block: places of the list that are taken */
+    unsigned base;  /* where this block's go */
+};
+
+/* Lists the entries of the row that are not below `least` (finite) in the first block's `list` of `room` numbers.
+ * Every block lists its own first: a place in its own shared memory costs a fraction of one in another block's.  The
+ * counts still have to be told; returns this block's. */
+template <class T, bool R, class Raw>
+__device__ unsigned gather(const Share<T, R> &share, Raw raw, float least, u64 *list, unsigned room, Gather &g, unsigned rank) {
+    constexpr int E = Elem<T>::E;
+#pragma unroll 2
+    for (int v = share.first; v < share.last; v += 32) {
+        const uint4 w = raw(v);
+        typename Elem<T>::Max largest;
+        largest.add(w);
+        if (!(largest.get() >= least)) continue;
+        float f[E];
+        Elem<T>::unpack(w, f);
+#pragma unroll 1
+        for (int i = 0; i < E; ++i) {
+            float x = f[0];
+#pragma unroll
+            for (int j = 1; j < E; ++j)
+                if (i == j) x = f[j];
+            if (x >= least) {
+                unsigned at = atomicAdd(&g.own, 1u);
+                if (rank == 0) at = atomicAdd(&g.count, 1u);
+                if (at < room) list[at] = entry_of(x, share.entry(v) + i);
+            }
+        }
+    }
+    __syncthreads();
+    const unsigned n = g.own;
+    if (rank != 0 && n != 0) {
+        if (threadIdx.x == 0) g.base = peer_count(peer_addr(shared_addr(&g.count), 0), n);
+        __syncthreads();
+        const unsigned to = peer_addr(shared_addr(list), 0), base = g.base;
+        for (unsigned i = threadIdx.x; i < min(n, room); i += kThreads)
+            if (base + i < room) peer_store1(to + (base + i) * 8, list[i]);
+    }
+    return n;
+}
+
+/* One message of every block to all blocks of its cluster, and the barrier after it; every exchange of a launch has a
+ * buffer of its own. */
+struct Told {
+    alignas(16) u64 block[3][kMaxCluster][2];
+    alignas(16) u64 warp[kMaxCluster * kWarps][2];
+};
+__device__ __forceinline__ void tell_all(u64 (&buffer)[kMaxCluster][2], u64 a, u64 b, unsigned rank, unsigned size) {
+    if (threadIdx.x < size) peer_store(peer_addr(shared_addr(&buffer[rank][0]), threadIdx.x), a, b);
+    cluster_sync(size);
+}
+
+/* sums over the block, the same in all threads; two barriers */
+__device__ __forceinline__ u64 block_sum(u64 v, u64 *scratch) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    u64 s = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += scratch[w];
+    __syncthreads();
+    return s;
+}
+/* sum over the threads before this one and itself */
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *scratch) {
+    v = warp_scan(v);
+    if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) v += scratch[w];
+    __syncthreads();
+    return v;
+}
+
 /* ------------------------------------------------------------- sampling */
 struct SampleParams {
     RowsIn in;
@@ -30,33 +128,76 @@ struct SampleParams {
     int *token;
     float *logprob;
 };
+constexpr int kSampleRoom = 1024; /* candidates of a row that a block sorts */
 
-/* the entries of vector v that `bits` (one per entry of the row) does not allow become -inf */
-template <class T, bool R> __device__ __forceinline__ uint4 only_allowed(const Share<T, R> &share, int v, uint4 w, const unsigned *bits) {
-    constexpr int E = Elem<T>::E;
-    float f[E];
-    Elem<T>::unpack(w, f);
-    const int e0 = share.entry(v);
-    unsigned m = 0;
-    if (share.whole(v)) {
-        const unsigned lo = bits[e0 >> 5], hi = (e0 & 31) + E > 32 ? bits[(e0 >> 5) + 1] : 0u;
-        m = __funnelshift_r(lo, hi, e0 & 31);
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (e0 + i >= 0 && e0 + i < share.n) m |= ((bits[(e0 + i) >> 5] >> ((e0 + i) & 31)) & 1u) << i;
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-        if (!((m >> i) & 1u)) f[i] = neg_inf();
-    return Elem<T>::pack(f);
+/* the whole part of uniform * total below total */
+__device__ __forceinline__ u64 drawn(float uniform, u64 total) {
+    const double want = floor((double)uniform * (double)total);
+    return want > 0.0 ? min((u64)want, total - 1) : 0;
 }
 
-template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_rows(const SampleParams p) {
+__device__ __forceinline__ void put_token(const SampleParams &p, long long row, int index, float value, float most, double temperature, u64 total) {
+    p.token[row] = index;
+    if (p.logprob) {
+        const double below = value == most ? 0.0 : ((double)value - (double)most) / temperature;
+        p.logprob[row] = (float)(below - log_64((double)total * (1.0 / (double)(1ull << kUnitLog2))));
+    }
+}
+
+/* Draws from the n candidates in `list`, which hold every entry that top_k and top_p could keep; by one block. */
+template <class W>
+__device__ __noinline__ void draw_from_list(const SampleParams &p, long long row, u64 *list, u64 *scratch, int n, int k, float top_p,
+                                                   float lowest, u64 total, float uniform, double temperature, float most, const W &weigh) {
+    sort_down(list, n, kSampleRoom);
+    if (k > 0) n = min(n, k);
+    /* weights, and how many of the sorted candidates are kept: a thread has `per` of them side by side */
+    const int per = (n + kThreads - 1) / kThreads, from = min(n, (int)threadIdx.x * per), to = min(n, from + per);
+    u64 mine = 0;
+    for (int i = from; i < to; ++i) mine += weigh.weight(score_of(list[i]));
+    u64 upto = block_scan(mine, scratch);
+    if (total == 0) total = block_sum(mine, scratch);
+    const u64 limit = top_p < 1.0f ? (u64)ceil((top_p > 0.0f ? (double)top_p : 0.0) * (double)total) : ~0ull;
+    u64 before = upto - mine, kept = 0;
+    for (int i = from; i < to; ++i) {
+        const float x = score_of(list[i]);
+        const u64 w = weigh.weight(x);
+        const bool keep = (before < limit || i == 0) && x >= lowest;
+        before += w;
+        kept += keep ? w : 0;
+        /* next: in the order of the indices, without the keys of those that are not kept */
+        list[i] = list[i] << 32 | (keep ? key_of(x) : 0u);
+    }
+    total = block_sum(kept, scratch);
+    const u64 target = drawn(uniform, total);
+    sort_down(list, n, kSampleRoom);
+    mine = 0;
+    for (int i = from; i < to; ++i)
+        if ((unsigned)list[i]) mine += weigh.weight(value_of((unsigned)list[i]));
+    upto = block_scan(mine, scratch);
+    before = upto - mine;
+    if (before <= target && target < upto) {
+        for (int i = from; i < to; ++i) {
+            const float x = value_of((unsigned)list[i]);
+            if ((unsigned)list[i]) before += weigh.weight(x);
+            if (target < before) {
+                put_token(p, row, index_of(list[i] >> 32), x, most, temperature, total);
+                return;
+            }
+        }
+    }
+}
+
+template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample_rows(const __grid_constant__ SampleParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 stage[];
-    __shared__ Exchange ex;
-    __shared__ Level lv;
+    __shared__ Told told;
+    __shared__ union {
+        Level level;
+        u64 list[kSampleRoom];
+    } sh;
+    __shared__ double table[kTable * kTableCopies];
+    __shared__ u64 scratch[kWarps];
+    __shared__ Gather g;
     const unsigned size = cluster_size(), rank = cluster_rank();
     const long long row = blockIdx.x / size;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -66,47 +207,61 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_ro
     share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
     share.fetch();
     const unsigned *bits = p.allowed ? p.allowed + row * p.allowed_pitch : nullptr;
-    float temperature = p.temperature ? p.temperature[row] : 1.0f;
-    const bool greedy = !(temperature > 0.0f);
-    if (greedy) temperature = 1.0f;
+    float warmth = p.temperature ? p.temperature[row] : 1.0f;
     int k = p.top_k ? p.top_k[row] : 0;
-    if (greedy) k = 1;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     const float min_p = p.min_p ? p.min_p[row] : 0.0f;
     const float uniform = p.uniform[row];
+    if (!(warmth > 0.0f)) k = 1;
+    const double temperature = warmth > 0.0f ? warmth : 1.0f;
+    if (k >= p.in.cols || k < 0) k = 0;
+    fill_table(table);
+    if (threadIdx.x == 0) g.own = g.count = 0;
     share.wait();
 
-    auto get = [&](int v, float *f) {
+    bool infinite = false; /* the row's maximum is +inf: its like weigh 1, all others nothing */
+    auto raw = [&](int v) {
         uint4 w = share.get(v);
-        if (!R && bits) w = only_allowed(share, v, w, bits);
-        Elem<T>::unpack(w, f);
+        if (!R) {
+            if (bits) w = only_allowed<T>(w, share.entry(v), share.n, bits);
+            if (infinite) {
+                float f[E];
+                Elem<T>::unpack(w, f);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] = f[i] == __uint_as_float(0x7f800000u) ? 0.0f : neg_inf();
+                w = Elem<T>::pack(f);
+            }
+        }
+        return w;
+    };
+    auto get = [&](int v, float *f) {
+        Elem<T>::unpack(raw(v), f);
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = not_nan(f[i]);
     };
 
-    /* the maximum, and the smallest of the threads' maxima: at least that many entries are as large */
-    float most = neg_inf();
+    /* the maximum, and where at least k entries lie above: a k-th part of the blocks' threads in each block */
+    typename Elem<T>::Max largest;
+#pragma unroll 4
     for (int v = share.first; v < share.last; v += 32) {
-        if (R && bits) stage[v - share.v0] = only_allowed(share, v, stage[v - share.v0], bits);
-        float f[E];
-        get(v, f);
+        uint4 w = raw(v);
+        if (R && bits) stage[v - share.v0] = w = only_allowed<T>(w, share.entry(v), share.n, bits);
+        largest.add(w);
+    }
+    float most = largest.get(), bound = neg_inf();
+    const int want = (k + (int)size - 1) / (int)size; /* of each block's threads */
+    if (k > 1 && k <= kSampleRoom && want <= kThreads) bound = bound_of(most, want);
+    most = warp_max(most);
+    if (lane == 0) scratch[warp] = __float_as_uint(most);
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
-    }
-    const float warp_most = warp_max(most), warp_least = warp_min(most);
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, __uint_as_float((unsigned)scratch[w]));
     if (size > 1) cluster_wait();
-    auto tell = [&](int buffer, u64 a, u64 b) {
-        if (lane < (int)size) peer_store(peer_addr(shared_addr(&ex.word[buffer][rank * kWarps + warp][0]), lane), a, b);
-        cluster_sync(size);
-    };
-    tell(0, __float_as_uint(warp_most), __float_as_uint(warp_least));
-    float least = __uint_as_float(0x7f800000u);
-    most = neg_inf();
-    for (int i = lane; i < (int)size * kWarps; i += 32) {
-        most = fmaxf(most, __uint_as_float((unsigned)ex.word[0][i][0]));
-        least = fminf(least, __uint_as_float((unsigned)ex.word[0][i][1]));
+    tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
+    for (int i = 0; i < (int)size; ++i) {
+        most = fmaxf(most, __uint_as_float((unsigned)told.block[0][i][0]));
+        bound = fminf(bound, __uint_as_float((unsigned)told.block[0][i][1]));
     }
-    most = warp_max(most), least = warp_min(least);
     if (most == neg_inf()) { /* nothing may be drawn: the same in every block of the row */
         if (rank == 0 && threadIdx.x == 0) {
             p.token[row] = -1;
@@ -114,81 +269,127 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_ro
         }
         return;
     }
-    const Scale scale{most, 1.4426950408889634 / (double)temperature};
-
-    /* the border of what is kept, beginning with every entry above -inf */
-    Border border{key_of(neg_inf()), 0, 0};
-    unsigned spare = 0;
-    bool cut = false;
-    if (k == 1) {
-        border = Border{key_of(most), 1, 1};
-    } else {
-        if (k > 0 && k < p.in.cols) {
-            const float from = k <= (int)size * kThreads ? least : neg_inf();
-            border = find_border<T, R, false>(share, get, lv, size, key_of(from), key_of(most), (u64)k, scale, 0.0, 0, 0);
-            spare = border.equals - border.ties;
-            cut = true;
-        }
-        if (top_p < 1.0f) {
-            u64 total = 0;
-            unsigned from = border.key;
-            if (!cut) {
-                u64 mine = 0;
-                for (int v = share.first; v < share.last; v += 32) {
-                    float f[E];
-                    get(v, f);
+    if (most == __uint_as_float(0x7f800000u)) {
+        if (R) {
+            for (int v = share.first; v < share.last; v += 32) {
+                float f[E];
+                get(v, f);
 #pragma unroll
-                    for (int i = 0; i < E; ++i) mine += scale.weight(f[i]);
-                }
-                tell(1, warp_sum(mine), 0);
-                for (int i = lane; i < (int)size * kWarps; i += 32) total += ex.word[1][i][0];
-                total = warp_sum(total);
-                /* entries so far below the maximum that all of them together weigh less than what is cut off */
-                const double left = 1.0 - (double)top_p;
-                const double low = (double)most - (log((double)p.in.cols / left) + 1.0) * (double)temperature;
-                if (left > 1e-5 && low > -3.0e38) from = key_of(__double2float_rd(low));
+                for (int i = 0; i < E; ++i) f[i] = f[i] == most ? 0.0f : neg_inf();
+                stage[v - share.v0] = Elem<T>::pack(f);
             }
-            const Border b = find_border<T, R, true>(share, get, lv, size, from, key_of(most), 0, scale, top_p > 0.0f ? (double)top_p : 0.0,
-                                                     total, spare);
+        }
+        infinite = true;
+        most = 0.0f, bound = neg_inf();
+    }
+
+    /* the lowest score that min_p keeps */
+    float lowest = -3.402823466e+38f;
+    if (min_p > 0.0f) {
+        const double low = (double)most + log_64(fmin((double)min_p, 1.0)) * temperature;
+        if (low > -3.0e38) lowest = __double2float_ru(low);
+    }
+    const Weigh<sizeof(T) == 4> weigh(most, temperature, table);
+    if (k == 1) bound = most;
+
+    /* the weight of the whole row, or of what min_p keeps where nothing else cuts: a warp's own in quarters, whose sums
+     * its lanes keep for the end */
+    u64 quarter[4] = {0, 0, 0, 0};
+    const int start = share.first - lane; /* of the warp's piece */
+    const int per_quarter = (max(0, share.last - start) + 127) >> 7;
+    u64 total = 0;
+    const bool cut = k > 0 || top_p < 1.0f;
+    if (k == 0) {
+        const float from = cut ? weigh.least : fmaxf(weigh.least, lowest);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
+#pragma unroll 1
+            for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
+                float f[E];
+                Elem<T>::unpack(raw(v), f);
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (f[i] >= from) quarter[q] += weigh.of(f[i]);
+            }
+        }
+    }
+    Border border{key_of(cut ? neg_inf() : fmaxf(lowest, -3.402823466e+38f)) - (cut ? 0u : 1u), 0, 0};
+    if (cut) {
+        if (k == 0) { /* top_p alone: entries so far down that all of them together weigh less than what is cut off */
+            const u64 block_total = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
+            tell_all(told.block[1], block_total, 0, rank, size);
+            for (int i = 0; i < (int)size; ++i) total += told.block[1][i][0];
+            const double left = (1.0 - (double)top_p) * ((double)total * (1.0 / (double)(1ull << kUnitLog2)));
+            const double low = (double)most + (log_64(left / (double)p.in.cols) - 0.01) * temperature;
+            bound = left > 1e-5 && low > -3.0e38 ? __double2float_rd(low) : neg_inf();
+        }
+        const float least = fmaxf(bound, -3.402823466e+38f);
+        const unsigned n = gather(share, raw, least, sh.list, kSampleRoom, g, rank);
+        tell_all(told.block[2], n, 0, rank, size);
+        unsigned all = 0;
+        for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[2][i][0];
+        if (all <= kSampleRoom) { /* the same in every block of the row */
+            if (rank == 0)
+                draw_from_list(p, row, sh.list, scratch, (int)all, k, top_p, lowest, k > 0 ? 0 : total, uniform, temperature,
+                               most, weigh);
+            return;
+        }
+        /* too many: the border of what is kept, from counts and weights of ranges of scores */
+        unsigned spare = 0;
+        if (k > 0) {
+            border = k == 1 ? Border{key_of(most), 1, 1}
+                            : find_border<T, R, false>(share, get, sh.level, size, key_of(bound), key_of(most), (u64)k, weigh, 0.0, 0, 0);
+            spare = k == 1 ? 0 : border.equals - border.ties;
+        }
+        if (top_p < 1.0f && k != 1) {
+            const unsigned from = k > 0 ? border.key : key_of(bound);
+            const Border b = find_border<T, R, true>(share, get, sh.level, size, from, key_of(most), 0, weigh, top_p > 0.0f ? (double)top_p : 0.0, total, spare);
             if (b.ties != 0xffffffffu) border = b;
         }
-        if (min_p > 0.0f) {
-            /* the lowest value whose share is min_p of the maximum's */
-            const double low = (double)most + log(fmin((double)min_p, 1.0)) * (double)temperature;
-            const unsigned below = key_of(low > -3.0e38 ? __double2float_ru(low) : neg_inf()) - 1u;
-            if (below >= border.key) border = Border{below, 0, 0};
-        }
+        const unsigned below = key_of(lowest) - 1u;
+        if (below >= border.key) border = Border{below, 0, 0};
     }
 
     /* weight above the border and number of entries on it, by warp; every warp then knows what precedes it */
-    u64 mass = 0;
     unsigned ties = 0;
-    for (int v = share.first; v < share.last; v += 32) {
-        float f[E];
-        get(v, f);
+    if (cut) {
+        const float from = weigh.least;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const unsigned key = key_of(f[i]);
-            if (key > border.key) mass += scale.weight(f[i]);
-            ties += key == border.key;
+        for (int q = 0; q < 4; ++q) {
+            quarter[q] = 0;
+            const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
+#pragma unroll 1
+            for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
+                float f[E];
+                get(v, f);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const unsigned key = key_of(f[i]);
+                    if (key > border.key && f[i] >= from) quarter[q] += weigh.of(f[i]);
+                    ties += key == border.key;
+                }
+            }
         }
+        ties = warp_sum(ties);
     }
-    mass = warp_sum(mass);
-    ties = warp_sum(ties);
-    tell(2, mass, ties);
-    const u64 tie_weight = border.ties ? scale.weight(value_of(border.key)) : 0;
+    const u64 mass = warp_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]));
+    if (lane < (int)size) peer_store(peer_addr(shared_addr(&told.warp[rank * kWarps + warp][0]), lane), mass, ties);
+    cluster_sync(size);
+    const u64 tie_weight = border.ties ? weigh.weight(value_of(border.key)) : 0;
     const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
-    u64 total = 0, before = 0;
-    unsigned ties_seen = 0, ties_before = 0, quota = 0;
+    u64 before = 0;
+    total = 0;
+    unsigned ties_seen = 0, quota = 0;
     for (int i0 = 0; i0 < nwarps; i0 += 32) {
         const int i = i0 + lane;
-        const u64 m = i < nwarps ? ex.word[2][i][0] : 0;
-        const unsigned n = i < nwarps ? (unsigned)ex.word[2][i][1] : 0;
+        const u64 m = i < nwarps ? told.warp[i][0] : 0;
+        const unsigned n = i < nwarps ? (unsigned)told.warp[i][1] : 0;
         const unsigned upto = ties_seen + warp_scan(n);
         const unsigned kept = min(upto, border.ties) - min(upto - n, border.ties);
         const u64 w = m + kept * tie_weight;
         const u64 sum = total + warp_scan(w);
-        if (i == self) before = sum - w, ties_before = upto - n, quota = kept;
+        if (i == self) before = sum - w, quota = kept;
         total = __shfl_sync(~0u, sum, 31);
         ties_seen = __shfl_sync(~0u, upto, 31);
     }
@@ -196,14 +397,20 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_ro
     quota = __shfl_sync(~0u, quota, self & 31);
     const u64 here = mass + quota * tie_weight;
     /* the first entry whose running sum exceeds uniform * total */
-    const double want = floor((double)uniform * (double)total);
-    const u64 target = want > 0.0 ? min((u64)want, total - 1) : 0;
+    const u64 target = drawn(uniform, total);
     if (!(before <= target && target < before + here)) return;
 
+    int v0 = start;
+    if (quota == 0) { /* which quarter of the warp's piece */
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const u64 w = warp_sum(quarter[q]);
+            if (v0 == start + 32 * per_quarter * q && before + w <= target) before += w, v0 += 32 * per_quarter;
+        }
+    }
     unsigned left = quota;
     u64 sum = before;
-    const int base = share.first - lane;
-    for (int v0 = base; v0 < share.last; v0 += 32) {
+    for (; v0 < share.last; v0 += 32) {
         const int v = v0 + lane;
         float f[E];
 #pragma unroll
@@ -220,7 +427,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_ro
             const unsigned key = key_of(f[i]);
             w[i] = 0;
             if (key > border.key) {
-                w[i] = scale.weight(f[i]);
+                w[i] = weigh.weight(f[i]);
             } else if (key == border.key && may) {
                 w[i] = tie_weight;
                 --may;
@@ -240,11 +447,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads) sample_ro
                     c += w[i];
                     if (!done && target < c) at = share.entry(v) + i, value = f[i], done = true;
                 }
-                p.token[row] = at;
-                if (p.logprob) {
-                    const double share_log = value == most ? 0.0 : ((double)value - (double)most) / (double)temperature;
-                    p.logprob[row] = (float)(share_log - log((double)total * (1.0 / (double)(1ull << kUnitLog2))));
-                }
+                put_token(p, row, at, value, most, temperature, total);
             }
             return;
         }
@@ -262,147 +465,142 @@ struct TopParams {
     float *lse;
     double temperature;
     int k;
+    int room; /* of the list of candidates, a power of two from 256 */
 };
 
-template <class T, bool R> __global__ void __launch_bounds__(kThreads) top_rows(const TopParams p) {
+template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_rows(const __grid_constant__ TopParams p) {
     constexpr int E = Elem<T>::E;
-    extern __shared__ uint4 stage[];
-    __shared__ Exchange ex;
-    __shared__ union {
-        Level lv;
-        u64 list[kMaxK]; /* of the first block of the row: key of the value, and 2^32 - 1 - index, so that larger comes first */
-    } sh;
-    __shared__ unsigned taken;
+    extern __shared__ uint4 dynamic[];
+    __shared__ Told told;
+    __shared__ u64 scratch[kWarps];
+    __shared__ Gather g;
     const unsigned size = cluster_size(), rank = cluster_rank();
     const long long row = blockIdx.x / size;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    u64 *list = reinterpret_cast<u64 *>(dynamic);
+    Level &level = *reinterpret_cast<Level *>(dynamic); /* in the list's place */
     if (size > 1) cluster_arrive();
 
     Share<T, R> share;
-    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, dynamic + max(p.room * 8, (int)sizeof(Level)) / 16);
     share.fetch();
-    if (threadIdx.x == 0) taken = 0;
+    if (threadIdx.x == 0) g.own = g.count = 0;
     share.wait();
+    auto raw = [&](int v) { return share.get(v); };
     auto get = [&](int v, float *f) {
         Elem<T>::unpack(share.get(v), f);
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = not_nan(f[i]);
     };
-    float most = neg_inf();
-    for (int v = share.first; v < share.last; v += 32) {
-        float f[E];
-        get(v, f);
-#pragma unroll
-        for (int i = 0; i < E; ++i) most = fmaxf(most, f[i]);
-    }
-    const float warp_most = warp_max(most), warp_least = warp_min(most);
-    if (size > 1) cluster_wait();
-    auto tell = [&](int buffer, u64 a, u64 b) {
-        if (lane < (int)size) peer_store(peer_addr(shared_addr(&ex.word[buffer][rank * kWarps + warp][0]), lane), a, b);
-        cluster_sync(size);
-    };
-    tell(0, __float_as_uint(warp_most), __float_as_uint(warp_least));
-    float least = __uint_as_float(0x7f800000u);
-    most = neg_inf();
-    for (int i = lane; i < (int)size * kWarps; i += 32) {
-        most = fmaxf(most, __uint_as_float((unsigned)ex.word[0][i][0]));
-        least = fminf(least, __uint_as_float((unsigned)ex.word[0][i][1]));
-    }
-    most = warp_max(most), least = warp_min(least);
-    if (most == neg_inf()) {
-        if (rank == 0) {
-            for (int i = threadIdx.x; i < p.k; i += kThreads) {
-                static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(neg_inf());
-                p.index[row * p.k + i] = -1;
-            }
-            if (p.lse && threadIdx.x == 0) p.lse[row] = neg_inf();
-        }
-        return;
-    }
-    const float from = p.k <= (int)size * kThreads ? least : neg_inf();
-    const Scale scale{most, 0.0};
-    const Border border = find_border<T, R, false>(share, get, sh.lv, size, key_of(from), key_of(most), (u64)p.k, scale, 0.0, 0, 0);
-
-    /* entries on the border and the sum of exponentials, by warp */
-    const float c = (float)(1.4426950408889634 / p.temperature);
-    unsigned ties = 0;
-    float sum = 0.0f;
-    for (int v = share.first; v < share.last; v += 32) {
-        float f[E];
-        get(v, f);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            ties += key_of(f[i]) == border.key;
-            if (p.lse) sum += f[i] == most ? 1.0f : exp2f((f[i] - most) * c);
-        }
-    }
-    ties = warp_sum(ties);
-    tell(1, ties, (u64)__double_as_longlong(warp_sum((double)sum)));
-    double all = 0.0;
-    unsigned quota = 0, seen = 0;
-    const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
-    for (int i0 = 0; i0 < nwarps; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned n = i < nwarps ? (unsigned)ex.word[1][i][0] : 0;
-        const unsigned upto = seen + warp_scan(n);
-        if (i == self) quota = min(upto, border.ties) - min(upto - n, border.ties);
-        seen = __shfl_sync(~0u, upto, 31);
-        if (i < nwarps) all += __longlong_as_double((long long)ex.word[1][i][1]);
-    }
-    quota = __shfl_sync(~0u, quota, self & 31);
-    all = warp_sum(all);
-    if (p.lse && rank == 0 && threadIdx.x == 0) p.lse[row] = (float)((double)most / p.temperature + log(all));
-
-    /* what is above the border, and the first of what is on it, goes to the first block of the row */
-    const unsigned lowest = key_of(neg_inf()), list = peer_addr(shared_addr(sh.list), 0), count = peer_addr(shared_addr(&taken), 0);
-    for (int v0 = share.first - lane; v0 < share.last; v0 += 32) {
-        const int v = v0 + lane;
-        float f[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = neg_inf();
-        if (v < share.last) get(v, f);
-        unsigned on = 0, above = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const unsigned key = key_of(f[i]);
-            if (key > lowest && v < share.last) on |= (unsigned)(key == border.key) << i, above |= (unsigned)(key > border.key) << i;
-        }
-        if (!__any_sync(~0u, on | above)) continue;
-        const unsigned n = __popc(on), upto = warp_scan(n);
-        unsigned may = quota > upto - n ? quota - (upto - n) : 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            bool take = (above >> i) & 1u;
-            if (((on >> i) & 1u) && may) take = true, --may;
-            if (take) {
-                const unsigned at = peer_count(count, 1);
-                if (at < (unsigned)p.k) peer_store1(list + at * 8, (u64)key_of(f[i]) << 32 | (0xffffffffu - (unsigned)(share.entry(v) + i)));
-            }
-        }
-        const unsigned took = __shfl_sync(~0u, upto, 31);
-        quota = quota > took ? quota - took : 0;
-    }
-    cluster_sync(size);
-    if (rank != 0) return;
-
-    /* bitonic sort of the next power of two, largest first; unused places hold 0, below every entry */
-    int m = 32;
-    while (m < p.k) m *= 2;
-    for (int i = (int)taken + threadIdx.x; i < m; i += kThreads) sh.list[i] = 0;
-    for (int len = 2; len <= m; len *= 2)
-        for (int d = len / 2; d; d /= 2) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < m / 2; i += kThreads) {
-                const int a = (i / d) * 2 * d + i % d, b = a + d;
-                const u64 u = sh.list[a], w = sh.list[b];
-                if ((u < w) == ((a & len) == 0)) sh.list[a] = w, sh.list[b] = u;
-            }
-        }
+    typename Elem<T>::Max largest;
+#pragma unroll 4
+    for (int v = share.first; v < share.last; v += 32) largest.add(share.get(v));
+    float most = largest.get(), bound = neg_inf();
+    const int want = (p.k + (int)size - 1) / (int)size; /* threads of each block whose maxima make up k entries */
+    if (want <= kThreads) bound = bound_of(most, want);
+    most = warp_max(most);
+    if (lane == 0) scratch[warp] = __float_as_uint(most);
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, __uint_as_float((unsigned)scratch[w]));
+    if (size > 1) cluster_wait();
+    tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
+    for (int i = 0; i < (int)size; ++i) {
+        most = fmaxf(most, __uint_as_float((unsigned)told.block[0][i][0]));
+        bound = fminf(bound, __uint_as_float((unsigned)told.block[0][i][1]));
+    }
+    unsigned n = 0, all = 0;
+    double sum = 0.0;
+    if (most > neg_inf()) {
+        if (p.lse) {
+            const float c = (float)(1.4426950408889634 / p.temperature);
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (most < __uint_as_float(0x7f800000u)) {
+#pragma unroll 2
+                for (int v = share.first; v < share.last; v += 32) {
+                    float f[E];
+                    get(v, f);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) part[i & 3] += fast_exp2((f[i] - most) * c);
+                }
+            }
+            const float warp_part = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
+            __syncthreads();
+            if (lane == 0) scratch[warp] = __float_as_uint(warp_part);
+        }
+        n = gather(share, raw, fmaxf(bound, -3.402823466e+38f), list, (unsigned)p.room, g, rank);
+        if (p.lse)
+            for (int w = 0; w < kWarps; ++w) sum += (double)__uint_as_float((unsigned)scratch[w]);
+        tell_all(told.block[1], n, (u64)__double_as_longlong(sum), rank, size);
+        sum = 0.0;
+        for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[1][i][0], sum += __longlong_as_double((long long)told.block[1][i][1]);
+    }
+    if (p.lse && rank == 0 && threadIdx.x == 0)
+        p.lse[row] = most > neg_inf() && most < __uint_as_float(0x7f800000u) ? (float)((double)most / p.temperature + log_64(sum)) : most;
+
+    if (all > (unsigned)p.room) {
+        /* too many (ties, or rows of few large entries side by side): find the border, then list what is above it and
+         * the first of what is on it */
+        const Weigh<sizeof(T) == 4> none(0.0f, 1.0, nullptr);
+        const Border border = find_border<T, R, false>(share, get, level, size, key_of(bound), key_of(most), (u64)p.k, none, 0.0, 0, 0);
+        unsigned ties = 0;
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) ties += key_of(f[i]) == border.key;
+        }
+        ties = warp_sum(ties);
+        if (threadIdx.x == 0) g.count = 0;
+        if (lane < (int)size) peer_store(peer_addr(shared_addr(&told.warp[rank * kWarps + warp][0]), lane), ties, 0);
+        cluster_sync(size);
+        unsigned quota = 0, seen = 0;
+        const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
+        for (int i0 = 0; i0 < nwarps; i0 += 32) {
+            const int i = i0 + lane;
+            const unsigned m = i < nwarps ? (unsigned)told.warp[i][0] : 0;
+            const unsigned upto = seen + warp_scan(m);
+            if (i == self) quota = min(upto, border.ties) - min(upto - m, border.ties);
+            seen = __shfl_sync(~0u, upto, 31);
+        }
+        quota = __shfl_sync(~0u, quota, self & 31);
+        const unsigned lowest = key_of(neg_inf()), to = peer_addr(shared_addr(list), 0), count = peer_addr(shared_addr(&g.count), 0);
+        for (int v0 = share.first - lane; v0 < share.last; v0 += 32) {
+            const int v = v0 + lane;
+            float f[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = neg_inf();
+            if (v < share.last) get(v, f);
+            unsigned on = 0, above = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const unsigned key = key_of(f[i]);
+                if (key > lowest && v < share.last) on |= (unsigned)(key == border.key) << i, above |= (unsigned)(key > border.key) << i;
+            }
+            if (!__any_sync(~0u, on | above)) continue;
+            const unsigned m = __popc(on), upto = warp_scan(m);
+            unsigned may = quota > upto - m ? quota - (upto - m) : 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                bool take = (above >> i) & 1u;
+                if (((on >> i) & 1u) && may) take = true, --may;
+                if (take) {
+                    const unsigned at = peer_count(count, 1);
+                    if (at < (unsigned)p.k) peer_store1(to + at * 8, entry_of(f[i], share.entry(v) + i));
+                }
+            }
+            const unsigned took = __shfl_sync(~0u, upto, 31);
+            quota = quota > took ? quota - took : 0;
+        }
+        cluster_sync(size);
+        all = rank == 0 ? g.count : 0;
+    }
+    if (rank != 0) return;
+    sort_down(list, (int)all, p.room);
     for (int i = threadIdx.x; i < p.k; i += kThreads) {
-        const u64 e = sh.list[i];
-        static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(e ? value_of((unsigned)(e >> 32)) : neg_inf());
-        p.index[row * p.k + i] = e ? (int)(0xffffffffu - (unsigned)e) : -1;
+        const u64 e = i < (int)all ? list[i] : 0;
+        static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(e ? score_of(e) : neg_inf());
+        p.index[row * p.k + i] = e ? index_of(e) : -1;
     }
 }
 
@@ -456,7 +654,7 @@ __device__ __noinline__ float row_loss(const RowSums &all, double named, double 
 }
 
 /* BACKWARD: the statistics are given, and no block needs the others. */
-template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const DistillParams p) {
+template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const __grid_constant__ DistillParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 dynamic[];
     __shared__ double scratch[kWarps];
@@ -807,9 +1005,12 @@ int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *
     if (!(temperature > 1e-30) || temperature > 1e30) return fail(ctx, ACCB_EINVAL, "top_rows: bad temperature %g", temperature);
     if (x->rows == 0) return ACCB_OK;
     if (!values || !index) return fail(ctx, ACCB_EINVAL, "top_rows: null result");
-    const TopParams p{rows_in(x), values, index, lse, temperature, k};
+    int room = 256;
+    while (room < 2 * k && room < 2 * kMaxK) room *= 2;
+    const TopParams p{rows_in(x), values, index, lse, temperature, k, room};
+    const size_t fixed = std::max(room * sizeof(u64), sizeof(Level));
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
-#define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, 0, (cudaStream_t)stream, "top_rows")
+#define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, fixed, (cudaStream_t)stream, "top_rows")
     return BY_TYPE(x->type, CALL);
 #undef CALL
 }

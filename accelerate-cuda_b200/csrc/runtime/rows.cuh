@@ -30,7 +30,7 @@ namespace accb_rows {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 4 * kThreads;    /* bins of one level of the border search: four per thread */
+constexpr int kBins = 2 * kThreads;    /* bins of one level of the border search: two per thread */
 constexpr int kMaxK = 1024;            /* most entries of a top list */
 constexpr long long kMaxCols = 1 << 20;
 
@@ -215,17 +215,16 @@ __device__ __forceinline__ uint4 peer_load(unsigned addr) {
                  : "memory");
     return v;
 }
+__device__ __forceinline__ u64 peer_load1(unsigned addr) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ unsigned peer_count(unsigned addr, unsigned n) {
     unsigned old;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(n) : "memory");
     return old;
 }
-
-/* What every warp of a row tells every other: four 64-bit words per warp and exchange.  A kernel uses every buffer
- * once, so none is overwritten while it is read. */
-struct Exchange {
-    alignas(16) u64 word[3][kMaxCluster * kWarps][4];
-};
 
 /* ----------------------------------------------------------------- rows */
 /* A block runs most of its code once per row, so what counts of rarely run code is its size: every instruction that
@@ -339,23 +338,107 @@ template <class V> __device__ __forceinline__ V warp_scan(V v) { /* inclusive */
     return v;
 }
 
-/* ------------------------------------------------- weights and borders */
-/* The share of an entry is exp((x - max) / T).  It is held as a whole number in units of 2^-43, so that sums do not
- * depend on their order -- on how a row is split over warps and blocks -- and a million entries (kMaxCols) still fit
- * into 64 bits.  Computed in 64 bits: two indices are told apart by a sum, and an error of 2^-24 in a row of 10^5
- * like entries would pick the wrong one every few thousand rows. */
+/* -------------------------------------------------------------- weights */
+/* The share of an entry is exp((x - top) / T), top the row's maximum.  It is held as a whole number in units of 2^-43,
+ * so that sums do not depend on their order -- on how a row is split over warps and blocks -- and a million entries
+ * (kMaxCols) still fit into 64 bits.  Two indices are told apart by a sum: an error of 2^-24 of each of 10^5 like
+ * entries would pick the wrong one every few thousand rows.  So 2^y is computed in 64 bits:
+ *     64 y = K + r, K whole, |r| <= 1/2;  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r)
+ * with the cubic Taylor polynomial of 2^(r / 64), wrong by less than (ln 2 / 128)^4 / 24 < 2^-34.6 of itself: eight
+ * 64-bit operations where the library's function takes some twenty.  The table is in shared memory sixteen times, a
+ * copy for every lane of a half warp, so that no two lanes meet in a bank. */
 constexpr int kUnitLog2 = 43;
-struct Scale {
-    float top;  /* the row's maximum */
-    double c;   /* log2(e) / T */
-    __device__ __forceinline__ u64 weight(float f) const {
-        if (f == top) return 1ull << kUnitLog2;
-        const double y = ((double)f - (double)top) * c;
-        if (!(y > -(kUnitLog2 + 2.0))) return 0; /* also f = -inf with T = inf, a NaN here */
-        return __double2ull_rn(exp2(y) * (double)(1ull << kUnitLog2));
+constexpr int kTable = 64;
+constexpr int kTableCopies = 16;
+
+static __device__ __noinline__ void fill_table(double *table) { /* kTable * kTableCopies; by all threads, a barrier follows */
+    const double v = exp2((double)(threadIdx.x % kTable) * (1.0 / kTable));
+    for (int i = threadIdx.x / kTable; i < kTableCopies; i += kThreads / kTable) table[(threadIdx.x % kTable) * kTableCopies + i] = v;
+}
+
+/* WIDE: scores of 24 bits, whose distance from the maximum takes 64 bits.  That of two 16-bit scores is exact in 32,
+ * but for scores nearer to 0 than 2^-16 of the maximum, where it is off by 2^-25 of itself. */
+template <bool WIDE> struct Weigh {
+    static constexpr double kRound = 6755399441055744.0; /* 1.5 * 2^52: adding it rounds to a whole number */
+    float top, least;    /* scores below `least` weigh less than half a unit, or are excluded */
+    double c;            /* 64 log2(e) / T */
+    const double *table; /* this lane's copy */
+
+    __device__ __forceinline__ Weigh(float maximum, double temperature, const double *shared_table) {
+        top = maximum;
+        table = shared_table + (threadIdx.x & (kTableCopies - 1));
+        c = 64.0 * 1.4426950408889634 / temperature;
+        least = fmaxf(-3.402823466e+38f, (float)((double)top - (kUnitLog2 + 2) * 0.69314718055994531 * temperature));
     }
+    /* for f >= least */
+    __device__ __forceinline__ u64 of(float f) const {
+        constexpr double l = 0.69314718055994531 / kTable;
+        const double x = WIDE ? (double)f - (double)top : (double)(f - top);
+        const double t = fma(x, c, kRound);
+        const int k = __double2loint(t);
+        const double r = fma(x, c, kRound - t);
+        double m = table[(k & (kTable - 1)) * kTableCopies];
+        m = __hiloint2double(__double2hiint(m) + ((k & ~(kTable - 1)) << 14), __double2loint(m));
+        const double unit = (double)(1ull << kUnitLog2);
+        /* 2^52 makes a unit of 2^-43 the last bit */
+        m = fma(m, fma(fma(fma(unit * l * l * l / 6.0, r, unit * l * l / 2.0), r, unit * l), r, unit), 4503599627370496.0);
+        return (u64)__double_as_longlong(m) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 weight(float f) const { return f >= least ? of(f) : 0; }
 };
 
+/* ------------------------------------------------------ candidate lists */
+/* An entry as one number: larger for larger scores and, among equal ones, for lower indices.  0 is no entry. */
+__device__ __forceinline__ u64 entry_of(float f, int index) { return (u64)key_of(f) << 32 | (0xffffffffu - (unsigned)index); }
+__device__ __forceinline__ float score_of(u64 e) { return value_of((unsigned)(e >> 32)); }
+__device__ __forceinline__ int index_of(u64 e) { return (int)(0xffffffffu - (unsigned)e); }
+
+/* Sorts a list in shared memory, largest first; `room`, a power of two, numbers fit.  Up to 256 different numbers are
+ * ranked by counting, one thread each, which takes two barriers; more by bitonic merging. */
+static __device__ __noinline__ void sort_down(u64 *list, int n, int room) {
+    if (n <= kThreads) {
+        const int t = threadIdx.x;
+        const u64 e = t < n ? list[t] : 0;
+        int above = 0;
+        if ((t & ~31) < n) {
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) above += list[j] > e;
+        }
+        __syncthreads();
+        if (t < n) list[above] = e;
+        __syncthreads();
+        return;
+    }
+    int m = 2 * kThreads;
+    while (m < n) m *= 2;
+    m = min(m, room);
+    for (int i = n + threadIdx.x; i < m; i += kThreads) list[i] = 0;
+    for (int len = 2; len <= m; len *= 2)
+        for (int d = len / 2; d; d /= 2) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < m / 2; i += kThreads) {
+                const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a + d;
+                const u64 u = list[a], w = list[b];
+                if ((u < w) == ((a & len) == 0)) list[a] = w, list[b] = u;
+            }
+        }
+    __syncthreads();
+}
+
+/* A score that at least `want` of the block's threads reach with the largest of theirs: the largest such value in 16
+ * leading bits of its key, bit by bit. */
+static __device__ __noinline__ float bound_of(float most, int want) {
+    const unsigned key = key_of(most) >> 16;
+    unsigned found = 0;
+#pragma unroll 1
+    for (int b = 15; b >= 0; --b) {
+        const unsigned trial = found | 1u << b;
+        if (__syncthreads_count(key >= trial) >= want) found = trial;
+    }
+    return found > 0x80u ? value_of(found << 16) : neg_inf();
+}
+
+/* ---------------------------------------------------------------- borders */
 /* The best entries of a row, in the order of falling value and, among equals, rising index: every entry whose key is
  * above `key`, and the first `ties` of those whose key it is. */
 struct Border {
@@ -367,7 +450,7 @@ struct Border {
 struct Level { /* one level of the border search */
     alignas(16) u64 mass[kBins];
     alignas(16) unsigned count[kBins];
-    u64 warp_total[kWarps], warp_mass[kWarps];
+    u64 warp_total[kWarps];
     u64 before;
     unsigned bin, bin_count;
     int found;
@@ -377,14 +460,15 @@ struct Level { /* one level of the border search */
  * row), that holds `target` entries (BY_MASS false) or the given fraction of a total weight (BY_MASS true; total 0:
  * what the range holds, less the weight of `spare` entries of key klo).
  *
- * Every level lays 1024 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
+ * Every level lays 512 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
  * the border lies and goes on with that bin's range; when a bin is one key, the rest is arithmetic.  For 16-bit
- * scores one level usually does, for 32-bit ones three.  Bins are summed over the cluster by reading the other
- * blocks' bins, four per thread; every block does that for itself and so learns the result without another message.
- * All threads of the cluster call it with the same arguments. */
+ * scores one or two levels do, for 32-bit ones up to four.  Bins are summed over the cluster by reading the other
+ * blocks' bins, two per thread; every block does that for itself and so learns the result without another message.
+ * The way for rows whose candidates are too many for a list.  All threads of the cluster call it with the same
+ * arguments. */
 template <class T, bool RESIDENT, bool BY_MASS, class Get>
 __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &lv, unsigned size, unsigned klo, unsigned khi,
-                              u64 target, const Scale &scale, double fraction, u64 total, unsigned spare) {
+                              u64 target, const Weigh<sizeof(T) == 4> &weigh, double fraction, u64 total, unsigned spare) {
     constexpr int E = Elem<T>::E, S0 = Elem<T>::kShift;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const unsigned bottom = klo;
@@ -392,36 +476,34 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
     if (BY_MASS && have_target) target = max(1ull, (u64)ceil(fraction * (double)total));
     for (;;) {
         const unsigned span = khi - klo;
-        const int shift = max(S0, 22 - __clz(span)); /* span >> shift < 1024 */
-        const bool weigh = BY_MASS && shift > S0;
+        const int shift = max(S0, 23 - __clz(span)); /* span >> shift < 512 */
+        const bool by_entry = BY_MASS && shift > S0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lv.count[t + i * kThreads] = 0, lv.mass[t + i * kThreads] = 0;
+        for (int i = 0; i < 2; ++i) lv.count[t + i * kThreads] = 0, lv.mass[t + i * kThreads] = 0;
         if (t == 0) lv.found = 0;
         __syncthreads();
         for (int v = share.first; v < share.last; v += 32) {
             float f[E];
             get(v, f);
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < E; ++i) {
                 const unsigned k = key_of(f[i]);
                 if (k - klo <= span) {
                     const unsigned b = (khi - k) >> shift;
                     atomicAdd(&lv.count[b], 1u);
-                    if (weigh) atomicAdd(&lv.mass[b], scale.weight(f[i]));
+                    if (by_entry) atomicAdd(&lv.mass[b], weigh.weight(f[i]));
                 }
             }
         }
         cluster_sync(size);
-        unsigned count[4] = {0, 0, 0, 0};
-        u64 mass[4] = {0, 0, 0, 0};
+        unsigned count[2] = {0, 0};
+        u64 mass[2] = {0, 0};
         for (unsigned r = 0; r < size; ++r) {
-            const uint4 c = peer_load(peer_addr(shared_addr(&lv.count[4 * t]), r));
-            count[0] += c.x, count[1] += c.y, count[2] += c.z, count[3] += c.w;
-            if (weigh) {
-                const uint4 a = peer_load(peer_addr(shared_addr(&lv.mass[4 * t]), r));
-                const uint4 b = peer_load(peer_addr(shared_addr(&lv.mass[4 * t + 2]), r));
+            const u64 c = peer_load1(peer_addr(shared_addr(&lv.count[2 * t]), r));
+            count[0] += (unsigned)c, count[1] += (unsigned)(c >> 32);
+            if (by_entry) {
+                const uint4 a = peer_load(peer_addr(shared_addr(&lv.mass[2 * t]), r));
                 mass[0] += (u64)a.y << 32 | a.x, mass[1] += (u64)a.w << 32 | a.z;
-                mass[2] += (u64)b.y << 32 | b.x, mass[3] += (u64)b.w << 32 | b.z;
             }
         }
         /* the one key of a bin once a bin is one key: keys of 16-bit types end in zeros above zero and in ones below */
@@ -431,8 +513,8 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
         };
         u64 sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (BY_MASS && !weigh && count[i]) mass[i] = count[i] * scale.weight(value_of(key_at(4 * t + i)));
+        for (int i = 0; i < 2; ++i) {
+            if (BY_MASS && !by_entry && count[i]) mass[i] = count[i] * weigh.weight(value_of(key_at(2 * t + i)));
             if (!BY_MASS) mass[i] = count[i];
             sum += mass[i];
         }
@@ -446,16 +528,16 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
             all += lv.warp_total[w];
         }
         if (!have_target) { /* the weight of the range is the total that the fraction is of */
-            all -= spare * scale.weight(value_of(bottom));
+            all -= spare * weigh.weight(value_of(bottom));
             target = max(1ull, (u64)ceil(fraction * (double)all));
             have_target = true;
         }
         u64 before = upto - sum;
         if (before < target && target <= upto) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 if (before < target && target <= before + mass[i]) {
-                    lv.bin = 4 * t + i;
+                    lv.bin = 2 * t + i;
                     lv.bin_count = count[i];
                     lv.before = before;
                     lv.found = 1;
@@ -467,20 +549,19 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
         if (!lv.found) return Border{klo, 0xffffffffu, 0xffffffffu}; /* less than was asked for: all of the range */
         const unsigned bin = lv.bin, bin_count = lv.bin_count;
         target -= lv.before;
+        __syncthreads(); /* lv is used again */
         if (shift == S0) {
             const unsigned key = key_at(bin);
             u64 ties = target;
             if (BY_MASS) {
-                const u64 w = scale.weight(value_of(key));
+                const u64 w = weigh.weight(value_of(key));
                 ties = (target + w - 1) / w; /* w > 0: the bin held some of the weight that was looked for */
             }
-            __syncthreads(); /* lv is used again */
             return Border{key, (unsigned)min(ties, (u64)bin_count), bin_count};
         }
         khi -= bin << shift;
         const unsigned width = (1u << shift) - 1u;
         if (khi - klo > width) klo = khi - width;
-        __syncthreads();
     }
 }
 
