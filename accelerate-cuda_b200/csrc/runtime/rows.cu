@@ -128,7 +128,8 @@ struct SampleParams {
     int *token;
     float *logprob;
 };
-constexpr int kSampleRoom = 1024; /* candidates of a row that a block sorts */
+constexpr int kSampleRoom = 512; /* candidates of a row that a block lists and sorts, ... */
+constexpr int kListed = 256;     /* ... asked for where top_k is no more */
 
 /* the whole part of uniform * total below total */
 __device__ __forceinline__ u64 drawn(float uniform, u64 total) {
@@ -192,8 +193,9 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     extern __shared__ uint4 stage[];
     __shared__ Told told;
     __shared__ union {
-        Level level;
         u64 list[kSampleRoom];
+        FineBins bins;
+        Level level;
     } sh;
     __shared__ double table[kTable * kTableCopies];
     __shared__ u64 scratch[kWarps];
@@ -250,7 +252,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     }
     float most = largest.get(), bound = neg_inf();
     const int want = (k + (int)size - 1) / (int)size; /* of each block's threads */
-    if (k > 1 && k <= kSampleRoom && want <= kThreads) bound = bound_of(most, want);
+    if (k > 1 && want <= kThreads) bound = bound_of(most, want);
     most = warp_max(most);
     if (lane == 0) scratch[warp] = __float_as_uint(most);
     __syncthreads();
@@ -299,7 +301,8 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     const int per_quarter = (max(0, share.last - start) + 127) >> 7;
     u64 total = 0;
     const bool cut = k > 0 || top_p < 1.0f;
-    if (k == 0) {
+    constexpr bool kBinsWeigh = Elem<T>::kShift == 16; /* counts by bin say the row's weight: a bin is one score */
+    if (k == 0 && !(cut && kBinsWeigh)) {
         const float from = cut ? weigh.least : fmaxf(weigh.least, lowest);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -316,37 +319,35 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     }
     Border border{key_of(cut ? neg_inf() : fmaxf(lowest, -3.402823466e+38f)) - (cut ? 0u : 1u), 0, 0};
     if (cut) {
-        if (k == 0) { /* top_p alone: entries so far down that all of them together weigh less than what is cut off */
-            const u64 block_total = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
-            tell_all(told.block[1], block_total, 0, rank, size);
-            for (int i = 0; i < (int)size; ++i) total += told.block[1][i][0];
-            const double left = (1.0 - (double)top_p) * ((double)total * (1.0 / (double)(1ull << kUnitLog2)));
-            const double low = (double)most + (log_64(left / (double)p.in.cols) - 0.01) * temperature;
-            bound = left > 1e-5 && low > -3.0e38 ? __double2float_rd(low) : neg_inf();
+        float least = fmaxf(bound, -3.402823466e+38f);
+        bool list = k > 0 && k <= kListed;
+        if (k == 0) { /* top_p alone */
+            least = weigh.least;
+            if (!kBinsWeigh) { /* entries so far down that all of them together weigh less than what is cut off */
+                const u64 block_total = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
+                tell_all(told.block[1], block_total, 0, rank, size);
+                for (int i = 0; i < (int)size; ++i) total += told.block[1][i][0];
+                const double left = (1.0 - (double)top_p) * ((double)total * (1.0 / (double)(1ull << kUnitLog2)));
+                const double low = (double)most + (log_64(left / (double)p.in.cols) - 0.01) * temperature;
+                if (left > 1e-5 && low > (double)least) least = __double2float_rd(low);
+                list = true;
+            }
         }
-        const float least = fmaxf(bound, -3.402823466e+38f);
-        const unsigned n = gather(share, raw, least, sh.list, kSampleRoom, g, rank);
-        tell_all(told.block[2], n, 0, rank, size);
-        unsigned all = 0;
-        for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[2][i][0];
-        if (all <= kSampleRoom) { /* the same in every block of the row */
-            if (rank == 0)
-                draw_from_list(p, row, sh.list, scratch, (int)all, k, top_p, lowest, k > 0 ? 0 : total, uniform, temperature,
-                               most, weigh);
-            return;
+        if (list) {
+            const unsigned n = gather(share, raw, least, sh.list, kSampleRoom, g, rank);
+            tell_all(told.block[2], n, 0, rank, size);
+            unsigned all = 0;
+            for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[2][i][0];
+            if (all <= kSampleRoom) { /* the same in every block of the row */
+                if (rank == 0)
+                    draw_from_list(p, row, sh.list, scratch, (int)all, k, top_p, lowest, total, uniform, temperature, most, weigh);
+                return;
+            }
         }
-        /* too many: the border of what is kept, from counts and weights of ranges of scores */
-        unsigned spare = 0;
-        if (k > 0) {
-            border = k == 1 ? Border{key_of(most), 1, 1}
-                            : find_border<T, R, false>(share, get, sh.level, size, key_of(bound), key_of(most), (u64)k, weigh, 0.0, 0, 0);
-            spare = k == 1 ? 0 : border.equals - border.ties;
-        }
-        if (top_p < 1.0f && k != 1) {
-            const unsigned from = k > 0 ? border.key : key_of(bound);
-            const Border b = find_border<T, R, true>(share, get, sh.level, size, from, key_of(most), 0, weigh, top_p > 0.0f ? (double)top_p : 0.0, total, spare);
-            if (b.ties != 0xffffffffu) border = b;
-        }
+        /* too many for a list */
+        border = k == 1 ? Border{key_of(most), 1, 1}
+                        : border_by_bins<T, R>(share, get, sh.bins, sh.level, size, weigh, least, most, (u64)k,
+                                               top_p < 1.0f ? (top_p > 0.0f ? (double)top_p : 0.0) : 1.0, total);
         const unsigned below = key_of(lowest) - 1u;
         if (below >= border.key) border = Border{below, 0, 0};
     }
@@ -542,7 +543,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
         /* too many (ties, or rows of few large entries side by side): find the border, then list what is above it and
          * the first of what is on it */
         const Weigh<sizeof(T) == 4> none(0.0f, 1.0, nullptr);
-        const Border border = find_border<T, R, false>(share, get, level, size, key_of(bound), key_of(most), (u64)p.k, none, 0.0, 0, 0);
+        const Border border = find_border<T, R, false>(share, get, level, size, key_of(bound), key_of(most), (u64)p.k, none, 0.0, 0);
         unsigned ties = 0;
         for (int v = share.first; v < share.last; v += 32) {
             float f[E];

@@ -457,8 +457,8 @@ struct Level { /* one level of the border search */
 };
 
 /* Finds the border of the shortest run of best entries, among those with klo <= key <= khi (khi >= every key of the
- * row), that holds `target` entries (BY_MASS false) or the given fraction of a total weight (BY_MASS true; total 0:
- * what the range holds, less the weight of `spare` entries of key klo).
+ * row, or what is above them is left out), that holds `target` entries (BY_MASS false) or, BY_MASS, the weight
+ * `target`, or where that is 0 the given fraction of what the range holds less the weight of `spare` entries of key klo.
  *
  * Every level lays 512 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
  * the border lies and goes on with that bin's range; when a bin is one key, the rest is arithmetic.  For 16-bit
@@ -468,12 +468,11 @@ struct Level { /* one level of the border search */
  * arguments. */
 template <class T, bool RESIDENT, bool BY_MASS, class Get>
 __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &lv, unsigned size, unsigned klo, unsigned khi,
-                              u64 target, const Weigh<sizeof(T) == 4> &weigh, double fraction, u64 total, unsigned spare) {
+                              u64 target, const Weigh<sizeof(T) == 4> &weigh, double fraction, unsigned spare) {
     constexpr int E = Elem<T>::E, S0 = Elem<T>::kShift;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const unsigned bottom = klo;
-    bool have_target = !BY_MASS || total != 0;
-    if (BY_MASS && have_target) target = max(1ull, (u64)ceil(fraction * (double)total));
+    bool have_target = target != 0;
     for (;;) {
         const unsigned span = khi - klo;
         const int shift = max(S0, 23 - __clz(span)); /* span >> shift < 512 */
@@ -485,7 +484,7 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
         for (int v = share.first; v < share.last; v += 32) {
             float f[E];
             get(v, f);
-#pragma unroll 1
+#pragma unroll
             for (int i = 0; i < E; ++i) {
                 const unsigned k = key_of(f[i]);
                 if (k - klo <= span) {
@@ -563,6 +562,191 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
         const unsigned width = (1u << shift) - 1u;
         if (khi - klo > width) klo = khi - width;
     }
+}
+
+/* ------------------------------------------------------------------- bins */
+/* For rows with too many candidates for a list: one pass counts entries by the 16 leading bits of their keys -- sign,
+ * exponent and seven bits of mantissa, which is all there is of a bfloat16.  Keys near zero, 2^-10 of the largest
+ * magnitude and below, would be most of the keys and hold next to no entries: they share the middle bin.  Keys below
+ * minus the largest magnitude share the last.  The weights of these two are added up entry by entry. */
+constexpr int kFineBins = 12 * kThreads; /* 11 octaves of 128 keys on either side of zero, the two shared bins: 2818 */
+struct FineBins {
+    alignas(16) unsigned count[kFineBins];
+    u64 warp[kWarps];
+    u64 shared[4]; /* weight and count of the middle bin, of the last one */
+    u64 before;
+    unsigned equals;
+    int found;
+};
+
+/* The order of bins: 0 for the largest scores. */
+struct BinOrder {
+    unsigned high, low, far, gap, top; /* leading bits of the smallest key above the middle bin, the largest below, the
+                                          largest of the last bin; keys left out; squeezed key of the maximum */
+    __device__ __forceinline__ BinOrder(float most, float from) {
+        const float reach = fmaxf(fabsf(most), fminf(fabsf(from), fmaxf(2.0f * fabsf(most), 64.0f)));
+        const int e = (int)(__float_as_uint(reach) >> 23); /* biased exponent of the largest magnitude */
+        const float z = __uint_as_float((unsigned)max(1, e - 10) << 23), m = __uint_as_float((unsigned)min(254, e + 1) << 23);
+        high = key_of(z) >> 16, low = key_of(-z) >> 16, far = key_of(-m) >> 16, gap = high - low - 2;
+        top = squeeze(key_of(most) >> 16);
+    }
+    __device__ __forceinline__ unsigned squeeze(unsigned k) const { return k >= high ? k - gap : k > low ? low + 1 : max(k, far); }
+    __device__ __forceinline__ unsigned bin(unsigned k) const { return top - squeeze(k); }
+    __device__ __forceinline__ int shared(unsigned k) const { return k < high && k > low ? 0 : k <= far ? 1 : -1; }
+    /* the bin's keys, leading bits */
+    __device__ __forceinline__ unsigned lowest(unsigned bin) const {
+        const unsigned c = top - bin;
+        return c > low + 1 ? c + gap : c == far ? 0 : c;
+    }
+    __device__ __forceinline__ unsigned highest(unsigned bin) const {
+        const unsigned c = top - bin;
+        return c > low + 1 ? c + gap : c == low + 1 ? high - 1 : c;
+    }
+};
+
+/* The border of the entries not below `from` that top_k (0: off) and then the fraction top_p (1: off) of their weight
+ * keep.  `total`: the weight of the row if it is known and k is 0, else 0.  All threads of the cluster call it with the
+ * same arguments; `lv` may lie in the place of `bins`. */
+template <class T, bool RESIDENT, class Get>
+__device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineBins &bins, Level &lv, unsigned size, const Weigh<sizeof(T) == 4> &weigh,
+                                 float from, float most, u64 k, double top_p, u64 total) {
+    constexpr int E = Elem<T>::E, PER = kFineBins / kThreads;
+    constexpr bool EXACT = Elem<T>::kShift == 16; /* a bin that is not shared is one key */
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const BinOrder order(most, from);
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
+    if (t < 4) bins.shared[t] = 0;
+    __syncthreads();
+    u64 weight[2] = {0, 0};
+    unsigned number[2] = {0, 0};
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        get(v, f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (!(f[i] >= from)) continue;
+            const unsigned key = key_of(f[i]) >> 16;
+            const int which = order.shared(key);
+            if (which < 0)
+                atomicAdd(&bins.count[order.bin(key)], 1u);
+            else if (which == 0)
+                weight[0] += weigh.weight(f[i]), ++number[0];
+            else
+                weight[1] += weigh.weight(f[i]), ++number[1];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (__any_sync(~0u, number[i] != 0)) {
+            const u64 w = warp_sum(weight[i]), n = warp_sum((u64)number[i]);
+            if (lane == 0) atomicAdd(&bins.shared[2 * i], w), atomicAdd(&bins.shared[2 * i + 1], n);
+        }
+    cluster_sync(size);
+    unsigned count[PER];
+    u64 shared[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) count[i] = 0;
+    for (unsigned r = 0; r < size; ++r) {
+#pragma unroll
+        for (int i = 0; i < PER / 4; ++i) {
+            const uint4 c = peer_load(peer_addr(shared_addr(&bins.count[PER * t + 4 * i]), r));
+            count[4 * i] += c.x, count[4 * i + 1] += c.y, count[4 * i + 2] += c.z, count[4 * i + 3] += c.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) shared[i] += peer_load1(peer_addr(shared_addr(&bins.shared[i]), r));
+    }
+    cluster_sync(size); /* no block reads another's bins any more: the sums take their place */
+#pragma unroll
+    for (int i = 0; i < PER; ++i) bins.count[PER * t + i] = count[i];
+    const int middle = (int)(order.top - (order.low + 1)), last = (int)(order.top - order.far);
+
+    auto counted = [&](int bin) -> u64 { return bin == middle ? shared[1] : bin == last ? shared[3] : bins.count[bin]; };
+    auto weighed = [&](int bin, bool high) -> u64 {
+        if (bin == middle) return shared[0];
+        if (bin == last) return shared[2];
+        const unsigned n = bins.count[bin];
+        /* the key of a bfloat16 ends in zeros above zero and in ones below */
+        const unsigned key = high || (EXACT && order.highest(bin) < 0x8000u) ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16;
+        return n ? n * weigh.weight(value_of(key)) : 0;
+    };
+    /* the first bin up to which the sum of `of` reaches what `goal` makes of the whole sum, or -1; what precedes it */
+    u64 before = 0;
+    unsigned equals = 0;
+    auto find = [&](auto of, auto goal) {
+        u64 mine = 0;
+#pragma unroll 1
+        for (int i = 0; i < PER; ++i) mine += of(PER * t + i);
+        u64 upto = warp_scan(mine), all = 0;
+        if (lane == 31) bins.warp[warp] = upto;
+        if (t == 0) bins.found = -1;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) upto += bins.warp[w];
+            all += bins.warp[w];
+        }
+        const u64 target = goal(all);
+        u64 sum = upto - mine;
+        if (sum < target && target <= upto) {
+#pragma unroll 1
+            for (int i = 0; i < PER; ++i) {
+                const u64 w = of(PER * t + i);
+                if (sum < target && target <= sum + w) bins.found = PER * t + i, bins.before = sum, bins.equals = (unsigned)counted(PER * t + i);
+                sum += w;
+            }
+        }
+        __syncthreads();
+        const int found = bins.found;
+        before = bins.before, equals = bins.equals;
+        __syncthreads();
+        return found;
+    };
+    if (k > 0) {
+        const int bin = find(counted, [&](u64) { return k; });
+        if (bin < 0) { /* fewer than k */
+            k = 0;
+            if (!(top_p < 1.0)) return Border{key_of(neg_inf()), 0, 0};
+            return find_border<T, RESIDENT, true>(share, get, lv, size, key_of(from), key_of(most), 0, weigh, top_p, 0);
+        }
+        Border border{EXACT && order.highest(bin) < 0x8000u ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16, (unsigned)(k - before), equals};
+        if (!EXACT || bin == middle || bin == last)
+            border = find_border<T, RESIDENT, false>(share, get, lv, size, order.lowest(bin) << 16, order.highest(bin) << 16 | 0xffffu, k - before, weigh, 0.0, 0);
+        if (!(top_p < 1.0)) return border;
+        const Border b = find_border<T, RESIDENT, true>(share, get, lv, size, border.key, key_of(most), 0, weigh, top_p, border.equals - border.ties);
+        return b.ties != 0xffffffffu ? b : border;
+    }
+    /* by weight: of a bin that is not one key only bounds are known, that of its lowest and of its highest score */
+    u64 target = 0;
+    auto goal = [&](u64 all) { return target = max(1ull, (u64)ceil(top_p * (double)(EXACT ? all : total))); };
+    int to = find([&](int bin) { return weighed(bin, false); }, goal), first = to;
+    if (EXACT && to >= 0 && to != middle && to != last) {
+        const unsigned key = order.highest(to) < 0x8000u ? order.highest(to) << 16 | 0xffffu : order.lowest(to) << 16;
+        const u64 w = weigh.weight(value_of(key));
+        return Border{key, (unsigned)min((target - before + w - 1) / w, (u64)equals), equals};
+    }
+    if (!EXACT) first = find([&](int bin) { return weighed(bin, true); }, goal);
+    const unsigned klo = to < 0 ? key_of(from) : max(key_of(from), order.lowest(to) << 16);
+    const unsigned khi = first < 0 ? key_of(most) : order.highest(first) << 16 | 0xffffu;
+    if (!EXACT) { /* what lies above the first bin that may hold the border */
+        u64 more = 0;
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (key_of(f[i]) > khi) more += weigh.weight(f[i]);
+        }
+        more = warp_sum(more);
+        if (lane == 0) bins.warp[warp] = more;
+        cluster_sync(size);
+        before = 0;
+        for (unsigned r = 0; r < size; ++r)
+            for (int w = 0; w < kWarps; ++w) before += peer_load1(peer_addr(shared_addr(&bins.warp[w]), r));
+        cluster_sync(size);
+    }
+    const Border b = find_border<T, RESIDENT, true>(share, get, lv, size, klo, khi, target - before, weigh, 0.0, 0);
+    return b.ties != 0xffffffffu ? b : Border{klo - 1, 0, 0};
 }
 
 }  // namespace accb_rows
