@@ -309,11 +309,17 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
             const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
 #pragma unroll 1
             for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
+                const uint4 w = raw(v);
+                typename Elem<T>::Max best;
+                best.add(w);
+                if (!(best.get() >= from)) continue;
                 float f[E];
-                Elem<T>::unpack(raw(v), f);
+                Elem<T>::unpack(w, f);
 #pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (f[i] >= from) quarter[q] += weigh.of(f[i]);
+                for (int i = 0; i < E; ++i) { /* no branch: the weights of a vector are computed side by side */
+                    const u64 x = weigh.of(f[i]);
+                    quarter[q] += f[i] >= from ? x : 0;
+                }
             }
         }
     }
@@ -355,19 +361,25 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     /* weight above the border and number of entries on it, by warp; every warp then knows what precedes it */
     unsigned ties = 0;
     if (cut) {
-        const float from = weigh.least;
+        const unsigned from = max(border.key, key_of(weigh.least) - 1u); /* keys above it have weight */
+        const float lowest_kept = border.ties ? value_of(border.key) : value_of(from + 1u);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             quarter[q] = 0;
             const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
 #pragma unroll 1
             for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
+                const uint4 w = raw(v);
+                typename Elem<T>::Max best;
+                best.add(w);
+                if (!(best.get() >= lowest_kept)) continue;
                 float f[E];
-                get(v, f);
+                Elem<T>::unpack(w, f);
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const unsigned key = key_of(f[i]);
-                    if (key > border.key && f[i] >= from) quarter[q] += weigh.of(f[i]);
+                    const unsigned key = key_of(not_nan(f[i]));
+                    const u64 x = weigh.of(f[i]);
+                    quarter[q] += key > from ? x : 0;
                     ties += key == border.key;
                 }
             }

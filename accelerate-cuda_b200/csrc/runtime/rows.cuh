@@ -220,6 +220,11 @@ __device__ __forceinline__ u64 peer_load1(unsigned addr) {
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ unsigned peer_load32(unsigned addr) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ unsigned peer_count(unsigned addr, unsigned n) {
     unsigned old;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(n) : "memory");
@@ -370,7 +375,7 @@ template <bool WIDE> struct Weigh {
         c = 64.0 * 1.4426950408889634 / temperature;
         least = fmaxf(-3.402823466e+38f, (float)((double)top - (kUnitLog2 + 2) * 0.69314718055994531 * temperature));
     }
-    /* for f >= least */
+    /* for f >= least; anything below */
     __device__ __forceinline__ u64 of(float f) const {
         constexpr double l = 0.69314718055994531 / kTable;
         const double x = WIDE ? (double)f - (double)top : (double)(f - top);
@@ -573,10 +578,9 @@ constexpr int kFineBins = 12 * kThreads; /* 11 octaves of 128 keys on either sid
 struct FineBins {
     alignas(16) unsigned count[kFineBins];
     u64 warp[kWarps];
-    u64 shared[4]; /* weight and count of the middle bin, of the last one */
-    u64 before;
-    unsigned equals;
-    int found;
+    u64 shared[kMaxCluster][2];   /* weights of the middle bin and the last, by block */
+    u64 total[2][kMaxCluster];    /* of the blocks' slices; by search */
+    u64 found[2][2];              /* what precedes the bin that was looked for; its count << 32 | bin, or ~0 */
 };
 
 /* The order of bins: 0 for the largest scores. */
@@ -592,7 +596,6 @@ struct BinOrder {
     }
     __device__ __forceinline__ unsigned squeeze(unsigned k) const { return k >= high ? k - gap : k > low ? low + 1 : max(k, far); }
     __device__ __forceinline__ unsigned bin(unsigned k) const { return top - squeeze(k); }
-    __device__ __forceinline__ int shared(unsigned k) const { return k < high && k > low ? 0 : k <= far ? 1 : -1; }
     /* the bin's keys, leading bits */
     __device__ __forceinline__ unsigned lowest(unsigned bin) const {
         const unsigned c = top - bin;
@@ -610,100 +613,120 @@ struct BinOrder {
 template <class T, bool RESIDENT, class Get>
 __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineBins &bins, Level &lv, unsigned size, const Weigh<sizeof(T) == 4> &weigh,
                                  float from, float most, u64 k, double top_p, u64 total) {
-    constexpr int E = Elem<T>::E, PER = kFineBins / kThreads;
+    constexpr int E = Elem<T>::E;
     constexpr bool EXACT = Elem<T>::kShift == 16; /* a bin that is not shared is one key */
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const unsigned rank = cluster_rank();
     const BinOrder order(most, from);
+    const int middle = (int)(order.top - (order.low + 1)), last = (int)(order.top - order.far);
 #pragma unroll
-    for (int i = 0; i < PER / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
-    if (t < 4) bins.shared[t] = 0;
+    for (int i = 0; i < kFineBins / kThreads / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
+    if (t < 2) bins.found[t][1] = ~0ull;
     __syncthreads();
-    u64 weight[2] = {0, 0};
-    unsigned number[2] = {0, 0};
     for (int v = share.first; v < share.last; v += 32) {
         float f[E];
         get(v, f);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (!(f[i] >= from)) continue;
-            const unsigned key = key_of(f[i]) >> 16;
-            const int which = order.shared(key);
-            if (which < 0)
-                atomicAdd(&bins.count[order.bin(key)], 1u);
-            else if (which == 0)
-                weight[0] += weigh.weight(f[i]), ++number[0];
-            else
-                weight[1] += weigh.weight(f[i]), ++number[1];
+        for (int i = 0; i < E; ++i)
+            if (f[i] >= from) atomicAdd(&bins.count[order.bin(key_of(f[i]) >> 16)], 1u);
+    }
+    __syncthreads();
+    u64 coarse[2] = {0, 0};
+    if ((middle >= 0 && bins.count[middle]) || bins.count[last]) {
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            get(v, f);
+#pragma unroll 1
+            for (int i = 0; i < E; ++i) {
+                float x = f[0];
+#pragma unroll
+                for (int j = 1; j < E; ++j)
+                    if (i == j) x = f[j];
+                const int bin = x >= from ? (int)order.bin(key_of(x) >> 16) : -1;
+                if (bin == last || (bin == middle && bin >= 0)) coarse[bin == last] += weigh.weight(x);
+            }
         }
     }
+    auto block_total = [&](u64 v) { /* two barriers */
+        v = warp_sum(v);
+        if (lane == 0) bins.warp[warp] = v;
+        __syncthreads();
+        u64 all = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (__any_sync(~0u, number[i] != 0)) {
-            const u64 w = warp_sum(weight[i]), n = warp_sum((u64)number[i]);
-            if (lane == 0) atomicAdd(&bins.shared[2 * i], w), atomicAdd(&bins.shared[2 * i + 1], n);
-        }
+        for (int w = 0; w < kWarps; ++w) all += bins.warp[w];
+        __syncthreads();
+        return all;
+    };
+    coarse[0] = block_total(coarse[0]), coarse[1] = block_total(coarse[1]);
+    if (t < (int)size) peer_store(peer_addr(shared_addr(&bins.shared[rank][0]), t), coarse[0], coarse[1]);
     cluster_sync(size);
-    unsigned count[PER];
-    u64 shared[4] = {0, 0, 0, 0};
+    /* every block adds up a slice of the bins, and puts the sums in place of its own counts, which nobody else reads */
+    const int slice = kFineBins / (int)size, per = (slice + kThreads - 1) / kThreads;
+    const int bin0 = (int)rank * slice + min(slice, t * per), bin1 = (int)rank * slice + min(slice, t * per + per);
+#pragma unroll 4
+    for (int bin = bin0; bin < bin1; ++bin) {
+        const unsigned at = shared_addr(&bins.count[bin]);
+        unsigned n = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) count[i] = 0;
-    for (unsigned r = 0; r < size; ++r) {
-#pragma unroll
-        for (int i = 0; i < PER / 4; ++i) {
-            const uint4 c = peer_load(peer_addr(shared_addr(&bins.count[PER * t + 4 * i]), r));
-            count[4 * i] += c.x, count[4 * i + 1] += c.y, count[4 * i + 2] += c.z, count[4 * i + 3] += c.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) shared[i] += peer_load1(peer_addr(shared_addr(&bins.shared[i]), r));
+        for (unsigned r = 0; r < kMaxCluster; ++r)
+            if (r < size) n += peer_load32(peer_addr(at, r));
+        bins.count[bin] = n;
     }
-    cluster_sync(size); /* no block reads another's bins any more: the sums take their place */
-#pragma unroll
-    for (int i = 0; i < PER; ++i) bins.count[PER * t + i] = count[i];
-    const int middle = (int)(order.top - (order.low + 1)), last = (int)(order.top - order.far);
+    coarse[0] = coarse[1] = 0;
+    for (unsigned r = 0; r < size; ++r) coarse[0] += bins.shared[r][0], coarse[1] += bins.shared[r][1];
 
-    auto counted = [&](int bin) -> u64 { return bin == middle ? shared[1] : bin == last ? shared[3] : bins.count[bin]; };
+    auto counted = [&](int bin) -> u64 { return bins.count[bin]; };
     auto weighed = [&](int bin, bool high) -> u64 {
-        if (bin == middle) return shared[0];
-        if (bin == last) return shared[2];
+        if (bin == middle) return coarse[0];
+        if (bin == last) return coarse[1];
         const unsigned n = bins.count[bin];
         /* the key of a bfloat16 ends in zeros above zero and in ones below */
         const unsigned key = high || (EXACT && order.highest(bin) < 0x8000u) ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16;
         return n ? n * weigh.weight(value_of(key)) : 0;
     };
-    /* the first bin up to which the sum of `of` reaches what `goal` makes of the whole sum, or -1; what precedes it */
+    /* the first bin up to which the sum of `of` reaches what `goal` makes of the whole sum, or -1; what precedes it.
+     * Search 0 and 1 of a call. */
     u64 before = 0;
     unsigned equals = 0;
-    auto find = [&](auto of, auto goal) {
+    auto find = [&](int search, auto of, auto goal) {
         u64 mine = 0;
 #pragma unroll 1
-        for (int i = 0; i < PER; ++i) mine += of(PER * t + i);
-        u64 upto = warp_scan(mine), all = 0;
+        for (int bin = bin0; bin < bin1; ++bin) mine += of(bin);
+        u64 upto = warp_scan(mine), block = 0, all = 0;
         if (lane == 31) bins.warp[warp] = upto;
-        if (t == 0) bins.found = -1;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) upto += bins.warp[w];
-            all += bins.warp[w];
+            block += bins.warp[w];
+        }
+        if (t < (int)size) peer_store1(peer_addr(shared_addr(&bins.total[search][rank]), t), block);
+        cluster_sync(size);
+        for (unsigned r = 0; r < size; ++r) {
+            if (r < rank) upto += bins.total[search][r];
+            all += bins.total[search][r];
         }
         const u64 target = goal(all);
         u64 sum = upto - mine;
         if (sum < target && target <= upto) {
 #pragma unroll 1
-            for (int i = 0; i < PER; ++i) {
-                const u64 w = of(PER * t + i);
-                if (sum < target && target <= sum + w) bins.found = PER * t + i, bins.before = sum, bins.equals = (unsigned)counted(PER * t + i);
+            for (int bin = bin0; bin < bin1; ++bin) {
+                const u64 w = of(bin);
+                if (sum < target && target <= sum + w)
+                    for (unsigned r = 0; r < size; ++r)
+                        peer_store(peer_addr(shared_addr(&bins.found[search][0]), r), sum, counted(bin) << 32 | (unsigned)bin);
                 sum += w;
             }
         }
+        cluster_sync(size);
+        before = bins.found[search][0];
+        const u64 f = bins.found[search][1];
+        equals = (unsigned)(f >> 32);
         __syncthreads();
-        const int found = bins.found;
-        before = bins.before, equals = bins.equals;
-        __syncthreads();
-        return found;
+        return f == ~0ull ? -1 : (int)(unsigned)f;
     };
     if (k > 0) {
-        const int bin = find(counted, [&](u64) { return k; });
+        const int bin = find(0, counted, [&](u64) { return k; });
         if (bin < 0) { /* fewer than k */
             k = 0;
             if (!(top_p < 1.0)) return Border{key_of(neg_inf()), 0, 0};
@@ -719,13 +742,13 @@ __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineB
     /* by weight: of a bin that is not one key only bounds are known, that of its lowest and of its highest score */
     u64 target = 0;
     auto goal = [&](u64 all) { return target = max(1ull, (u64)ceil(top_p * (double)(EXACT ? all : total))); };
-    int to = find([&](int bin) { return weighed(bin, false); }, goal), first = to;
+    int to = find(0, [&](int bin) { return weighed(bin, false); }, goal), first = to;
     if (EXACT && to >= 0 && to != middle && to != last) {
         const unsigned key = order.highest(to) < 0x8000u ? order.highest(to) << 16 | 0xffffu : order.lowest(to) << 16;
         const u64 w = weigh.weight(value_of(key));
         return Border{key, (unsigned)min((target - before + w - 1) / w, (u64)equals), equals};
     }
-    if (!EXACT) first = find([&](int bin) { return weighed(bin, true); }, goal);
+    if (!EXACT) first = find(1, [&](int bin) { return weighed(bin, true); }, goal);
     const unsigned klo = to < 0 ? key_of(from) : max(key_of(from), order.lowest(to) << 16);
     const unsigned khi = first < 0 ? key_of(most) : order.highest(first) << 16 | 0xffffu;
     if (!EXACT) { /* what lies above the first bin that may hold the border */
@@ -737,13 +760,12 @@ __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineB
             for (int i = 0; i < E; ++i)
                 if (key_of(f[i]) > khi) more += weigh.weight(f[i]);
         }
-        more = warp_sum(more);
-        if (lane == 0) bins.warp[warp] = more;
+        more = block_total(more);
+        if (t < (int)size) peer_store1(peer_addr(shared_addr(&bins.shared[rank][0]), t), more);
         cluster_sync(size);
         before = 0;
-        for (unsigned r = 0; r < size; ++r)
-            for (int w = 0; w < kWarps; ++w) before += peer_load1(peer_addr(shared_addr(&bins.warp[w]), r));
-        cluster_sync(size);
+        for (unsigned r = 0; r < size; ++r) before += bins.shared[r][0];
+        __syncthreads();
     }
     const Border b = find_border<T, RESIDENT, true>(share, get, lv, size, klo, khi, target - before, weigh, 0.0, 0);
     return b.ties != 0xffffffffu ? b : Border{klo - 1, 0, 0};
