@@ -284,11 +284,17 @@ def _bytes_of(value, dtype=None):
 ROWS_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 
 
+_element_types = {}  # names by dtype
+
+
 def _element_type(t) -> str:
     """"float32", "bfloat16", ... of a tensor or a ``DeviceArray``."""
-    if not hasattr(t, "dtype"):
-        raise TypeError(f"not a device array: {type(t)!r}")
-    return str(t.dtype).rsplit(".", 1)[-1]
+    try:
+        return _element_types[t.dtype]
+    except KeyError:
+        return _element_types.setdefault(t.dtype, str(t.dtype).rsplit(".", 1)[-1])
+    except AttributeError:
+        raise TypeError(f"not a device array: {type(t)!r}") from None
 
 
 class DeviceArray:
@@ -559,24 +565,22 @@ class Context:
         return b if in_b.value else a
 
     # -- rows of scores
-    def _on_device(self, name, t, kinds, shape):
+    def _address(self, name, t, kinds, shape):
         """The address of an argument that must be a contiguous device array of this shape and one of these types."""
         if t is None:
             return None
         kind = _element_type(t)
         if kind not in kinds:
             raise AccbError(EINVAL, f"{name}: elements of type {kind}, not {' or '.join(kinds)}")
-        if tuple(t.shape) != tuple(shape):
-            raise AccbError(EINVAL, f"{name}: shape {tuple(t.shape)}, not {tuple(shape)}")
-        if hasattr(t, "is_contiguous") and not t.is_contiguous():
+        if t.shape != shape:
+            raise AccbError(EINVAL, f"{name}: shape {tuple(t.shape)}, not {shape}")
+        if isinstance(t, DeviceArray):
+            return t.ptr
+        if not t.is_contiguous():
             raise AccbError(EINVAL, f"{name}: not contiguous")
-        self._check_device(name, t)
-        return C.c_void_p(_ptr(t))
-
-    def _check_device(self, name, t):
-        device = getattr(t, "device", None)
-        if device is not None and (device.type != "cuda" or device.index != self.device):
-            raise AccbError(EINVAL, f"{name}: on {device}, not on cuda:{self.device}")
+        if t.get_device() != self.device:
+            raise AccbError(EINVAL, f"{name}: on {t.device}, not on cuda:{self.device}")
+        return t.data_ptr()
 
     def _rows(self, name, t) -> accb_rows_array:
         """A matrix of scores: contiguous rows, any distance from row to row."""
@@ -585,26 +589,24 @@ class Context:
             raise AccbError(EINVAL, f"{name}: elements of type {kind}, not {' or '.join(ROWS_TYPES)}")
         if len(t.shape) != 2:
             raise AccbError(EINVAL, f"{name}: rank {len(t.shape)}, not 2")
-        rows, cols = (int(e) for e in t.shape)
-        pitch = cols
-        if hasattr(t, "stride"):
-            if cols > 1 and t.stride(1) != 1:
-                raise AccbError(EINVAL, f"{name}: the entries of a row are not contiguous")
-            pitch = int(t.stride(0)) if rows > 1 else cols
+        rows, cols = t.shape
         if cols >= 1 << 31:
             raise AccbError(EINVAL, f"{name}: rows of {cols} entries")
-        self._check_device(name, t)
-        return accb_rows_array(_ptr(t), ROWS_TYPES[kind], cols, rows, pitch)
+        if isinstance(t, DeviceArray):
+            return accb_rows_array(t.ptr, ROWS_TYPES[kind], cols, rows, cols)
+        pitch, inner = t.stride()
+        if cols > 1 and inner != 1:
+            raise AccbError(EINVAL, f"{name}: the entries of a row are not contiguous")
+        if t.get_device() != self.device:
+            raise AccbError(EINVAL, f"{name}: on {t.device}, not on cuda:{self.device}")
+        return accb_rows_array(t.data_ptr(), ROWS_TYPES[kind], cols, rows, pitch if rows > 1 else cols)
 
     def _own_stream(self, stream):
         """The given stream, or the current one of this context's device."""
-        if stream is not None:
-            return C.c_void_p(int(stream))
-        try:
+        if stream is None:
             import torch
-        except ImportError:
-            return C.c_void_p(0)
-        return C.c_void_p(int(torch.cuda.current_stream(self.device).cuda_stream))
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return int(stream)
 
     def top_rows(self, x, values, index, lse=None, temperature: float = 1.0, stream=None):
         """The ``k`` largest scores of every row of ``x`` in falling order (equal ones by rising index) and where they
@@ -614,10 +616,10 @@ class Context:
         if len(values.shape) != 2:
             raise AccbError(EINVAL, f"values: rank {len(values.shape)}, not 2")
         k = int(values.shape[1])
-        v = self._on_device("values", values, (_element_type(x),), (a.rows, k))
-        i = self._on_device("index", index, ("int32",), (a.rows, k))
-        s = self._on_device("lse", lse, ("float32",), (a.rows,))
-        _check(lib().accb_top_rows(self.handle, self._own_stream(stream), C.byref(a), temperature, k, v, i, s), self.handle)
+        v = self._address("values", values, (_element_type(x),), (a.rows, k))
+        i = self._address("index", index, ("int32",), (a.rows, k))
+        s = self._address("lse", lse, ("float32",), (a.rows,))
+        _check(lib().accb_top_rows(self.handle, self._own_stream(stream), a, temperature, k, v, i, s), self.handle)
 
     def sample_rows(self, x, uniform, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None,
                     allowed=None, stream=None):
@@ -625,22 +627,23 @@ class Context:
         ``top_k``, ``top_p`` and ``min_p`` keep (arrays of one value per row, or None).  ``allowed``: rows x
         ceil(cols / 32) words of bits.  See ``accb_sample_rows`` in ``include/accb200.h``."""
         a = self._rows("x", x)
-        each = [self._on_device(name, t, kinds, (a.rows,)) for name, t, kinds in (
-            ("uniform", uniform, ("float32",)), ("temperature", temperature, ("float32",)), ("top_k", top_k, ("int32",)),
-            ("top_p", top_p, ("float32",)), ("min_p", min_p, ("float32",)), ("token", token, ("int32",)),
-            ("logprob", logprob, ("float32",)))]
+        n, f32, i32 = (a.rows,), ("float32",), ("int32",)
+        each = (self._address("uniform", uniform, f32, n), self._address("temperature", temperature, f32, n),
+                self._address("top_k", top_k, i32, n), self._address("top_p", top_p, f32, n),
+                self._address("min_p", min_p, f32, n), self._address("token", token, i32, n),
+                self._address("logprob", logprob, f32, n))
         words = (a.cols + 31) // 32
-        bits = self._on_device("allowed", allowed, ("int32", "uint32"), (a.rows, words))
-        _check(lib().accb_sample_rows(self.handle, self._own_stream(stream), C.byref(a), bits, words, *each), self.handle)
+        bits = self._address("allowed", allowed, ("int32", "uint32"), (a.rows, words))
+        _check(lib().accb_sample_rows(self.handle, self._own_stream(stream), a, bits, words, *each), self.handle)
 
     def _teacher(self, a, teacher, index, teacher_lse, weight):
         if len(teacher.shape) != 2:
             raise AccbError(EINVAL, f"teacher: rank {len(teacher.shape)}, not 2")
         k = int(teacher.shape[1])
-        t = self._on_device("teacher", teacher, tuple(ROWS_TYPES), (a.rows, k))
-        i = self._on_device("index", index, ("int32",), (a.rows, k))
-        s = self._on_device("teacher_lse", teacher_lse, ("float32",), (a.rows,))
-        w = self._on_device("weight", weight, ("float32",), (a.rows,))
+        t = self._address("teacher", teacher, ROWS_TYPES, (a.rows, k))
+        i = self._address("index", index, ("int32",), (a.rows, k))
+        s = self._address("teacher_lse", teacher_lse, ("float32",), (a.rows,))
+        w = self._address("weight", weight, ("float32",), (a.rows,))
         return t, ROWS_TYPES[_element_type(teacher)], i, k, s, w
 
     def distill_rows(self, student, teacher, index, loss, grad=None, stats=None, teacher_lse=None, weight=None,
@@ -650,11 +653,10 @@ class Context:
         ``distill_rows_backward`` needs.  See ``accb_distill_rows`` in ``include/accb200.h``."""
         a = self._rows("student", student)
         t = self._teacher(a, teacher, index, teacher_lse, weight)
-        lo = self._on_device("loss", loss, ("float32",), (a.rows,))
-        st = self._on_device("stats", stats, ("float32",), (a.rows, 4))
+        lo = self._address("loss", loss, ("float32",), (a.rows,))
+        st = self._address("stats", stats, ("float32",), (a.rows, 4))
         g = self._rows("grad", grad) if grad is not None else None
-        _check(lib().accb_distill_rows(self.handle, self._own_stream(stream), C.byref(a), *t, temperature, lo, st,
-                                       C.byref(g) if g is not None else None), self.handle)
+        _check(lib().accb_distill_rows(self.handle, self._own_stream(stream), a, *t, temperature, lo, st, g), self.handle)
 
     def distill_rows_backward(self, student, teacher, index, stats, upstream, grad, teacher_lse=None, weight=None,
                               temperature: float = 1.0, stream=None):
@@ -662,11 +664,11 @@ class Context:
         losses (None: 1).  See ``accb_distill_rows_backward`` in ``include/accb200.h``."""
         a = self._rows("student", student)
         t = self._teacher(a, teacher, index, teacher_lse, weight)
-        st = self._on_device("stats", stats, ("float32",), (a.rows, 4))
-        up = self._on_device("upstream", upstream, ("float32",), (a.rows,))
+        st = self._address("stats", stats, ("float32",), (a.rows, 4))
+        up = self._address("upstream", upstream, ("float32",), (a.rows,))
         g = self._rows("grad", grad)
-        _check(lib().accb_distill_rows_backward(self.handle, self._own_stream(stream), C.byref(a), *t, temperature, st, up,
-                                                C.byref(g)), self.handle)
+        _check(lib().accb_distill_rows_backward(self.handle, self._own_stream(stream), a, *t, temperature, st, up, g),
+               self.handle)
 
     # -- synthetic inputs
     def gen_uniform_f32(self, dst, n, first, seed, stream_id, lo, hi, stream=None):

@@ -174,6 +174,7 @@ struct accb_context {
     std::set<CUfunction> carveout_set; /* entries already told to prefer shared memory over L1 */
     const void *rows_ready[32] = {}; /* kernels of rows.cu whose shared memory this context has raised */
     int rows_ready_count = 0;
+    std::map<std::tuple<const void *, int, size_t>, int> rows_clusters; /* clusters of such a kernel that the GPU holds at a time */
     std::map<std::tuple<CUfunction, int, size_t>, int> occupancy_cache; /* resident blocks per SM */
     size_t mem_hits = 0, disk_hits = 0, compiles = 0;
     bool trace_exec = false, trace_gc = false, trace_cc = false;

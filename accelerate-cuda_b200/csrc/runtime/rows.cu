@@ -40,19 +40,15 @@ template <class T> __device__ __noinline__ uint4 only_allowed(uint4 w, int e0, i
     return Elem<T>::pack(f);
 }
 
-/* Where a row's candidates are gathered: in the first block of its cluster. */
-struct Gather {
-    unsigned own;   /* entries of this block */
-    unsigned count; /* in the first block: places of the list that are taken */
-    unsigned base;  /* where this block's go */
-};
-
-/* Lists the entries of the row that are not below `least` (finite) in the first block's `list` of `room` numbers.
- * Every block lists its own first: a place in its own shared memory costs a fraction of one in another block's.  The
- * counts still have to be told; returns this block's. */
+/* Lists the entries of the row that are not below `least` (finite) in `list` of the block `to` of the cluster, which
+ * finishes the row: a part of `room / size` places for every block.  `own`, zero before, counts this block's; a block
+ * lists its own first, since a place in its own shared memory costs a fraction of one in another block's.  The counts
+ * still have to be told; returns this block's. */
 template <class T, bool R, class Raw>
-__device__ unsigned gather(const Share<T, R> &share, Raw raw, float least, u64 *list, unsigned room, Gather &g, unsigned rank) {
+__device__ unsigned gather(const Share<T, R> &share, Raw raw, float least, u64 *mine, u64 *list, unsigned room, unsigned &own, unsigned rank,
+                           unsigned size, unsigned to) {
     constexpr int E = Elem<T>::E;
+    const unsigned part = room / size;
 #pragma unroll 2
     for (int v = share.first; v < share.last; v += 32) {
         const uint4 w = raw(v);
@@ -61,29 +57,36 @@ __device__ unsigned gather(const Share<T, R> &share, Raw raw, float least, u64 *
         if (!(largest.get() >= least)) continue;
         float f[E];
         Elem<T>::unpack(w, f);
-#pragma unroll 1
-        for (int i = 0; i < E; ++i) {
-            float x = f[0];
+        unsigned found = 0;
 #pragma unroll
-            for (int j = 1; j < E; ++j)
-                if (i == j) x = f[j];
-            if (x >= least) {
-                unsigned at = atomicAdd(&g.own, 1u);
-                if (rank == 0) at = atomicAdd(&g.count, 1u);
-                if (at < room) list[at] = entry_of(x, share.entry(v) + i);
-            }
-        }
+        for (int i = 0; i < E; ++i) found |= (unsigned)(f[i] >= least) << i;
+        unsigned at = atomicAdd(&own, __popc(found));
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (((found >> i) & 1u) && at < part) mine[at++] = entry_of(f[i], share.entry(v) + i);
     }
     __syncthreads();
-    const unsigned n = g.own;
-    if (rank != 0 && n != 0) {
-        if (threadIdx.x == 0) g.base = peer_count(peer_addr(shared_addr(&g.count), 0), n);
-        __syncthreads();
-        const unsigned to = peer_addr(shared_addr(list), 0), base = g.base;
-        for (unsigned i = threadIdx.x; i < min(n, room); i += kThreads)
-            if (base + i < room) peer_store1(to + (base + i) * 8, list[i]);
-    }
+    const unsigned n = own, base = peer_addr(shared_addr(list + rank * part), to);
+    for (unsigned i = threadIdx.x; i < min(n, part); i += kThreads) peer_store1(base + i * 8, mine[i]);
     return n;
+}
+
+/* Puts the parts of a list side by side, by all threads of its block; parts hold counts(0 .. size - 1) entries. */
+template <class C> __device__ void close_up(u64 *list, unsigned room, unsigned size, C counts) {
+    const unsigned part = room / size;
+    unsigned at = counts(0);
+    for (unsigned r = 1; r < size; ++r) { /* a part moves down by less than it is away: entries first, then places */
+        const unsigned n = counts(r);
+        for (unsigned i0 = 0; i0 < n; i0 += kThreads) {
+            const unsigned i = i0 + threadIdx.x;
+            u64 e = 0;
+            if (i < n) e = list[r * part + i];
+            __syncthreads();
+            if (i < n) list[at + i] = e;
+            __syncthreads();
+        }
+        at += n;
+    }
 }
 
 /* One message of every block to all blocks of its cluster, and the barrier after it; every exchange of a launch has a
@@ -129,7 +132,17 @@ struct SampleParams {
     float *logprob;
 };
 constexpr int kSampleRoom = 512; /* candidates of a row that a block lists and sorts, ... */
-constexpr int kListed = 256;     /* ... asked for where top_k is no more */
+constexpr int kListed = 192;     /* ... asked for where top_k is no more */
+
+/* A row whose candidates are listed and that waits for its block to draw from them. */
+struct PendingDraw {
+    long long row;
+    u64 total;
+    double temperature;
+    float most, lowest, top_p, uniform;
+    int k;
+    unsigned n[kMaxCluster]; /* candidates by block */
+};
 
 /* the whole part of uniform * total below total */
 __device__ __forceinline__ u64 drawn(float uniform, u64 total) {
@@ -145,10 +158,16 @@ __device__ __forceinline__ void put_token(const SampleParams &p, long long row, 
     }
 }
 
-/* Draws from the n candidates in `list`, which hold every entry that top_k and top_p could keep; by one block. */
-template <class W>
-__device__ __noinline__ void draw_from_list(const SampleParams &p, long long row, u64 *list, u64 *scratch, int n, int k, float top_p,
-                                                   float lowest, u64 total, float uniform, double temperature, float most, const W &weigh) {
+/* Draws from the candidates in `list`, which hold every entry that top_k and top_p could keep; by one block. */
+template <class W> __device__ __noinline__ void draw_from_list(const SampleParams &p, const PendingDraw &d, u64 *list, u64 *scratch, unsigned size, const double *table) {
+    const W weigh(d.most, d.temperature, table);
+    const int k = d.k;
+    const float top_p = d.top_p, lowest = d.lowest;
+    u64 total = d.total;
+    int n = 0;
+    for (unsigned r = 0; r < size; ++r) n += (int)d.n[r];
+    close_up(list, kSampleRoom, size, [&](unsigned r) { return d.n[r]; });
+    __syncthreads();
     sort_down(list, n, kSampleRoom);
     if (k > 0) n = min(n, k);
     /* weights, and how many of the sorted candidates are kept: a thread has `per` of them side by side */
@@ -169,7 +188,7 @@ __device__ __noinline__ void draw_from_list(const SampleParams &p, long long row
         list[i] = list[i] << 32 | (keep ? key_of(x) : 0u);
     }
     total = block_sum(kept, scratch);
-    const u64 target = drawn(uniform, total);
+    const u64 target = drawn(d.uniform, total);
     sort_down(list, n, kSampleRoom);
     mine = 0;
     for (int i = from; i < to; ++i)
@@ -181,7 +200,7 @@ __device__ __noinline__ void draw_from_list(const SampleParams &p, long long row
             const float x = value_of((unsigned)list[i]);
             if ((unsigned)list[i]) before += weigh.weight(x);
             if (target < before) {
-                put_token(p, row, index_of(list[i] >> 32), x, most, temperature, total);
+                put_token(p, d.row, index_of(list[i] >> 32), x, d.most, d.temperature, total);
                 return;
             }
         }
@@ -191,23 +210,46 @@ __device__ __noinline__ void draw_from_list(const SampleParams &p, long long row
 template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample_rows(const __grid_constant__ SampleParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 stage[];
-    __shared__ Told told;
+    __shared__ Told told_by_turns[2];
     __shared__ union {
-        u64 list[kSampleRoom];
+        u64 mine[kSampleRoom];
         FineBins bins;
         Level level;
     } sh;
+    __shared__ u64 list[kSampleRoom];
     __shared__ double table[kTable * kTableCopies];
     __shared__ u64 scratch[kWarps];
-    __shared__ Gather g;
+    __shared__ unsigned own;
+    __shared__ PendingDraw pending;
+    __shared__ Extent extent;
     const unsigned size = cluster_size(), rank = cluster_rank();
-    const long long row = blockIdx.x / size;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (size > 1) cluster_arrive(); /* every block of the row has started: waited for before the first message */
+    const T *x = static_cast<const T *>(p.in.x);
+    const long long step = gridDim.x / size;
+    if (size > 1) cluster_arrive(); /* every block of the cluster has started: waited for before the first message */
 
     Share<T, R> share;
-    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    share.init(x + (blockIdx.x / size) * p.in.pitch, p.in.cols, rank, size, stage);
     share.fetch();
+    fill_table(table);
+    if (size > 1) cluster_wait();
+    int turn = 0;
+    unsigned finisher = 0; /* the block that draws from this row's list: blocks take it in turns and draw side by side */
+    bool waiting = false;  /* a list waits in this block */
+    for (long long row = blockIdx.x / size; row < p.in.rows; row += step, turn ^= 1) {
+    Told &told = told_by_turns[turn];
+    const bool more = row + step < p.in.rows;
+    auto draw = [&] {
+        if (!waiting) return;
+        draw_from_list<Weigh<sizeof(T) == 4>>(p, pending, list, scratch, size, table);
+        waiting = false;
+        __syncthreads(); /* the list is used again */
+    };
+    auto next = [&] { /* the scores of the next row take the place of this one's, which this thread has read */
+        if (!more) return;
+        share.init(x + (row + step) * p.in.pitch, p.in.cols, rank, size, stage);
+        share.fetch();
+    };
     const unsigned *bits = p.allowed ? p.allowed + row * p.allowed_pitch : nullptr;
     float warmth = p.temperature ? p.temperature[row] : 1.0f;
     int k = p.top_k ? p.top_k[row] : 0;
@@ -217,8 +259,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     if (!(warmth > 0.0f)) k = 1;
     const double temperature = warmth > 0.0f ? warmth : 1.0f;
     if (k >= p.in.cols || k < 0) k = 0;
-    fill_table(table);
-    if (threadIdx.x == 0) g.own = g.count = 0;
+    if (threadIdx.x == 0) own = 0;
     share.wait();
 
     bool infinite = false; /* the row's maximum is +inf: its like weigh 1, all others nothing */
@@ -250,15 +291,8 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
         if (R && bits) stage[v - share.v0] = w = only_allowed<T>(w, share.entry(v), share.n, bits);
         largest.add(w);
     }
-    float most = largest.get(), bound = neg_inf();
-    const int want = (k + (int)size - 1) / (int)size; /* of each block's threads */
-    if (k > 1 && want <= kThreads) bound = bound_of(most, want);
-    most = warp_max(most);
-    if (lane == 0) scratch[warp] = __float_as_uint(most);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, __uint_as_float((unsigned)scratch[w]));
-    if (size > 1) cluster_wait();
+    const float2 ext = extent_of(largest.get(), k > 1 ? (k + (int)size - 1) / (int)size : 0, extent);
+    float most = ext.x, bound = ext.y;
     tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
     for (int i = 0; i < (int)size; ++i) {
         most = fmaxf(most, __uint_as_float((unsigned)told.block[0][i][0]));
@@ -269,7 +303,9 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
             p.token[row] = -1;
             if (p.logprob) p.logprob[row] = neg_inf();
         }
-        return;
+        next();
+        if (!more) draw();
+        continue;
     }
     if (most == __uint_as_float(0x7f800000u)) {
         if (R) {
@@ -326,7 +362,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     Border border{key_of(cut ? neg_inf() : fmaxf(lowest, -3.402823466e+38f)) - (cut ? 0u : 1u), 0, 0};
     if (cut) {
         float least = fmaxf(bound, -3.402823466e+38f);
-        bool list = k > 0 && k <= kListed;
+        bool listed = k > 0 && k <= kListed;
         if (k == 0) { /* top_p alone */
             least = weigh.least;
             if (!kBinsWeigh) { /* entries so far down that all of them together weigh less than what is cut off */
@@ -336,18 +372,28 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
                 const double left = (1.0 - (double)top_p) * ((double)total * (1.0 / (double)(1ull << kUnitLog2)));
                 const double low = (double)most + (log_64(left / (double)p.in.cols) - 0.01) * temperature;
                 if (left > 1e-5 && low > (double)least) least = __double2float_rd(low);
-                list = true;
+                listed = true;
             }
         }
-        if (list) {
-            const unsigned n = gather(share, raw, least, sh.list, kSampleRoom, g, rank);
+        if (listed) {
+            const unsigned n = gather(share, raw, least, sh.mine, list, kSampleRoom, own, rank, size, finisher);
             tell_all(told.block[2], n, 0, rank, size);
-            unsigned all = 0;
-            for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[2][i][0];
-            if (all <= kSampleRoom) { /* the same in every block of the row */
-                if (rank == 0)
-                    draw_from_list(p, row, sh.list, scratch, (int)all, k, top_p, lowest, total, uniform, temperature, most, weigh);
-                return;
+            unsigned longest = 0;
+            for (int i = 0; i < (int)size; ++i) longest = max(longest, (unsigned)told.block[2][i][0]);
+            if (longest <= kSampleRoom / size) { /* the same in every block of the row */
+                next();
+                if (rank == finisher) {
+                    waiting = true;
+                    if (threadIdx.x < size) pending.n[threadIdx.x] = (unsigned)told.block[2][threadIdx.x][0];
+                    if (threadIdx.x == 0) {
+                        pending.row = row, pending.total = total, pending.temperature = temperature, pending.most = most;
+                        pending.lowest = lowest, pending.top_p = top_p, pending.uniform = uniform, pending.k = k;
+                    }
+                    __syncthreads();
+                }
+                finisher = finisher + 1 == size ? 0 : finisher + 1;
+                if (finisher == 0 || !more) draw();
+                continue;
             }
         }
         /* too many for a list */
@@ -411,7 +457,11 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     const u64 here = mass + quota * tie_weight;
     /* the first entry whose running sum exceeds uniform * total */
     const u64 target = drawn(uniform, total);
-    if (!(before <= target && target < before + here)) return;
+    if (!more) draw();
+    if (!(before <= target && target < before + here)) {
+        next();
+        continue;
+    }
 
     int v0 = start;
     if (quota == 0) { /* which quarter of the warp's piece */
@@ -462,11 +512,13 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
                 }
                 put_token(p, row, at, value, most, temperature, total);
             }
-            return;
+            break;
         }
         sum = __shfl_sync(~0u, reach, 31);
         const unsigned took = __shfl_sync(~0u, upto, 31);
         left = left > took ? left - took : 0;
+    }
+    next();
     }
 }
 
@@ -478,26 +530,35 @@ struct TopParams {
     float *lse;
     double temperature;
     int k;
-    int room; /* of the list of candidates, a power of two from 256 */
+    int room; /* of the list of candidates, a power of two from 512 */
 };
 
 template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_rows(const __grid_constant__ TopParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 dynamic[];
-    __shared__ Told told;
+    __shared__ Told told_by_turns[2];
     __shared__ u64 scratch[kWarps];
-    __shared__ Gather g;
+    __shared__ unsigned own, taken, counts[kMaxCluster];
+    __shared__ Extent extent;
     const unsigned size = cluster_size(), rank = cluster_rank();
-    const long long row = blockIdx.x / size;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    u64 *list = reinterpret_cast<u64 *>(dynamic);
-    Level &level = *reinterpret_cast<Level *>(dynamic); /* in the list's place */
-    if (size > 1) cluster_arrive();
+    u64 *list = reinterpret_cast<u64 *>(dynamic), *mine = list + p.room; /* `mine`: room / size places, or a Level */
+    Level &level = *reinterpret_cast<Level *>(mine);
+    const T *x = static_cast<const T *>(p.in.x);
+    const long long step = gridDim.x / size;
+    if (size > 1) cluster_arrive(); /* every block of the cluster has started: waited for before the first message */
 
     Share<T, R> share;
-    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, dynamic + max(p.room * 8, (int)sizeof(Level)) / 16);
+    share.init(x + (blockIdx.x / size) * p.in.pitch, p.in.cols, rank, size, dynamic + (p.room + max(p.room / (int)size, (int)sizeof(Level) / 8)) / 2);
     share.fetch();
-    if (threadIdx.x == 0) g.own = g.count = 0;
+    if (size > 1) cluster_wait();
+    int turn = 0;
+    unsigned finisher = 0;       /* the block that sorts this row's list: blocks take it in turns and sort side by side */
+    long long waiting = -1;      /* the row whose list waits in this block */
+    for (long long row = blockIdx.x / size; row < p.in.rows; row += step, turn ^= 1) {
+    Told &told = told_by_turns[turn];
+    const bool more = row + step < p.in.rows;
+    if (threadIdx.x == 0) own = taken = 0;
     share.wait();
     auto raw = [&](int v) { return share.get(v); };
     auto get = [&](int v, float *f) {
@@ -505,24 +566,23 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = not_nan(f[i]);
     };
+    auto next = [&] { /* the scores of the next row take the place of this one's, which this thread has read */
+        if (!more) return;
+        share.init(x + (row + step) * p.in.pitch, p.in.cols, rank, size, share.stage);
+        share.fetch();
+    };
     typename Elem<T>::Max largest;
 #pragma unroll 4
     for (int v = share.first; v < share.last; v += 32) largest.add(share.get(v));
-    float most = largest.get(), bound = neg_inf();
-    const int want = (p.k + (int)size - 1) / (int)size; /* threads of each block whose maxima make up k entries */
-    if (want <= kThreads) bound = bound_of(most, want);
-    most = warp_max(most);
-    if (lane == 0) scratch[warp] = __float_as_uint(most);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, __uint_as_float((unsigned)scratch[w]));
-    if (size > 1) cluster_wait();
+    /* threads of each block whose maxima make up k entries */
+    const float2 ext = extent_of(largest.get(), (p.k + (int)size - 1) / (int)size, extent);
+    float most = ext.x, bound = ext.y;
     tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
     for (int i = 0; i < (int)size; ++i) {
         most = fmaxf(most, __uint_as_float((unsigned)told.block[0][i][0]));
         bound = fminf(bound, __uint_as_float((unsigned)told.block[0][i][1]));
     }
-    unsigned n = 0, all = 0;
+    unsigned n = 0, longest = 0;
     double sum = 0.0;
     if (most > neg_inf()) {
         if (p.lse) {
@@ -541,17 +601,18 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             __syncthreads();
             if (lane == 0) scratch[warp] = __float_as_uint(warp_part);
         }
-        n = gather(share, raw, fmaxf(bound, -3.402823466e+38f), list, (unsigned)p.room, g, rank);
+        n = gather(share, raw, fmaxf(bound, -3.402823466e+38f), mine, list, (unsigned)p.room, own, rank, size, finisher);
         if (p.lse)
             for (int w = 0; w < kWarps; ++w) sum += (double)__uint_as_float((unsigned)scratch[w]);
         tell_all(told.block[1], n, (u64)__double_as_longlong(sum), rank, size);
         sum = 0.0;
-        for (int i = 0; i < (int)size; ++i) all += (unsigned)told.block[1][i][0], sum += __longlong_as_double((long long)told.block[1][i][1]);
+        for (int i = 0; i < (int)size; ++i) longest = max(longest, (unsigned)told.block[1][i][0]), sum += __longlong_as_double((long long)told.block[1][i][1]);
     }
     if (p.lse && rank == 0 && threadIdx.x == 0)
         p.lse[row] = most > neg_inf() && most < __uint_as_float(0x7f800000u) ? (float)((double)most / p.temperature + log_64(sum)) : most;
 
-    if (all > (unsigned)p.room) {
+    const bool crowded = longest > (unsigned)p.room / size;
+    if (crowded) {
         /* too many (ties, or rows of few large entries side by side): find the border, then list what is above it and
          * the first of what is on it */
         const Weigh<sizeof(T) == 4> none(0.0f, 1.0, nullptr);
@@ -564,7 +625,6 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             for (int i = 0; i < E; ++i) ties += key_of(f[i]) == border.key;
         }
         ties = warp_sum(ties);
-        if (threadIdx.x == 0) g.count = 0;
         if (lane < (int)size) peer_store(peer_addr(shared_addr(&told.warp[rank * kWarps + warp][0]), lane), ties, 0);
         cluster_sync(size);
         unsigned quota = 0, seen = 0;
@@ -577,7 +637,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             seen = __shfl_sync(~0u, upto, 31);
         }
         quota = __shfl_sync(~0u, quota, self & 31);
-        const unsigned lowest = key_of(neg_inf()), to = peer_addr(shared_addr(list), 0), count = peer_addr(shared_addr(&g.count), 0);
+        const unsigned lowest = key_of(neg_inf()), to = peer_addr(shared_addr(list), finisher), count = peer_addr(shared_addr(&taken), finisher);
         for (int v0 = share.first - lane; v0 < share.last; v0 += 32) {
             const int v = v0 + lane;
             float f[E];
@@ -606,14 +666,28 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             quota = quota > took ? quota - took : 0;
         }
         cluster_sync(size);
-        all = rank == 0 ? g.count : 0;
     }
-    if (rank != 0) return;
-    sort_down(list, (int)all, p.room);
-    for (int i = threadIdx.x; i < p.k; i += kThreads) {
-        const u64 e = i < (int)all ? list[i] : 0;
-        static_cast<T *>(p.values)[row * p.k + i] = Elem<T>::down(e ? score_of(e) : neg_inf());
-        p.index[row * p.k + i] = e ? index_of(e) : -1;
+    next();
+    if (rank == finisher) {
+        waiting = row;
+        if (threadIdx.x < size) counts[threadIdx.x] = most == neg_inf() ? 0 : crowded ? (threadIdx.x == 0 ? taken : 0) : (unsigned)told.block[1][threadIdx.x][0];
+        __syncthreads();
+    }
+    finisher = finisher + 1 == size ? 0 : finisher + 1;
+    if ((finisher == 0 || !more) && waiting >= 0) {
+        unsigned all = 0;
+        for (unsigned r = 0; r < size; ++r) all += counts[r];
+        close_up(list, (unsigned)p.room, size, [&](unsigned r) { return counts[r]; });
+        __syncthreads();
+        sort_down(list, (int)all, p.room);
+        for (int i = threadIdx.x; i < p.k; i += kThreads) {
+            const u64 e = i < (int)all ? list[i] : 0;
+            static_cast<T *>(p.values)[waiting * p.k + i] = Elem<T>::down(e ? score_of(e) : neg_inf());
+            p.index[waiting * p.k + i] = e ? index_of(e) : -1;
+        }
+        waiting = -1;
+        __syncthreads(); /* the list is used again */
+    }
     }
 }
 
@@ -921,7 +995,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
 }
 
 /* ----------------------------------------------------------------- host */
-constexpr size_t kSharedMost = 200u << 10; /* dynamic shared memory a block may ask for (227 KB less what it declares) */
+constexpr size_t kSharedMost = 192u << 10; /* dynamic shared memory a block may ask for (227 KB less what it declares) */
 constexpr long long kShareBytes = 64 << 10; /* the share of a row a block aims to hold */
 
 /* Blocks per row: as few as hold the row in shares of 64 KB (two or three blocks of an SM then overlap one another's
@@ -966,13 +1040,16 @@ static int check_rows(accb_context *ctx, const accb_rows_array *a, const char *w
 
 static RowsIn rows_in(const accb_rows_array *a) { return RowsIn{a->ptr, a->rows, a->pitch, a->cols}; }
 
+/* shared memory of a block's share of a row */
+static size_t share_bytes(const accb_rows_array *a, int size) {
+    return 16 * (size_t)(a->type == ACCB_ROWS_F32 ? Share<float, true>::per_block(a->cols, size) : Share<__half, true>::per_block(a->cols, size));
+}
+
 /* one launch with `size` blocks per row; `fixed` bytes of dynamic shared memory besides the share */
 template <class P>
 static int launch_rows(accb_context *ctx, void (*resident)(const P), void (*streaming)(const P), const P &p, const accb_rows_array *a, int size,
-                       size_t fixed, cudaStream_t stream, const char *name) {
-    const long long per16 = 16 / (long long)size_of(a->type);
-    const long long nvec = (a->cols + 2 * per16 - 2) / per16; /* of the worst placed row */
-    const size_t share = (size_t)((nvec + size - 1) / size) * 16;
+                       size_t fixed, bool persistent, cudaStream_t stream, const char *name) {
+    const size_t share = share_bytes(a, size);
     const bool fits = fixed + share <= kSharedMost;
     void (*kernel)(const P) = fits ? resident : streaming;
     const size_t smem = fixed + (fits ? share : 0);
@@ -983,20 +1060,31 @@ static int launch_rows(accb_context *ctx, void (*resident)(const P), void (*stre
         if (st != ACCB_OK) return st;
         ctx->rows_ready[ctx->rows_ready_count++] = (const void *)kernel;
     }
-    if (ctx->trace_exec)
-        fprintf(stderr, "[accb exec] %s<<<%lld,%d,%zu>>> rows=%lld cols=%d\n", name, a->rows * size, kThreads, smem, a->rows, a->cols);
+    long long clusters = a->rows;
     cudaLaunchAttribute attr;
     memset(&attr, 0, sizeof attr);
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)size;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(a->rows * size));
+    cfg.gridDim = dim3((unsigned)(clusters * size));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    if (persistent) { /* as many clusters as the GPU holds at a time, if there are more rows */
+        int &most = ctx->rows_clusters[std::make_tuple((const void *)kernel, size, smem)];
+        if (most == 0) {
+            const int st = check_cuda(ctx, cudaOccupancyMaxActiveClusters(&most, (const void *)kernel, &cfg), name);
+            if (st != ACCB_OK) return st;
+            most = std::max(1, most);
+        }
+        clusters = std::min<long long>(clusters, most);
+        cfg.gridDim = dim3((unsigned)(clusters * size));
+    }
+    if (ctx->trace_exec)
+        fprintf(stderr, "[accb exec] %s<<<%lld,%d,%zu>>> rows=%lld cols=%d\n", name, clusters * size, kThreads, smem, a->rows, a->cols);
     void *args[] = {const_cast<P *>(&p)};
     const int st = check_cuda(ctx, cudaLaunchKernelExC(&cfg, (const void *)kernel, args), name);
     if (st == ACCB_OK) ctx->launches++;
@@ -1018,12 +1106,12 @@ int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *
     if (!(temperature > 1e-30) || temperature > 1e30) return fail(ctx, ACCB_EINVAL, "top_rows: bad temperature %g", temperature);
     if (x->rows == 0) return ACCB_OK;
     if (!values || !index) return fail(ctx, ACCB_EINVAL, "top_rows: null result");
-    int room = 256;
-    while (room < 2 * k && room < 2 * kMaxK) room *= 2;
+    int room = 512;
+    while (room < 2 * k) room *= 2;
     const TopParams p{rows_in(x), values, index, lse, temperature, k, room};
-    const size_t fixed = std::max(room * sizeof(u64), sizeof(Level));
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
-#define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, fixed, (cudaStream_t)stream, "top_rows")
+    const size_t fixed = room * sizeof(u64) + std::max(room / size * sizeof(u64), sizeof(Level));
+#define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, fixed, true, (cudaStream_t)stream, "top_rows")
     return BY_TYPE(x->type, CALL);
 #undef CALL
 }
@@ -1039,7 +1127,7 @@ int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_rows_arra
     if (!uniform || !token) return fail(ctx, ACCB_EINVAL, "sample_rows: null random numbers or result");
     const SampleParams p{rows_in(x), allowed, allowed_pitch, uniform, temperature, top_p, min_p, top_k, token, logprob};
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
-#define CALL(T) launch_rows(ctx, sample_rows<T, true>, sample_rows<T, false>, p, x, size, 0, (cudaStream_t)stream, "sample_rows")
+#define CALL(T) launch_rows(ctx, sample_rows<T, true>, sample_rows<T, false>, p, x, size, 0, true, (cudaStream_t)stream, "sample_rows")
     return BY_TYPE(x->type, CALL);
 #undef CALL
 }
@@ -1064,13 +1152,12 @@ static int distill(accb_context *ctx, accb_stream stream, const accb_rows_array 
     if (backward ? !p.stats || !grad : !p.loss) return fail(ctx, ACCB_EINVAL, "%s: null result or statistics", what);
     p.in = rows_in(student);
     const int size = cluster_for(student->rows, (long long)student->cols * size_of(student->type), ctx->sm_count);
-    const long long e = 16 / (long long)size_of(student->type);
-    const long long share = ((student->cols + 2 * e - 2) / e + size - 1) / size * e; /* entries of a block's share, at most */
+    const long long share = (long long)share_bytes(student, size) / size_of(student->type); /* entries of a block's share, at most */
     p.map_words = (int)((share + 31) / 32 + 3) & ~3;
     const size_t fixed = (size_t)(p.map_words * 4 + p.k * sizeof(Named) + 15) / 16 * 16;
 #define CALL(T)                                                                                                                       \
-    (backward ? launch_rows(ctx, distill_rows<T, true, true>, distill_rows<T, false, true>, p, student, size, fixed, (cudaStream_t)stream, what) \
-              : launch_rows(ctx, distill_rows<T, true, false>, distill_rows<T, false, false>, p, student, size, fixed, (cudaStream_t)stream, what))
+    (backward ? launch_rows(ctx, distill_rows<T, true, true>, distill_rows<T, false, true>, p, student, size, fixed, false, (cudaStream_t)stream, what) \
+              : launch_rows(ctx, distill_rows<T, true, false>, distill_rows<T, false, false>, p, student, size, fixed, false, (cudaStream_t)stream, what))
     return BY_TYPE(student->type, CALL);
 #undef CALL
 }

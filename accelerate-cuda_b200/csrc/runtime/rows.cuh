@@ -260,7 +260,9 @@ static __device__ __noinline__ double exp_64(double x) { return exp(x); }
 static __device__ __noinline__ double log_64(double x) { return log(x); }
 
 /* A block's share of one row, in vectors of 16 bytes counted from the row's address rounded down to 16 bytes.
- * Entries of an edge vector that lie outside the row read as -inf. */
+ * Entries of an edge vector that lie outside the row read as -inf.  Which vectors a thread has, and where they are
+ * staged, is the same for all rows of a matrix, wherever they start: a thread may replace its own vectors by those of
+ * the next row as soon as it has read them. */
 template <class T, bool RESIDENT> struct Share {
     static constexpr int E = Elem<T>::E;
     const T *base;   /* the row's address rounded down to 16 bytes */
@@ -270,15 +272,17 @@ template <class T, bool RESIDENT> struct Share {
     int first, last; /* this thread's: first, first + 32, ... below last */
     uint4 *stage;
 
+    static __host__ __device__ __forceinline__ int per_block(int cols, int size) { /* vectors of a share, at most */
+        return ((cols + 2 * E - 2) / E + size - 1) / size;
+    }
     __device__ __forceinline__ void init(const T *row, int cols, unsigned rank, unsigned size, uint4 *smem) {
         lead = (int)((reinterpret_cast<unsigned long long>(row) & 15u) / sizeof(T));
         base = row - lead;
         n = cols;
-        const int nvec = (lead + cols + E - 1) / E;
-        const int per = (nvec + (int)size - 1) / (int)size;
-        v0 = min(nvec, (int)rank * per);
-        v1 = min(nvec, v0 + per);
-        const int piece = ((v1 - v0 + kWarps - 1) / kWarps + 31) & ~31;
+        const int nvec = (lead + cols + E - 1) / E, per = per_block(cols, (int)size);
+        v0 = (int)rank * per;
+        v1 = max(v0, min(nvec, v0 + per));
+        const int piece = ((per + kWarps - 1) / kWarps + 31) & ~31;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         first = v0 + warp * piece + lane;
         last = min(v1, v0 + (warp + 1) * piece);
@@ -292,6 +296,7 @@ template <class T, bool RESIDENT> struct Share {
     }
     /* start the copies of this thread's vectors; wait() before the first get() */
     __device__ __forceinline__ void fetch() const {
+#pragma unroll 4
         for (int v = RESIDENT ? first : last; v < last; v += 32) {
             if (whole(v))
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(stage + (v - v0))),
@@ -300,10 +305,9 @@ template <class T, bool RESIDENT> struct Share {
             else
                 stage[v - v0] = edge<T>(base, v, lead, n);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     }
     __device__ __forceinline__ void wait() const {
-        if (RESIDENT) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (RESIDENT) asm volatile("cp.async.wait_all;" ::: "memory");
     }
     __device__ __forceinline__ uint4 get(int v) const { return RESIDENT ? stage[v - v0] : from_memory(v); }
 };
@@ -430,17 +434,40 @@ static __device__ __noinline__ void sort_down(u64 *list, int n, int room) {
     __syncthreads();
 }
 
-/* A score that at least `want` of the block's threads reach with the largest of theirs: the largest such value in 16
- * leading bits of its key, bit by bit. */
-static __device__ __noinline__ float bound_of(float most, int want) {
-    const unsigned key = key_of(most) >> 16;
-    unsigned found = 0;
-#pragma unroll 1
-    for (int b = 15; b >= 0; --b) {
-        const unsigned trial = found | 1u << b;
-        if (__syncthreads_count(key >= trial) >= want) found = trial;
+/* The largest of the block's scores, and one that at least `want` of its threads reach with the largest of theirs: the
+ * want-th largest of these, rounded down to a bfloat16 (-inf where want is 0 or more than there are threads).  A
+ * thread counts how many of the 256 are above its own, two at a time. */
+struct Extent {
+    alignas(16) __nv_bfloat16 thread[kThreads];
+    float warp[kWarps][2];
+};
+static __device__ __noinline__ float2 extent_of(float most, int want, Extent &x) {
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const bool search = want > 0 && want <= kThreads;
+    float bound = neg_inf();
+    if (search) {
+        const __nv_bfloat16 own = __float2bfloat16_rd(most);
+        const __nv_bfloat162 pair = __halves2bfloat162(own, own);
+        x.thread[t] = own;
+        __syncthreads();
+        __nv_bfloat162 above[2] = {__floats2bfloat162_rn(0.0f, 0.0f), __floats2bfloat162_rn(0.0f, 0.0f)}; /* exact up to 256 */
+#pragma unroll 4
+        for (int i = 0; i < kThreads / 8; ++i) {
+            const uint4 w = reinterpret_cast<const uint4 *>(x.thread)[i];
+            const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) above[j & 1] = __hadd2(above[j & 1], __hgt2(*reinterpret_cast<const __nv_bfloat162 *>(&u[j]), pair));
+        }
+        const float2 a = __bfloat1622float2(above[0]), b = __bfloat1622float2(above[1]);
+        bound = a.x + a.y + b.x + b.y < (float)want ? __bfloat162float(own) : __uint_as_float(0x7f800000u);
+        bound = warp_min(bound);
     }
-    return found > 0x80u ? value_of(found << 16) : neg_inf();
+    most = warp_max(most);
+    if (lane == 0) x.warp[warp][0] = most, x.warp[warp][1] = bound;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, x.warp[w][0]), bound = fminf(bound, x.warp[w][1]);
+    return make_float2(most, bound);
 }
 
 /* ---------------------------------------------------------------- borders */
