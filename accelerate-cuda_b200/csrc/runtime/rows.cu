@@ -41,29 +41,43 @@ template <class T> __device__ __noinline__ uint4 only_allowed(uint4 w, int e0, i
 }
 
 /* Lists the entries of the row that are not below `least` (finite) in `list` of the block `to` of the cluster, which
- * finishes the row: a part of `room / size` places for every block.  `own`, zero before, counts this block's; a block
- * lists its own first, since a place in its own shared memory costs a fraction of one in another block's.  The counts
- * still have to be told; returns this block's. */
+ * finishes the row: a part of `room / size` places for every block.  `most` is the largest of this thread's scores:
+ * where few threads have any such entry, a warp looks through their vectors together, a lane each.  `own`, zero
+ * before, counts this block's; a block lists its own first, since a place in its own shared memory costs a fraction of
+ * one in another block's.  The counts still have to be told; returns this block's. */
 template <class T, bool R, class Raw>
-__device__ unsigned gather(const Share<T, R> &share, Raw raw, float least, u64 *mine, u64 *list, unsigned room, unsigned &own, unsigned rank,
-                           unsigned size, unsigned to) {
+__device__ unsigned gather(const Share<T, R> &share, Raw raw, float most, float least, u64 *mine, u64 *list, unsigned room, unsigned &own,
+                           unsigned rank, unsigned size, unsigned to) {
     constexpr int E = Elem<T>::E;
     const unsigned part = room / size;
-#pragma unroll 2
-    for (int v = share.first; v < share.last; v += 32) {
-        const uint4 w = raw(v);
-        typename Elem<T>::Max largest;
-        largest.add(w);
-        if (!(largest.get() >= least)) continue;
-        float f[E];
-        Elem<T>::unpack(w, f);
-        unsigned found = 0;
+    const int lane = threadIdx.x & 31, start = share.first - lane;
+    /* a round: lane by lane of those that have any, or vector by vector of all lanes, whichever takes fewer */
+    unsigned have = __ballot_sync(~0u, most >= least);
+    const bool by_lane = 32 * __popc(have) < share.last - start;
+    const int far = by_lane ? 32 * 32 : 32;
+    int v = start + lane;
+    for (;;) {
+        if (by_lane) {
+            if (!have) break;
+            v = start + __ffs(have) - 1 + 32 * lane;
+            have &= have - 1;
+        }
+        for (; v < share.last; v += far) {
+            const uint4 w = raw(v);
+            typename Elem<T>::Max largest;
+            largest.add(w);
+            if (!(largest.get() >= least)) continue;
+            float f[E];
+            Elem<T>::unpack(w, f);
+            unsigned found = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) found |= (unsigned)(f[i] >= least) << i;
-        unsigned at = atomicAdd(&own, __popc(found));
+            for (int i = 0; i < E; ++i) found |= (unsigned)(f[i] >= least) << i;
+            unsigned at = atomicAdd(&own, __popc(found));
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (((found >> i) & 1u) && at < part) mine[at++] = entry_of(f[i], share.entry(v) + i);
+            for (int i = 0; i < E; ++i)
+                if (((found >> i) & 1u) && at < part) mine[at++] = entry_of(f[i], share.entry(v) + i);
+        }
+        if (!by_lane) break;
     }
     __syncthreads();
     const unsigned n = own, base = peer_addr(shared_addr(list + rank * part), to);
@@ -291,7 +305,8 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
         if (R && bits) stage[v - share.v0] = w = only_allowed<T>(w, share.entry(v), share.n, bits);
         largest.add(w);
     }
-    const float2 ext = extent_of(largest.get(), k > 1 ? (k + (int)size - 1) / (int)size : 0, extent);
+    float thread_most = largest.get();
+    const float2 ext = extent_of(thread_most, k > 1 ? (k + (int)size - 1) / (int)size : 0, extent);
     float most = ext.x, bound = ext.y;
     tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
     for (int i = 0; i < (int)size; ++i) {
@@ -318,7 +333,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
             }
         }
         infinite = true;
-        most = 0.0f, bound = neg_inf();
+        most = 0.0f, bound = neg_inf(), thread_most = thread_most == __uint_as_float(0x7f800000u) ? 0.0f : neg_inf();
     }
 
     /* the lowest score that min_p keeps */
@@ -376,7 +391,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
             }
         }
         if (listed) {
-            const unsigned n = gather(share, raw, least, sh.mine, list, kSampleRoom, own, rank, size, finisher);
+            const unsigned n = gather(share, raw, thread_most, least, sh.mine, list, kSampleRoom, own, rank, size, finisher);
             tell_all(told.block[2], n, 0, rank, size);
             unsigned longest = 0;
             for (int i = 0; i < (int)size; ++i) longest = max(longest, (unsigned)told.block[2][i][0]);
@@ -530,7 +545,7 @@ struct TopParams {
     float *lse;
     double temperature;
     int k;
-    int room; /* of the list of candidates, a power of two from 512 */
+    int room; /* of the list of candidates, a power of two from 256 */
 };
 
 template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_rows(const __grid_constant__ TopParams p) {
@@ -575,7 +590,8 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
 #pragma unroll 4
     for (int v = share.first; v < share.last; v += 32) largest.add(share.get(v));
     /* threads of each block whose maxima make up k entries */
-    const float2 ext = extent_of(largest.get(), (p.k + (int)size - 1) / (int)size, extent);
+    const float thread_most = largest.get();
+    const float2 ext = extent_of(thread_most, (p.k + (int)size - 1) / (int)size, extent);
     float most = ext.x, bound = ext.y;
     tell_all(told.block[0], __float_as_uint(most), __float_as_uint(bound), rank, size);
     for (int i = 0; i < (int)size; ++i) {
@@ -601,7 +617,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             __syncthreads();
             if (lane == 0) scratch[warp] = __float_as_uint(warp_part);
         }
-        n = gather(share, raw, fmaxf(bound, -3.402823466e+38f), mine, list, (unsigned)p.room, own, rank, size, finisher);
+        n = gather(share, raw, thread_most, fmaxf(bound, -3.402823466e+38f), mine, list, (unsigned)p.room, own, rank, size, finisher);
         if (p.lse)
             for (int w = 0; w < kWarps; ++w) sum += (double)__uint_as_float((unsigned)scratch[w]);
         tell_all(told.block[1], n, (u64)__double_as_longlong(sum), rank, size);
@@ -1106,7 +1122,7 @@ int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *
     if (!(temperature > 1e-30) || temperature > 1e30) return fail(ctx, ACCB_EINVAL, "top_rows: bad temperature %g", temperature);
     if (x->rows == 0) return ACCB_OK;
     if (!values || !index) return fail(ctx, ACCB_EINVAL, "top_rows: null result");
-    int room = 512;
+    int room = 256;
     while (room < 2 * k) room *= 2;
     const TopParams p{rows_in(x), values, index, lse, temperature, k, room};
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);

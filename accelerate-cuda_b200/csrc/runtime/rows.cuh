@@ -30,7 +30,7 @@ namespace accb_rows {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 2 * kThreads;    /* bins of one level of the border search: two per thread */
+constexpr int kBins = kThreads;        /* bins of one level of the border search: one per thread */
 constexpr int kMaxK = 1024;            /* most entries of a top list */
 constexpr long long kMaxCols = 1 << 20;
 
@@ -435,24 +435,31 @@ static __device__ __noinline__ void sort_down(u64 *list, int n, int room) {
 }
 
 /* The largest of the block's scores, and one that at least `want` of its threads reach with the largest of theirs: the
- * want-th largest of these, rounded down to a bfloat16 (-inf where want is 0 or more than there are threads).  A
- * thread counts how many of the 256 are above its own, two at a time. */
+ * want-th largest of these, or of the largest of four neighbours each where that leaves enough, rounded down to a
+ * bfloat16 (-inf where want is 0 or more than there are threads).  A thread counts how many are above its own, two at a
+ * time. */
 struct Extent {
     alignas(16) __nv_bfloat16 thread[kThreads];
     float warp[kWarps][2];
 };
 static __device__ __noinline__ float2 extent_of(float most, int want, Extent &x) {
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const bool search = want > 0 && want <= kThreads;
     float bound = neg_inf();
-    if (search) {
-        const __nv_bfloat16 own = __float2bfloat16_rd(most);
+    if (want > 0 && want <= kThreads) {
+        const bool fours = want <= kThreads / 8;
+        float group = most;
+        if (fours) {
+            group = fmaxf(group, __shfl_xor_sync(~0u, group, 1));
+            group = fmaxf(group, __shfl_xor_sync(~0u, group, 2));
+        }
+        const __nv_bfloat16 own = __float2bfloat16_rd(group);
         const __nv_bfloat162 pair = __halves2bfloat162(own, own);
-        x.thread[t] = own;
+        if (!fours || (lane & 3) == 0) x.thread[fours ? t >> 2 : t] = own;
         __syncthreads();
         __nv_bfloat162 above[2] = {__floats2bfloat162_rn(0.0f, 0.0f), __floats2bfloat162_rn(0.0f, 0.0f)}; /* exact up to 256 */
+        const int vectors = (fours ? kThreads / 4 : kThreads) / 8;
 #pragma unroll 4
-        for (int i = 0; i < kThreads / 8; ++i) {
+        for (int i = 0; i < vectors; ++i) {
             const uint4 w = reinterpret_cast<const uint4 *>(x.thread)[i];
             const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -492,10 +499,10 @@ struct Level { /* one level of the border search */
  * row, or what is above them is left out), that holds `target` entries (BY_MASS false) or, BY_MASS, the weight
  * `target`, or where that is 0 the given fraction of what the range holds less the weight of `spare` entries of key klo.
  *
- * Every level lays 512 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
- * the border lies and goes on with that bin's range; when a bin is one key, the rest is arithmetic.  For 16-bit
- * scores one or two levels do, for 32-bit ones up to four.  Bins are summed over the cluster by reading the other
- * blocks' bins, two per thread; every block does that for itself and so learns the result without another message.
+ * Every level lays 256 bins over the range of keys, counts (and weighs) the entries of each, finds the bin in which
+ * the border lies and goes on with that bin's range; when a bin is one key, the rest is arithmetic.  Bins are summed
+ * over the cluster by reading the other blocks' bins, one per thread; every block does that for itself and so learns
+ * the result without another message.
  * The way for rows whose candidates are too many for a list.  All threads of the cluster call it with the same
  * arguments. */
 template <class T, bool RESIDENT, bool BY_MASS, class Get>
@@ -507,10 +514,9 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
     bool have_target = target != 0;
     for (;;) {
         const unsigned span = khi - klo;
-        const int shift = max(S0, 23 - __clz(span)); /* span >> shift < 512 */
+        const int shift = max(S0, 24 - __clz(span)); /* span >> shift < 256 */
         const bool by_entry = BY_MASS && shift > S0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) lv.count[t + i * kThreads] = 0, lv.mass[t + i * kThreads] = 0;
+        lv.count[t] = 0, lv.mass[t] = 0;
         if (t == 0) lv.found = 0;
         __syncthreads();
         for (int v = share.first; v < share.last; v += 32) {
@@ -527,28 +533,19 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
             }
         }
         cluster_sync(size);
-        unsigned count[2] = {0, 0};
-        u64 mass[2] = {0, 0};
+        unsigned count = 0;
+        u64 sum = 0;
         for (unsigned r = 0; r < size; ++r) {
-            const u64 c = peer_load1(peer_addr(shared_addr(&lv.count[2 * t]), r));
-            count[0] += (unsigned)c, count[1] += (unsigned)(c >> 32);
-            if (by_entry) {
-                const uint4 a = peer_load(peer_addr(shared_addr(&lv.mass[2 * t]), r));
-                mass[0] += (u64)a.y << 32 | a.x, mass[1] += (u64)a.w << 32 | a.z;
-            }
+            count += peer_load32(peer_addr(shared_addr(&lv.count[t]), r));
+            if (by_entry) sum += peer_load1(peer_addr(shared_addr(&lv.mass[t]), r));
         }
         /* the one key of a bin once a bin is one key: keys of 16-bit types end in zeros above zero and in ones below */
         auto key_at = [&](unsigned bin) {
             const unsigned hi = khi - (bin << shift), low = (1u << S0) - 1u;
             return (hi & 0x80000000u) ? (hi & ~low) : ((hi + 1u) & ~low) - 1u;
         };
-        u64 sum = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (BY_MASS && !by_entry && count[i]) mass[i] = count[i] * weigh.weight(value_of(key_at(2 * t + i)));
-            if (!BY_MASS) mass[i] = count[i];
-            sum += mass[i];
-        }
+        if (BY_MASS && !by_entry && count) sum = count * weigh.weight(value_of(key_at(t)));
+        if (!BY_MASS) sum = count;
         u64 upto = warp_scan(sum);
         if (lane == 31) lv.warp_total[warp] = upto;
         __syncthreads();
@@ -563,18 +560,11 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
             target = max(1ull, (u64)ceil(fraction * (double)all));
             have_target = true;
         }
-        u64 before = upto - sum;
-        if (before < target && target <= upto) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (before < target && target <= before + mass[i]) {
-                    lv.bin = 2 * t + i;
-                    lv.bin_count = count[i];
-                    lv.before = before;
-                    lv.found = 1;
-                }
-                before += mass[i];
-            }
+        if (upto - sum < target && target <= upto) {
+            lv.bin = t;
+            lv.bin_count = count;
+            lv.before = upto - sum;
+            lv.found = 1;
         }
         cluster_sync(size); /* the result is there, and no block reads the bins any more */
         if (!lv.found) return Border{klo, 0xffffffffu, 0xffffffffu}; /* less than was asked for: all of the range */
