@@ -106,8 +106,7 @@ template <class C> __device__ void close_up(u64 *list, unsigned room, unsigned s
 /* One message of every block to all blocks of its cluster, and the barrier after it; every exchange of a launch has a
  * buffer of its own. */
 struct Told {
-    alignas(16) u64 block[3][kMaxCluster][2];
-    alignas(16) u64 warp[kMaxCluster * kWarps][2];
+    alignas(16) u64 block[4][kMaxCluster][2];
 };
 __device__ __forceinline__ void tell_all(u64 (&buffer)[kMaxCluster][2], u64 a, u64 b, unsigned rank, unsigned size) {
     if (threadIdx.x < size) peer_store(peer_addr(shared_addr(&buffer[rank][0]), threadIdx.x), a, b);
@@ -231,6 +230,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
         Level level;
     } sh;
     __shared__ u64 list[kSampleRoom];
+    __shared__ u64 warp_part[kWarps][2];
     __shared__ double table[kTable * kTableCopies];
     __shared__ u64 scratch[kWarps];
     __shared__ unsigned own;
@@ -345,42 +345,59 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
     const Weigh<sizeof(T) == 4> weigh(most, temperature, table);
     if (k == 1) bound = most;
 
-    /* the weight of the whole row, or of what min_p keeps where nothing else cuts: a warp's own in quarters, whose sums
-     * its lanes keep for the end */
-    u64 quarter[4] = {0, 0, 0, 0};
+    /* weight above a border and number of entries on it, of this thread: the weight in quarters of the warp's piece,
+     * which are kept to find the token's */
+    u64 quarter[4];
+    unsigned ties = 0;
     const int start = share.first - lane; /* of the warp's piece */
     const int per_quarter = (max(0, share.last - start) + 127) >> 7;
-    u64 total = 0;
-    const bool cut = k > 0 || top_p < 1.0f;
-    constexpr bool kBinsWeigh = Elem<T>::kShift == 16; /* counts by bin say the row's weight: a bin is one score */
-    if (k == 0 && !(cut && kBinsWeigh)) {
-        const float from = cut ? weigh.least : fmaxf(weigh.least, lowest);
+    auto pass = [&](const Border &border, bool most_count) {
+        const float above = value_of(max(border.key, key_of(-3.402823466e+38f) - 1u)), on = value_of(border.key);
+        const bool count = border.ties != 0;
+        const float from = fmaxf(weigh.least, value_of(border.key + 1u));
+        ties = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+            quarter[q] = 0;
             const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
 #pragma unroll 1
             for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
                 const uint4 w = raw(v);
                 typename Elem<T>::Max best;
                 best.add(w);
-                if (!(best.get() >= from)) continue;
+                if (!(most_count ? best.get() >= from : count ? best.get() >= on : best.get() > above)) continue;
                 float f[E];
                 Elem<T>::unpack(w, f);
+                if (most_count) { /* without a branch: the weights of a vector are computed side by side */
 #pragma unroll
-                for (int i = 0; i < E; ++i) { /* no branch: the weights of a vector are computed side by side */
-                    const u64 x = weigh.of(f[i]);
-                    quarter[q] += f[i] >= from ? x : 0;
+                    for (int i = 0; i < E; ++i) {
+                        const u64 x = weigh.of(f[i]);
+                        quarter[q] += f[i] >= from ? x : 0;
+                    }
+                    continue;
+                }
+                quarter[q] += weigh.template some<E>(f, [&](float x) { return x > above; });
+                if (count) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) ties += f[i] == on;
                 }
             }
         }
-    }
-    Border border{key_of(cut ? neg_inf() : fmaxf(lowest, -3.402823466e+38f)) - (cut ? 0u : 1u), 0, 0};
+    };
+    u64 total = 0;
+    const bool cut = k > 0 || top_p < 1.0f;
+    BlockPart part{0, 0, false};
+    bool passed = false;
+    Border border{key_of(cut ? -3.402823466e+38f : lowest) - 1u, 0, 0}; /* without cuts: of min_p */
     if (cut) {
         float least = fmaxf(bound, -3.402823466e+38f);
         bool listed = k > 0 && k <= kListed;
         if (k == 0) { /* top_p alone */
             least = weigh.least;
-            if (!kBinsWeigh) { /* entries so far down that all of them together weigh less than what is cut off */
+            /* counts by bin say what a row of bfloat16 weighs; else, or where min_p leaves few to list, a pass does, and
+             * how far down entries lie that all of them together weigh less than what is cut off */
+            if (Elem<T>::kShift != 16 || min_p > 0.0f) {
+                pass(border, true);
                 const u64 block_total = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
                 tell_all(told.block[1], block_total, 0, rank, size);
                 for (int i = 0; i < (int)size; ++i) total += told.block[1][i][0];
@@ -390,8 +407,10 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
                 listed = true;
             }
         }
+        /* what min_p drops is not needed to weigh the rest, unless top_p takes its share of what top_k keeps */
+        const float above = k == 0 || !(top_p < 1.0f) ? fmaxf(least, lowest) : least;
         if (listed) {
-            const unsigned n = gather(share, raw, thread_most, least, sh.mine, list, kSampleRoom, own, rank, size, finisher);
+            const unsigned n = gather(share, raw, thread_most, above, sh.mine, list, kSampleRoom, own, rank, size, finisher);
             tell_all(told.block[2], n, 0, rank, size);
             unsigned longest = 0;
             for (int i = 0; i < (int)size; ++i) longest = max(longest, (unsigned)told.block[2][i][0]);
@@ -413,67 +432,54 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) sample
         }
         /* too many for a list */
         border = k == 1 ? Border{key_of(most), 1, 1}
-                        : border_by_bins<T, R>(share, get, sh.bins, sh.level, size, weigh, least, most, (u64)k,
-                                               top_p < 1.0f ? (top_p > 0.0f ? (double)top_p : 0.0) : 1.0, total);
+                        : border_by_bins<T, R>(share, raw, get, sh.bins, sh.level, size, weigh, k > 0 ? least : weigh.least, most, (u64)k,
+                                               top_p < 1.0f ? (top_p > 0.0f ? (double)top_p : 0.0) : 1.0, total, part);
         const unsigned below = key_of(lowest) - 1u;
-        if (below >= border.key) border = Border{below, 0, 0};
+        if (below >= border.key) border = Border{below, 0, 0}, part.known = false;
     }
 
-    /* weight above the border and number of entries on it, by warp; every warp then knows what precedes it */
-    unsigned ties = 0;
-    if (cut) {
-        const unsigned from = max(border.key, key_of(weigh.least) - 1u); /* keys above it have weight */
-        const float lowest_kept = border.ties ? value_of(border.key) : value_of(from + 1u);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            quarter[q] = 0;
-            const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
-#pragma unroll 1
-            for (int v = share.first + 32 * per_quarter * q; v < end; v += 32) {
-                const uint4 w = raw(v);
-                typename Elem<T>::Max best;
-                best.add(w);
-                if (!(best.get() >= lowest_kept)) continue;
-                float f[E];
-                Elem<T>::unpack(w, f);
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const unsigned key = key_of(not_nan(f[i]));
-                    const u64 x = weigh.of(f[i]);
-                    quarter[q] += key > from ? x : 0;
-                    ties += key == border.key;
-                }
-            }
-        }
-        ties = warp_sum(ties);
+    /* what every block holds of what is kept; the token lies in the one that its random number points to */
+    if (!part.known) {
+        pass(border, !cut);
+        passed = true;
+        part.mass = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
+        part.ties = border.ties ? (unsigned)block_sum(ties, scratch) : 0;
     }
-    const u64 mass = warp_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]));
-    if (lane < (int)size) peer_store(peer_addr(shared_addr(&told.warp[rank * kWarps + warp][0]), lane), mass, ties);
-    cluster_sync(size);
+    tell_all(told.block[3], part.mass, part.ties, rank, size);
     const u64 tie_weight = border.ties ? weigh.weight(value_of(border.key)) : 0;
-    const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
-    u64 before = 0;
-    total = 0;
+    u64 before = 0, here = 0;
     unsigned ties_seen = 0, quota = 0;
-    for (int i0 = 0; i0 < nwarps; i0 += 32) {
-        const int i = i0 + lane;
-        const u64 m = i < nwarps ? told.warp[i][0] : 0;
-        const unsigned n = i < nwarps ? (unsigned)told.warp[i][1] : 0;
-        const unsigned upto = ties_seen + warp_scan(n);
-        const unsigned kept = min(upto, border.ties) - min(upto - n, border.ties);
-        const u64 w = m + kept * tie_weight;
-        const u64 sum = total + warp_scan(w);
-        if (i == self) before = sum - w, quota = kept;
-        total = __shfl_sync(~0u, sum, 31);
-        ties_seen = __shfl_sync(~0u, upto, 31);
+    total = 0;
+    for (int i = 0; i < (int)size; ++i) {
+        const unsigned n = (unsigned)told.block[3][i][1], kept = min(ties_seen + n, border.ties) - min(ties_seen, border.ties);
+        const u64 w = told.block[3][i][0] + kept * tie_weight;
+        if (i == (int)rank) before = total, here = w, quota = kept;
+        total += w, ties_seen += n;
     }
-    before = __shfl_sync(~0u, before, self & 31);
-    quota = __shfl_sync(~0u, quota, self & 31);
-    const u64 here = mass + quota * tie_weight;
     /* the first entry whose running sum exceeds uniform * total */
     const u64 target = drawn(uniform, total);
     if (!more) draw();
-    if (!(before <= target && target < before + here)) {
+    if (!(before <= target && target < before + here)) { /* in another block */
+        next();
+        continue;
+    }
+    if (!passed) pass(border, false);
+    {
+        const u64 mass = warp_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]));
+        const unsigned n = warp_sum(ties);
+        if (lane == 0) warp_part[warp][0] = mass, warp_part[warp][1] = n;
+        __syncthreads();
+        unsigned seen = 0, block_quota = quota;
+        for (int w = 0; w <= warp; ++w) {
+            const unsigned m = (unsigned)warp_part[w][1];
+            quota = min(seen + m, block_quota) - min(seen, block_quota);
+            here = warp_part[w][0] + quota * tie_weight;
+            if (w < warp) before += here;
+            seen += m;
+        }
+        __syncthreads();
+    }
+    if (!(before <= target && target < before + here)) { /* in another warp's piece */
         next();
         continue;
     }
@@ -554,6 +560,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
     __shared__ Told told_by_turns[2];
     __shared__ u64 scratch[kWarps];
     __shared__ unsigned own, taken, counts[kMaxCluster];
+    __shared__ u64 ties_of[kMaxCluster * kWarps]; /* entries on the border, by warp */
     __shared__ Extent extent;
     const unsigned size = cluster_size(), rank = cluster_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -641,13 +648,13 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
             for (int i = 0; i < E; ++i) ties += key_of(f[i]) == border.key;
         }
         ties = warp_sum(ties);
-        if (lane < (int)size) peer_store(peer_addr(shared_addr(&told.warp[rank * kWarps + warp][0]), lane), ties, 0);
+        if (lane < (int)size) peer_store1(peer_addr(shared_addr(&ties_of[rank * kWarps + warp]), lane), ties);
         cluster_sync(size);
         unsigned quota = 0, seen = 0;
         const int nwarps = (int)size * kWarps, self = (int)rank * kWarps + warp;
         for (int i0 = 0; i0 < nwarps; i0 += 32) {
             const int i = i0 + lane;
-            const unsigned m = i < nwarps ? (unsigned)told.warp[i][0] : 0;
+            const unsigned m = i < nwarps ? (unsigned)ties_of[i] : 0;
             const unsigned upto = seen + warp_scan(m);
             if (i == self) quota = min(upto, border.ties) - min(upto - m, border.ties);
             seen = __shfl_sync(~0u, upto, 31);

@@ -201,7 +201,7 @@ __device__ __forceinline__ unsigned peer_addr(unsigned addr, unsigned rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void peer_store(unsigned addr, u64 a, u64 b) {
+__device__ __forceinline__ void peer_store(unsigned addr, u64 a, u64 b) { /* 16-byte aligned */
     asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(addr), "l"(a), "l"(b) : "memory");
 }
 __device__ __forceinline__ void peer_store1(unsigned addr, u64 a) {
@@ -394,6 +394,30 @@ template <bool WIDE> struct Weigh {
         return (u64)__double_as_longlong(m) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 weight(float f) const { return f >= least ? of(f) : 0; }
+    /* The weight of those of a vector's scores (none below `least`) that `wanted` takes: one after the other where they
+     * are few; else all of them side by side, without a branch, which hides the latency of the 64-bit operations. */
+    template <int E, class F> __device__ __forceinline__ u64 some(const float (&f)[E], F wanted) const {
+        unsigned found = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) found |= (unsigned)(wanted(f[i]) && f[i] >= least) << i;
+        u64 sum = 0;
+        if (__popc(found) > 2) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const u64 w = of(f[i]);
+                sum += (found >> i) & 1u ? w : 0;
+            }
+        } else {
+            for (; found; found &= found - 1) {
+                float x = f[0];
+#pragma unroll
+                for (int i = 1; i < E; ++i)
+                    if ((found >> i) & 1u && !(found & ((1u << i) - 1u))) x = f[i];
+                sum += of(x);
+            }
+        }
+        return sum;
+    }
 };
 
 /* ------------------------------------------------------ candidate lists */
@@ -592,25 +616,34 @@ __device__ Border find_border(const Share<T, RESIDENT> &share, Get get, Level &l
  * magnitude and below, would be most of the keys and hold next to no entries: they share the middle bin.  Keys below
  * minus the largest magnitude share the last.  The weights of these two are added up entry by entry. */
 constexpr int kFineBins = 12 * kThreads; /* 11 octaves of 128 keys on either side of zero, the two shared bins: 2818 */
+constexpr int kNear = 512;
 struct FineBins {
-    alignas(16) unsigned count[kFineBins];
+    alignas(16) unsigned count[kFineBins]; /* of this block */
+    float near[kNear];                     /* scores of its shared bins, if they are so few */
+    unsigned n_near;
     u64 warp[kWarps];
-    u64 shared[kMaxCluster][2];   /* weights of the middle bin and the last, by block */
+    alignas(16) u64 shared[kMaxCluster][2]; /* weights of the middle bin and the last, by block */
     u64 total[2][kMaxCluster];    /* of the blocks' slices; by search */
-    u64 found[2][2];              /* what precedes the bin that was looked for; its count << 32 | bin, or ~0 */
+    alignas(16) u64 found[2][2];  /* what precedes the bin that was looked for; its count << 32 | bin, or ~0 */
 };
 
 /* The order of bins: 0 for the largest scores. */
 struct BinOrder {
     unsigned high, low, far, gap, top; /* leading bits of the smallest key above the middle bin, the largest below, the
                                           largest of the last bin; keys left out; squeezed key of the maximum */
+    float zero, end;                   /* scores between -zero and zero are in the middle, -end and below in the last */
+    int middle, last;                  /* the shared bins; middle may lie beyond the maximum, below 0 */
     __device__ __forceinline__ BinOrder(float most, float from) {
         const float reach = fmaxf(fabsf(most), fminf(fabsf(from), fmaxf(2.0f * fabsf(most), 64.0f)));
         const int e = (int)(__float_as_uint(reach) >> 23); /* biased exponent of the largest magnitude */
         const float z = __uint_as_float((unsigned)max(1, e - 10) << 23), m = __uint_as_float((unsigned)min(254, e + 1) << 23);
         high = key_of(z) >> 16, low = key_of(-z) >> 16, far = key_of(-m) >> 16, gap = high - low - 2;
         top = squeeze(key_of(most) >> 16);
+        zero = z, end = m;
+        middle = (int)(top - (low + 1)), last = (int)(top - far);
     }
+    __device__ __forceinline__ int of(float f) const { return (int)bin((__float_as_uint(f) >> 16) ^ ((unsigned)((int)__float_as_uint(f) >> 31) >> 16 | 0x8000u)); }
+    __device__ __forceinline__ bool shared(float f) const { return fabsf(f) < zero || f <= -end; }
     __device__ __forceinline__ unsigned squeeze(unsigned k) const { return k >= high ? k - gap : k > low ? low + 1 : max(k, far); }
     __device__ __forceinline__ unsigned bin(unsigned k) const { return top - squeeze(k); }
     /* the bin's keys, leading bits */
@@ -624,82 +657,134 @@ struct BinOrder {
     }
 };
 
+/* Counts this block's entries that are not below `from`; returns its weights of the two shared bins.  All threads of the
+ * block call it; barriers follow its writes. */
+template <class T, bool RESIDENT, class Raw>
+__device__ void count_bins(const Share<T, RESIDENT> &share, Raw raw, FineBins &bins, const BinOrder &order, const Weigh<sizeof(T) == 4> &weigh, float from,
+                           u64 (&coarse)[2]) {
+    constexpr int E = Elem<T>::E;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+#pragma unroll
+    for (int i = 0; i < kFineBins / kThreads / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
+    if (t < 2) bins.found[t][1] = ~0ull;
+    if (t == 0) bins.n_near = 0;
+    __syncthreads();
+    for (int v = share.first; v < share.last; v += 32) {
+        const uint4 w = raw(v);
+        typename Elem<T>::Max best;
+        best.add(w);
+        if (!(best.get() >= from)) continue;
+        float f[E];
+        Elem<T>::unpack(w, f);
+        unsigned near = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const bool in = f[i] >= from;
+            if (in) atomicAdd(&bins.count[order.of(f[i])], 1u);
+            near |= (unsigned)(in && order.shared(f[i])) << i;
+        }
+        if (near) {
+            unsigned at = atomicAdd(&bins.n_near, __popc(near));
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (((near >> i) & 1u) && at < kNear) bins.near[at++] = f[i];
+        }
+    }
+    __syncthreads();
+    coarse[0] = coarse[1] = 0;
+    const int n = (int)bins.n_near;
+    if (n == 0) return; /* the same in all threads */
+    if (n <= kNear) {
+        for (int i = t; i < n; i += kThreads) coarse[bins.near[i] <= -order.end] += weigh.weight(bins.near[i]);
+    } else {
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            Elem<T>::unpack(raw(v), f);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const u64 w = f[i] >= from && order.shared(f[i]) ? weigh.weight(f[i]) : 0;
+                coarse[0] += f[i] <= -order.end ? 0 : w, coarse[1] += f[i] <= -order.end ? w : 0;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const u64 w = warp_sum(coarse[i]);
+        if (lane == 0) bins.warp[warp] = w;
+        __syncthreads();
+        coarse[i] = 0;
+#pragma unroll
+        for (int j = 0; j < kWarps; ++j) coarse[i] += bins.warp[j];
+        __syncthreads();
+    }
+}
+
+/* the weight of n entries of a bin that is not shared: of its highest or its lowest score, which are one for a bfloat16
+ * (whose key ends in zeros above zero and in ones below) */
+template <bool EXACT> __device__ __forceinline__ unsigned key_of_bin(const BinOrder &order, int bin, bool high) {
+    return high || (EXACT && order.highest(bin) < 0x8000u) ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16;
+}
+
+/* The weight of this block's counted entries in the bins before `end`, by all threads; two barriers. */
+template <bool WIDE> __device__ u64 weight_before(FineBins &bins, const BinOrder &order, const Weigh<WIDE> &weigh, const u64 (&coarse)[2], int end) {
+    u64 mine = 0;
+#pragma unroll 1
+    for (int bin = threadIdx.x; bin < min(end, kFineBins); bin += kThreads) {
+        const unsigned n = bins.count[bin];
+        if (n && bin != order.middle && bin != order.last) mine += n * weigh.weight(value_of(key_of_bin<true>(order, bin, false)));
+    }
+    if (threadIdx.x == 0) mine += (order.middle < end ? coarse[0] : 0) + (order.last < end ? coarse[1] : 0);
+    mine = warp_sum(mine);
+    if ((threadIdx.x & 31) == 0) bins.warp[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all += bins.warp[w];
+    __syncthreads();
+    return all;
+}
+
+/* What a block holds of the entries that are kept, where the bins say so. */
+struct BlockPart {
+    u64 mass;      /* above the border */
+    unsigned ties; /* on it */
+    bool known;
+};
+
 /* The border of the entries not below `from` that top_k (0: off) and then the fraction top_p (1: off) of their weight
- * keep.  `total`: the weight of the row if it is known and k is 0, else 0.  All threads of the cluster call it with the
+ * keep.  `total`: the weight of the row, needed where k is 0 and a bin is not one key.  All threads of the cluster call it with the
  * same arguments; `lv` may lie in the place of `bins`. */
-template <class T, bool RESIDENT, class Get>
-__device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineBins &bins, Level &lv, unsigned size, const Weigh<sizeof(T) == 4> &weigh,
-                                 float from, float most, u64 k, double top_p, u64 total) {
+template <class T, bool RESIDENT, class Raw, class Get>
+__device__ Border border_by_bins(const Share<T, RESIDENT> &share, Raw raw, Get get, FineBins &bins, Level &lv, unsigned size,
+                                 const Weigh<sizeof(T) == 4> &weigh, float from, float most, u64 k, double top_p, u64 total, BlockPart &part) {
     constexpr int E = Elem<T>::E;
     constexpr bool EXACT = Elem<T>::kShift == 16; /* a bin that is not shared is one key */
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const unsigned rank = cluster_rank();
     const BinOrder order(most, from);
-    const int middle = (int)(order.top - (order.low + 1)), last = (int)(order.top - order.far);
-#pragma unroll
-    for (int i = 0; i < kFineBins / kThreads / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
-    if (t < 2) bins.found[t][1] = ~0ull;
-    __syncthreads();
-    for (int v = share.first; v < share.last; v += 32) {
-        float f[E];
-        get(v, f);
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (f[i] >= from) atomicAdd(&bins.count[order.bin(key_of(f[i]) >> 16)], 1u);
-    }
-    __syncthreads();
-    u64 coarse[2] = {0, 0};
-    if ((middle >= 0 && bins.count[middle]) || bins.count[last]) {
-        for (int v = share.first; v < share.last; v += 32) {
-            float f[E];
-            get(v, f);
-#pragma unroll 1
-            for (int i = 0; i < E; ++i) {
-                float x = f[0];
-#pragma unroll
-                for (int j = 1; j < E; ++j)
-                    if (i == j) x = f[j];
-                const int bin = x >= from ? (int)order.bin(key_of(x) >> 16) : -1;
-                if (bin == last || (bin == middle && bin >= 0)) coarse[bin == last] += weigh.weight(x);
-            }
-        }
-    }
-    auto block_total = [&](u64 v) { /* two barriers */
-        v = warp_sum(v);
-        if (lane == 0) bins.warp[warp] = v;
-        __syncthreads();
-        u64 all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all += bins.warp[w];
-        __syncthreads();
-        return all;
-    };
-    coarse[0] = block_total(coarse[0]), coarse[1] = block_total(coarse[1]);
-    if (t < (int)size) peer_store(peer_addr(shared_addr(&bins.shared[rank][0]), t), coarse[0], coarse[1]);
+    u64 coarse[2], own_coarse[2];
+    count_bins(share, raw, bins, order, weigh, from, own_coarse);
+    if (t < (int)size) peer_store(peer_addr(shared_addr(&bins.shared[rank][0]), t), own_coarse[0], own_coarse[1]);
     cluster_sync(size);
-    /* every block adds up a slice of the bins, and puts the sums in place of its own counts, which nobody else reads */
+    coarse[0] = coarse[1] = 0;
+    for (unsigned r = 0; r < size; ++r) coarse[0] += bins.shared[r][0], coarse[1] += bins.shared[r][1];
+    /* every block adds up a slice of the bins of all */
     const int slice = kFineBins / (int)size, per = (slice + kThreads - 1) / kThreads;
     const int bin0 = (int)rank * slice + min(slice, t * per), bin1 = (int)rank * slice + min(slice, t * per + per);
-#pragma unroll 4
-    for (int bin = bin0; bin < bin1; ++bin) {
+    const int middle = order.middle, last = order.last;
+    auto counted = [&](int bin) -> u64 {
         const unsigned at = shared_addr(&bins.count[bin]);
         unsigned n = 0;
 #pragma unroll
         for (unsigned r = 0; r < kMaxCluster; ++r)
             if (r < size) n += peer_load32(peer_addr(at, r));
-        bins.count[bin] = n;
-    }
-    coarse[0] = coarse[1] = 0;
-    for (unsigned r = 0; r < size; ++r) coarse[0] += bins.shared[r][0], coarse[1] += bins.shared[r][1];
-
-    auto counted = [&](int bin) -> u64 { return bins.count[bin]; };
+        return n;
+    };
     auto weighed = [&](int bin, bool high) -> u64 {
         if (bin == middle) return coarse[0];
         if (bin == last) return coarse[1];
-        const unsigned n = bins.count[bin];
-        /* the key of a bfloat16 ends in zeros above zero and in ones below */
-        const unsigned key = high || (EXACT && order.highest(bin) < 0x8000u) ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16;
-        return n ? n * weigh.weight(value_of(key)) : 0;
+        const u64 n = counted(bin);
+        return n ? n * weigh.weight(value_of(key_of_bin<EXACT>(order, bin, high))) : 0;
     };
     /* the first bin up to which the sum of `of` reaches what `goal` makes of the whole sum, or -1; what precedes it.
      * Search 0 and 1 of a call. */
@@ -749,7 +834,7 @@ __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineB
             if (!(top_p < 1.0)) return Border{key_of(neg_inf()), 0, 0};
             return find_border<T, RESIDENT, true>(share, get, lv, size, key_of(from), key_of(most), 0, weigh, top_p, 0);
         }
-        Border border{EXACT && order.highest(bin) < 0x8000u ? order.highest(bin) << 16 | 0xffffu : order.lowest(bin) << 16, (unsigned)(k - before), equals};
+        Border border{key_of_bin<EXACT>(order, bin, false), (unsigned)(k - before), equals};
         if (!EXACT || bin == middle || bin == last)
             border = find_border<T, RESIDENT, false>(share, get, lv, size, order.lowest(bin) << 16, order.highest(bin) << 16 | 0xffffu, k - before, weigh, 0.0, 0);
         if (!(top_p < 1.0)) return border;
@@ -761,8 +846,10 @@ __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineB
     auto goal = [&](u64 all) { return target = max(1ull, (u64)ceil(top_p * (double)(EXACT ? all : total))); };
     int to = find(0, [&](int bin) { return weighed(bin, false); }, goal), first = to;
     if (EXACT && to >= 0 && to != middle && to != last) {
-        const unsigned key = order.highest(to) < 0x8000u ? order.highest(to) << 16 | 0xffffu : order.lowest(to) << 16;
+        const unsigned key = key_of_bin<EXACT>(order, to, false);
         const u64 w = weigh.weight(value_of(key));
+        part.mass = weight_before(bins, order, weigh, own_coarse, to), part.ties = bins.count[to], part.known = true;
+        __syncthreads();
         return Border{key, (unsigned)min((target - before + w - 1) / w, (u64)equals), equals};
     }
     if (!EXACT) first = find(1, [&](int bin) { return weighed(bin, true); }, goal);
@@ -770,14 +857,22 @@ __device__ Border border_by_bins(const Share<T, RESIDENT> &share, Get get, FineB
     const unsigned khi = first < 0 ? key_of(most) : order.highest(first) << 16 | 0xffffu;
     if (!EXACT) { /* what lies above the first bin that may hold the border */
         u64 more = 0;
+        const float above = value_of(khi);
         for (int v = share.first; v < share.last; v += 32) {
+            const uint4 w = raw(v);
+            typename Elem<T>::Max best;
+            best.add(w);
+            if (!(best.get() > above)) continue;
             float f[E];
-            get(v, f);
-#pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (key_of(f[i]) > khi) more += weigh.weight(f[i]);
+            Elem<T>::unpack(w, f);
+            more += weigh.template some<E>(f, [&](float x) { return x > above; });
         }
-        more = block_total(more);
+        more = warp_sum(more);
+        if (lane == 0) bins.warp[warp] = more;
+        __syncthreads();
+        more = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) more += bins.warp[w];
         if (t < (int)size) peer_store1(peer_addr(shared_addr(&bins.shared[rank][0]), t), more);
         cluster_sync(size);
         before = 0;
