@@ -29,7 +29,8 @@ def _newest(paths):
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
     srcs = sorted(glob.glob(os.path.join(CSRC, "runtime", "*.cc")) + glob.glob(os.path.join(CSRC, "runtime", "*.cu")))
-    deps = srcs + glob.glob(os.path.join(CSRC, "runtime", "*.h")) + glob.glob(os.path.join(CSRC, "cubits", "*")) + [
+    deps = srcs + glob.glob(os.path.join(CSRC, "runtime", "*.h")) + glob.glob(os.path.join(CSRC, "runtime", "*.cuh")) + \
+        glob.glob(os.path.join(CSRC, "cubits", "*")) + [
         os.path.join(HERE, "..", "include", "accb200.h")]
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _newest(deps):
         return LIB

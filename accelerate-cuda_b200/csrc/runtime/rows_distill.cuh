@@ -1,0 +1,312 @@
+/*
+ * rows_distill.cuh -- the divergence of every row from a teacher's best entries, and its gradient (accb_distill_rows,
+ * accb_distill_rows_backward).
+ */
+#pragma once
+#include "rows.cuh"
+
+namespace accb_rows {
+
+struct DistillParams {
+    RowsIn in;
+    const void *teacher; /* rows x k, element type teacher_type */
+    const int *index;
+    const float *teacher_lse, *weight, *upstream;
+    float *loss, *stats; /* stats: rows x 4, see accb_distill_rows */
+    void *grad;          /* element type of the scores */
+    long long grad_pitch;
+    double temperature;
+    int k, teacher_type;
+    int map_words; /* 32-bit words of the map of named entries of a block's share */
+};
+
+__device__ __forceinline__ float teacher_value(const DistillParams &p, long long i) {
+    if (p.teacher_type == ACCB_ROWS_F32) return static_cast<const float *>(p.teacher)[i];
+    if (p.teacher_type == ACCB_ROWS_F16) return __half2float(static_cast<const __half *>(p.teacher)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p.teacher)[i]);
+}
+
+/* What a block keeps of an entry that the teacher names.  Probabilities are 64-bit: what they leave of 1 is the
+ * difference of like numbers. */
+struct Named {
+    double p;
+    float score; /* of the teacher */
+    float z;     /* of the student, if the entry lies in this block's share */
+    int at;      /* index, or -1 for an entry that names nothing or lies in another share */
+    int first;   /* the first of its index that was met */
+};
+
+/* The row as all its blocks know it. */
+struct RowSums {
+    float top, others_top;         /* maximum of the row, and of the entries not named (-inf: none) */
+    double sum, others_sum, cross; /* sums of exponentials below those maxima; sum of p (teacher's - student's score) / tau */
+};
+
+/* What the loss is computed from, by one warp of the row: its logarithms are taken by four lanes at once. */
+__device__ __noinline__ float row_loss(const RowSums &all, double named, double teacher_sum, double rest, double inv) {
+    const int lane = threadIdx.x & 31;
+    const double of = lane == 0 ? all.sum : lane == 1 ? teacher_sum : lane == 2 ? rest : all.others_sum;
+    const double l = lane < 4 ? log_64(of) : 0.0;
+    const double log_sum = __shfl_sync(~0u, l, 0), log_teacher = __shfl_sync(~0u, l, 1), log_rest = __shfl_sync(~0u, l, 2),
+                 log_others = __shfl_sync(~0u, l, 3);
+    const double lse = (double)all.top * inv + log_sum;
+    double loss = all.cross + named * (lse - log_teacher);
+    if (rest > 0.0) loss += rest * (log_rest - ((double)all.others_top * inv + log_others - lse));
+    return (float)loss;
+}
+
+/* BACKWARD: the statistics are given, and no block needs the others. */
+template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const __grid_constant__ DistillParams p) {
+    constexpr int E = Elem<T>::E;
+    extern __shared__ uint4 dynamic[];
+    __shared__ double scratch[kWarps];
+    __shared__ float warp_top[kWarps];
+    __shared__ alignas(16) u64 told[kMaxCluster * kWarps][4];
+    __shared__ int twice;
+    Named *named = reinterpret_cast<Named *>(dynamic);
+    unsigned *map = reinterpret_cast<unsigned *>(named + p.k);
+    uint4 *stage = dynamic + (p.map_words * 4 + p.k * sizeof(Named) + 15) / 16;
+    const unsigned size = cluster_size(), rank = cluster_rank();
+    const long long row = blockIdx.x / size;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    Share<T, R> share;
+    share.init(static_cast<const T *>(p.in.x) + row * p.in.pitch, p.in.cols, rank, size, stage);
+    T *grad = p.grad ? static_cast<T *>(p.grad) + row * p.grad_pitch : nullptr;
+    const bool same = ((reinterpret_cast<unsigned long long>(grad) ^ reinterpret_cast<unsigned long long>(share.base + share.lead)) & 15u) == 0;
+    const float weight = p.weight ? p.weight[row] : 1.0f;
+    float top = 0.0f, inverse = 0.0f, at_named = 0.0f, elsewhere = 0.0f;
+    bool live = weight != 0.0f;
+    if (BACKWARD) {
+        const float *st = p.stats + row * 4;
+        top = st[0], inverse = st[1], at_named = st[2], elsewhere = st[3];
+        live = live && inverse != 0.0f;
+    }
+    if (!BACKWARD && size > 1) cluster_arrive(); /* every block of the row has started: waited for before the first message */
+    const bool rest = p.teacher_lse != nullptr;
+    const double inv = 1.0 / p.temperature;
+    double shift = 0.0, total = 0.0, named_p = 0.0;
+    float teacher_top = neg_inf();
+    if (live) {
+        /* the first entries are asked for before the copies of the row fill the queues */
+        int index = -1;
+        float score = neg_inf();
+        if ((int)threadIdx.x < p.k) index = p.index[row * p.k + threadIdx.x], score = teacher_value(p, row * p.k + threadIdx.x);
+        if (rest) shift = p.teacher_lse[row];
+        share.fetch();
+        for (int i = threadIdx.x; i < p.map_words; i += kThreads) map[i] = 0;
+        if (threadIdx.x == 0) twice = 0;
+        for (int j = threadIdx.x; j < p.k; j += kThreads) {
+            if (j >= kThreads) index = p.index[row * p.k + j], score = teacher_value(p, row * p.k + j);
+            const bool names = index >= 0 && index < p.in.cols && score > neg_inf();
+            named[j].at = names ? index : -1;
+            named[j].score = score;
+            if (names) teacher_top = fmaxf(teacher_top, score);
+        }
+        teacher_top = warp_max(teacher_top);
+        if (lane == 0) warp_top[warp] = teacher_top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) teacher_top = fmaxf(teacher_top, warp_top[w]);
+        live = teacher_top > neg_inf();
+    }
+    /* rows that do not count: nothing of the scores is looked at */
+    auto nothing = [&] {
+        share.wait();
+        if (grad)
+            for (int v = share.first; v < share.last; v += 32) put(share, grad, same, v, make_uint4(0, 0, 0, 0));
+        if (!BACKWARD && rank == 0 && threadIdx.x < 4) {
+            if (threadIdx.x == 0) p.loss[row] = 0.0f;
+            if (p.stats) p.stats[row * 4 + threadIdx.x] = 0.0f;
+        }
+    };
+    if (!live) {
+        if (!BACKWARD && size > 1) cluster_wait();
+        nothing();
+        return;
+    }
+
+    /* the teacher's probabilities: exp(score / tau - shift), over their sum unless that is given with teacher_lse */
+    if (!rest) shift = (double)teacher_top * inv;
+    double sum_p = 0.0;
+    for (int j = threadIdx.x; j < p.k; j += kThreads) {
+        const double e = named[j].at >= 0 ? exp_64((double)named[j].score * inv - shift) : 0.0;
+        named[j].p = e;
+        sum_p += e;
+    }
+    if (warp * 32 < p.k) sum_p = warp_sum(sum_p);
+    if (lane == 0) scratch[warp] = sum_p;
+    share.wait();
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += scratch[w];
+    const double norm = rest ? 1.0 : 1.0 / total;
+    named_p = total * norm;
+
+    /* which entries of the share the teacher names; an entry named twice is counted once */
+    const int origin = share.entry(share.v0), width = (share.v1 - share.v0) * E;
+    const float c = (float)(1.4426950408889634 / p.temperature);
+    float most_named = neg_inf();
+    double cross = 0.0;
+    for (int j = threadIdx.x; j < p.k; j += kThreads) {
+        Named &n = named[j];
+        const int at = n.at, e = at - origin;
+        const bool here = at >= 0 && e >= 0 && e < width;
+        const double prob = n.p * norm;
+        n.first = 0;
+        if (here) {
+            n.first = !((atomicOr(&map[e >> 5], 1u << (e & 31)) >> (e & 31)) & 1u);
+            if (!n.first) twice = 1;
+            n.z = R ? Elem<T>::up(reinterpret_cast<const T *>(stage)[e]) : Elem<T>::up(share.base[share.lead + at]);
+            if (n.first) most_named = fmaxf(most_named, n.z);
+            /* sum of p (log p - z / tau): what is left of the loss is the two log-sum-exps */
+            if (prob > 0.0) cross += prob * (((double)n.score - (double)n.z) * inv);
+        }
+        n.p = prob;
+        n.at = here ? at : -1;
+    }
+    __syncthreads();
+
+    if (!BACKWARD) {
+        /* the rest of the row (all of it without teacher_lse) and the named entries, each as maximum and sum */
+        if (R && rest) { /* named entries leave the staged row */
+            for (int j = threadIdx.x; j < p.k; j += kThreads)
+                if (named[j].first) reinterpret_cast<T *>(stage)[named[j].at - origin] = Elem<T>::down(neg_inf());
+            __syncthreads();
+        }
+        auto get = [&](int v) {
+            uint4 w = share.get(v);
+            if (!R && rest) {
+                const int e = (v - share.v0) * E;
+                const unsigned m = map[e >> 5] >> (e & 31);
+                float f[E];
+                Elem<T>::unpack(w, f);
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if ((m >> i) & 1u) f[i] = neg_inf();
+                w = Elem<T>::pack(f);
+            }
+            return w;
+        };
+        typename Elem<T>::Max largest;
+#pragma unroll 4
+        for (int v = share.first; v < share.last; v += 32) largest.add(get(v));
+        const float most = warp_max(largest.get()), base = most > neg_inf() ? most : 0.0f;
+        const Pair less(-base, -base), by(c, c);
+        Pair part[2] = {Pair(0.0f, 0.0f), Pair(0.0f, 0.0f)};
+#pragma unroll 2
+        for (int v = share.first; v < share.last; v += 32) {
+            float f[E];
+            Elem<T>::unpack(get(v), f);
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) part[i & 1] = part[i & 1] + fast_exp2((Pair(f[2 * i], f[2 * i + 1]) + less) * by);
+        }
+        float part_a, part_b;
+        (part[0] + part[1]).get(part_a, part_b);
+        double named_sum = 0.0;
+        if (warp * 32 < p.k) {
+            if (rest) {
+                most_named = warp_max(most_named);
+                const float named_base = most_named > neg_inf() ? most_named : 0.0f;
+                for (int j = threadIdx.x; j < p.k; j += kThreads)
+                    if (named[j].first) named_sum += (double)fast_exp2((named[j].z - named_base) * c);
+                named_sum = warp_sum(named_sum);
+            }
+            cross = warp_sum(cross);
+        }
+        const double others = warp_sum((double)part_a + (double)part_b);
+        if (size > 1) cluster_wait();
+        if (lane < (int)size) {
+            const unsigned to = peer_addr(shared_addr(&told[rank * kWarps + warp][0]), lane);
+            peer_store(to, __double_as_longlong(others), __double_as_longlong(named_sum));
+            peer_store(to + 16, __double_as_longlong(cross), (u64)__float_as_uint(most) << 32 | __float_as_uint(rest ? most_named : neg_inf()));
+        }
+        cluster_sync(size);
+        if (!grad && rank != 0) return;
+        /* every warp adds up what all warps of the row found */
+        const int n = (int)size * kWarps;
+        RowSums all{neg_inf(), neg_inf(), 0.0, 0.0, 0.0};
+        for (int i = lane; i < n; i += 32) {
+            all.others_top = fmaxf(all.others_top, __uint_as_float((unsigned)(told[i][3] >> 32)));
+            all.top = fmaxf(all.top, __uint_as_float((unsigned)told[i][3]));
+        }
+        all.others_top = warp_max(all.others_top), all.top = fmaxf(all.others_top, warp_max(all.top));
+        for (int i = lane; i < n; i += 32) {
+            /* a sum that is 0 belongs to no entry; one that is not, at a maximum of -inf, to entries that are NaN */
+            const double a = __longlong_as_double((long long)told[i][0]), b = __longlong_as_double((long long)told[i][1]);
+            const float at_a = __uint_as_float((unsigned)(told[i][3] >> 32)), at_b = __uint_as_float((unsigned)told[i][3]);
+            if (a != 0.0) all.others_sum += a * (double)fast_exp2((at_a - all.others_top) * c);
+            if (b != 0.0) all.sum += b * (double)fast_exp2((at_b - all.top) * c);
+            all.cross += __longlong_as_double((long long)told[i][2]);
+        }
+        all.others_sum = warp_sum(all.others_sum), all.sum = warp_sum(all.sum);
+        const float down = fast_exp2((all.others_top - all.top) * c); /* from one maximum to the other */
+        if (all.others_sum != 0.0) all.sum += all.others_sum * (double)down;
+        if (all.top == neg_inf() && all.sum == 0.0) { /* the student excludes every entry: the same in every block of the row */
+            nothing();
+            return;
+        }
+        top = all.top;
+        inverse = (float)(1.0 / all.sum);
+        double r = rest ? fmax(0.0, 1.0 - named_p) : 0.0;
+        if (!(all.others_top > neg_inf())) r = 0.0;
+        at_named = (float)(named_p + r);
+        /* r over the student's share of the others, which may be too small for its own exponential */
+        elsewhere = at_named;
+        if (r > 0.0) {
+            const double over = down > 0.0f ? all.sum / (all.others_sum * (double)down)
+                                            : all.sum / all.others_sum * exp_64(((double)all.top - (double)all.others_top) * inv);
+            elsewhere = (float)(named_p + r - r * over);
+        }
+        if (rank == 0 && warp == 0) {
+            all.cross = warp_sum(all.cross);
+            /* log of the teacher's sum: with teacher_lse the scores are relative to it, else to their maximum */
+            const double shifted = all.cross; /* sum of p (score - z) / tau */
+            const float loss = row_loss(RowSums{all.top, all.others_top, all.sum, all.others_sum, shifted - named_p * shift}, named_p,
+                                        rest ? 1.0 : total, r, inv);
+            if (lane == 0) {
+                p.loss[row] = weight * loss;
+                if (p.stats) {
+                    float *s = p.stats + row * 4;
+                    s[0] = top, s[1] = inverse, s[2] = at_named, s[3] = elsewhere;
+                }
+            }
+        }
+        if (!grad) return;
+    }
+
+    /* gradient: elsewhere * q everywhere, then the named entries once more with their own value */
+    float g = (float)((double)weight * inv);
+    if (BACKWARD && p.upstream) g *= p.upstream[row];
+    const float factor = g * elsewhere * inverse;
+    const Pair times(factor, factor), less(-top, -top), by(c, c);
+#pragma unroll 2
+    for (int v = share.first; v < share.last; v += 32) {
+        float f[E];
+        Elem<T>::unpack(share.get(v), f);
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i)
+            (times * fast_exp2((Pair(f[2 * i], f[2 * i + 1]) + less) * by)).get(f[2 * i], f[2 * i + 1]);
+        put(share, grad, same, v, Elem<T>::pack(f));
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.k; j += kThreads) {
+        const int at = named[j].at;
+        if (at < 0) continue;
+        double sum = named[j].p;
+        if (twice) { /* the first entry of an index in the list writes the sum of all of them, in the list's order */
+            bool earlier = false;
+            sum = 0.0;
+            for (int o = 0; o < p.k; ++o)
+                if (named[o].at == at) {
+                    if (o < j) earlier = true;
+                    sum += named[o].p;
+                }
+            if (earlier) continue;
+        }
+        const float q = inverse * fast_exp2((named[j].z - top) * c);
+        grad[at] = Elem<T>::down(g * (float)((double)at_named * q - sum));
+    }
+}
+
+}  // namespace accb_rows

@@ -269,7 +269,8 @@ ACCB_API int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_row
  *           0 and below: the first),
  *   min_p   of those, the ones whose weight is at least min_p of the best one's (0 and below: off; above 1 as 1),
  * and the row's token is the first kept index, in index order, at which the running sum of the kept weights exceeds
- * uniform times their total.  A temperature that is not above 0 takes the best entry.  `allowed` (or NULL) holds bits
+ * uniform times their total.  A temperature that is not above 0 takes the best entry, one above 1e30 counts as 1e30.
+ * `allowed` (or NULL) holds bits
  * for the entries, bit j % 32 of word j / 32 for entry j, rows every allowed_pitch words: the others are not there,
  * whatever their score; nor are -inf and NaN.  A row with no entry gives token -1.  logprob (or NULL): log of the
  * token's share of the kept weight; -inf with token -1.

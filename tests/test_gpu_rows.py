@@ -170,6 +170,27 @@ def test_sample_with_cuts(ctx, torch_cuda, rng, kind, cols, temperature, cuts):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,cols", [(1500, 700), (1200, 5003)])
+def test_sample_many_rows(ctx, torch_cuda, rng, kind, rows, cols):
+    """More rows than the GPU holds at a time, so that a cluster of blocks takes one after the other."""
+    t = torch_cuda
+    x = scores(t, rng, rows, cols, kind, cols + 3, 1)
+    x[::4] = scores(t, rng, (rows + 3) // 4, cols, kind, spread=0.05, peaks=False)
+    x[7] = -float("inf")
+    x[8, 1:] = float("nan")
+    temperature = rng.choice([0.5, 1.0, 1.0, 2.0], rows)
+    temperature[16] = 0.0
+    temperature[17] = 1e-35
+    temperature[18] = np.inf
+    check_sample(ctx, t, x, uniform=rng.random(rows), temperature=temperature)
+    check_sample(ctx, t, x, uniform=rng.random(rows), min_p=0.02)
+    top_k = np.where(np.arange(rows) % 3 == 0, 20, 0)  # rows with and without cuts side by side
+    check_sample(ctx, t, x, uniform=rng.random(rows), temperature=temperature, top_k=top_k)
+    u = np.where(np.arange(rows) % 2 == 0, 0.0, 1.0 - 2.0**-24)
+    check_sample(ctx, t, x, uniform=u, temperature=temperature)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_sample_flat_rows(ctx, torch_cuda, rng, kind):
     """Rows without a peak: every entry is near the border, and there are many ties in 16 bits."""
     x = scores(torch_cuda, rng, 8, 70001, kind, spread=0.3, peaks=False)
