@@ -438,7 +438,9 @@ template <bool WIDE> struct Weigh {
         least = fmaxf(-3.402823466e+38f, (float)((double)top - (kUnitLog2 + 2) * 0.69314718055994531 * temperature));
     }
     /* for f >= least; anything below */
-    __device__ __forceinline__ u64 of(float f) const {
+    __device__ __forceinline__ u64 of(float f) const { return (u64)__double_as_longlong(above_2_52(f)) & 0xfffffffffffffull; }
+    /* 2^52 + the weight */
+    __device__ __forceinline__ double above_2_52(float f) const {
         constexpr double l = 0.69314718055994531 / kTable;
         const double x = WIDE ? (double)f - (double)top : (double)(f - top);
         const double t = fma(x, c, kRound);
@@ -448,25 +450,24 @@ template <bool WIDE> struct Weigh {
         m = __hiloint2double(__double2hiint(m) + ((k & ~(kTable - 1)) << 14), __double2loint(m));
         const double unit = (double)(1ull << kUnitLog2);
         /* 2^52 makes a unit of 2^-43 the last bit */
-        m = fma(m, fma(fma(fma(unit * l * l * l / 6.0, r, unit * l * l / 2.0), r, unit * l), r, unit), 4503599627370496.0);
-        return (u64)__double_as_longlong(m) & 0xfffffffffffffull;
+        return fma(m, fma(fma(fma(unit * l * l * l / 6.0, r, unit * l * l / 2.0), r, unit * l), r, unit), 4503599627370496.0);
     }
     __device__ __forceinline__ u64 weight(float f) const { return f >= least ? of(f) : 0; }
     /* The weight of those of a vector's scores that are not below `from` (at least `least`): one after the other where
      * they are few; else, or where `most` are said to be, all of them side by side and without a branch, which hides the
-     * latency of the 64-bit operations. */
-    template <int E> __device__ __forceinline__ u64 some(const float (&f)[E], float from, bool most) const {
+     * latency of the 64-bit operations.  Sums of up to 512 weights are exact in a double. */
+    template <int E> __device__ __forceinline__ double some(const float (&f)[E], float from, bool most) const {
         unsigned found = 0;
         if (!most) {
 #pragma unroll
             for (int i = 0; i < E; ++i) found |= (unsigned)(f[i] >= from) << i;
         }
-        u64 sum = 0;
+        double sum = 0.0;
         if (most || __popc(found) > 2) {
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const u64 w = of(f[i]);
-                sum += f[i] >= from ? w : 0;
+                const double w = above_2_52(f[i]) - 4503599627370496.0;
+                if (f[i] >= from) sum += w;
             }
         } else {
             for (; found; found &= found - 1) {
@@ -474,7 +475,7 @@ template <bool WIDE> struct Weigh {
 #pragma unroll
                 for (int i = 1; i < E; ++i)
                     if ((found >> i) & 1u && !(found & ((1u << i) - 1u))) x = f[i];
-                sum += of(x);
+                sum += above_2_52(x) - 4503599627370496.0;
             }
         }
         return sum;

@@ -212,7 +212,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
             int v = share.first;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
-                u64 sum = 0;
+                double sum = 0.0;
                 const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
 #pragma unroll 1
                 for (; v < end; v += 32) {
@@ -228,7 +228,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
                     }
                     sum += weigh.template some<E>(f, from, most_count);
                 }
-                quarter[0] = quarter[1], quarter[1] = quarter[2], quarter[2] = quarter[3], quarter[3] = sum;
+                quarter[0] = quarter[1], quarter[1] = quarter[2], quarter[2] = quarter[3], quarter[3] = (u64)sum;
             }
         };
         u64 total = 0;

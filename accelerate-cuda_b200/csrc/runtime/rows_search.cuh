@@ -547,7 +547,7 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
             if (!(best.get() > above)) continue;
             float f[E];
             Elem<T>::unpack(w, f);
-            more += weigh.template some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), false);
+            more += (u64)weigh.template some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), false);
         }
         more = warp_sum(more);
         if (lane == 0) bins.warp[warp] = more;
