@@ -413,13 +413,15 @@ template <class V> __device__ __forceinline__ V warp_scan(V v) { /* inclusive */
  *     64 y = K + r, K whole, |r| <= 1/2;  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r)
  * with the cubic Taylor polynomial of 2^(r / 64), wrong by less than (ln 2 / 128)^4 / 24 < 2^-34.6 of itself: eight
  * 64-bit operations where the library's function takes some twenty.  The table is in shared memory sixteen times, a
- * copy for every lane of a half warp, so that no two lanes meet in a bank. */
+ * copy for every lane of a half warp, so that no two lanes meet in a bank; entry j is stored with j << 14 taken from its
+ * upper half, so that adding K << 14 there adds K >> 6 to the exponent. */
 constexpr int kUnitLog2 = 43;
 constexpr int kTable = 64;
 constexpr int kTableCopies = 16;
 
 static __device__ __noinline__ void fill_table(double *table) { /* kTable * kTableCopies; by all threads, a barrier follows */
-    const double v = exp2((double)(threadIdx.x % kTable) * (1.0 / kTable));
+    double v = exp2((double)(threadIdx.x % kTable) * (1.0 / kTable));
+    v = __hiloint2double(__double2hiint(v) - ((threadIdx.x % kTable) << 14), __double2loint(v));
     for (int i = threadIdx.x / kTable; i < kTableCopies; i += kThreads / kTable) table[(threadIdx.x % kTable) * kTableCopies + i] = v;
 }
 
@@ -447,7 +449,7 @@ template <bool WIDE> struct Weigh {
         const int k = __double2loint(t);
         const double r = fma(x, c, kRound - t);
         double m = table[(k & (kTable - 1)) * kTableCopies];
-        m = __hiloint2double(__double2hiint(m) + ((k & ~(kTable - 1)) << 14), __double2loint(m));
+        m = __hiloint2double(__double2hiint(m) + (k << 14), __double2loint(m));
         const double unit = (double)(1ull << kUnitLog2);
         /* 2^52 makes a unit of 2^-43 the last bit */
         return fma(m, fma(fma(fma(unit * l * l * l / 6.0, r, unit * l * l / 2.0), r, unit * l), r, unit), 4503599627370496.0);
