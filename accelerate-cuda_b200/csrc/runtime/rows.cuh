@@ -278,6 +278,8 @@ template <class T, bool RESIDENT> struct Share {
     int n;           /* entries of the row */
     int v0, v1;      /* this block's vectors */
     int first, last; /* this thread's: first, first + 32, ... below last */
+    int in0;
+    unsigned in; /* vectors in0 .. in0 + in - 1 of the row lie wholly inside it */
     uint4 *stage;
 
     static __host__ __device__ __forceinline__ int per_block(int cols, int size) { /* vectors of a share, at most */
@@ -294,25 +296,38 @@ template <class T, bool RESIDENT> struct Share {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         first = v0 + warp * piece + lane;
         last = min(v1, v0 + (warp + 1) * piece);
+        in0 = lead != 0;
+        in = (unsigned)max(0, (lead + cols) / E - in0);
         stage = smem;
     }
     __device__ __forceinline__ int entry(int v) const { return v * E - lead; } /* index of a vector's first entry */
-    __device__ __forceinline__ bool whole(int v) const { return entry(v) >= 0 && entry(v) + E <= n; }
+    __device__ __forceinline__ bool whole(int v) const { return (unsigned)(v - in0) < in; }
 
     __device__ __forceinline__ uint4 from_memory(int v) const {
         return whole(v) ? reinterpret_cast<const uint4 *>(base)[v] : edge<T>(base, v, lead, n);
     }
-    /* start the copies of this thread's vectors; wait() before the first get() */
+    /* start the copies of this thread's vectors; wait() before the first get().  No branch but at the edges of the row,
+     * which are at most two vectors of all threads. */
     __device__ __forceinline__ void fetch() const {
+        if (!RESIDENT) return;
+        const uint4 *from = reinterpret_cast<const uint4 *>(base) + first;
+        unsigned to = shared_addr(stage + (first - v0));
+        const unsigned i0 = (unsigned)(first - in0);
 #pragma unroll 4
-        for (int v = RESIDENT ? first : last; v < last; v += 32) {
-            if (whole(v))
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_addr(stage + (v - v0))),
-                             "l"(reinterpret_cast<const uint4 *>(base) + v)
-                             : "memory");
-            else
-                stage[v - v0] = edge<T>(base, v, lead, n);
+        for (int d = 0; d < last - first; d += 32) {
+            const int go = i0 + (unsigned)d < in;
+            asm volatile(
+                "{\n"
+                ".reg .pred p;\n"
+                "setp.ne.s32 p, %2, 0;\n"
+                "@p cp.async.cg.shared.global [%0], [%1], 16;\n"
+                "}\n" ::"r"(to + d * 16),
+                "l"(from + d), "r"(go)
+                : "memory");
         }
+        if (in0 && first == 0 && last > 0) stage[0] = edge<T>(base, 0, lead, n);
+        const int v = in0 + (int)in;
+        if (v >= first && v < last && ((v - first) & 31) == 0) stage[v - v0] = edge<T>(base, v, lead, n);
     }
     __device__ __forceinline__ void wait() const {
         if (RESIDENT) asm volatile("cp.async.wait_all;" ::: "memory");

@@ -66,17 +66,24 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
         if (most > neg_inf()) {
             if (p.lse) {
                 const float c = (float)(1.4426950408889634 / p.temperature);
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const Pair less(-most, -most), by(c, c);
+                Pair part[2] = {Pair(0.0f, 0.0f), Pair(0.0f, 0.0f)};
                 if (most < __uint_as_float(0x7f800000u)) {
 #pragma unroll 2
                     for (int v = share.first; v < share.last; v += 32) {
                         float f[E];
-                        share.floats(v, f);
+                        Elem<T>::unpack(share.raw(v), f);
 #pragma unroll
-                        for (int i = 0; i < E; ++i) part[i & 3] += fast_exp2((f[i] - most) * c);
+                        for (int i = 0; i < E / 2; ++i) {
+                            float y[2];
+                            ((Pair(f[2 * i], f[2 * i + 1]) + less) * by).get(y[0], y[1]);
+                            part[i & 1] = part[i & 1] + fast_exp2(Pair(fmaxf(y[0], -200.0f), fmaxf(y[1], -200.0f))); /* NaN: 0 */
+                        }
                     }
                 }
-                const float warp_part = warp_sum((part[0] + part[1]) + (part[2] + part[3]));
+                float part_a, part_b;
+                (part[0] + part[1]).get(part_a, part_b);
+                const float warp_part = warp_sum(part_a + part_b);
                 __syncthreads();
                 if (lane == 0) scratch[warp] = __float_as_uint(warp_part);
             }
