@@ -16,14 +16,14 @@
 namespace accb_rows {
 
 constexpr size_t kSharedMost = 192u << 10; /* dynamic shared memory a block may ask for (227 KB less what it declares) */
-constexpr long long kShareBytes = 64 << 10; /* the share of a row a block aims to hold */
+constexpr long long kShareBytes = 68 << 10; /* the share of a row that a block holds at most, if eight blocks do */
 
-/* Blocks per row: as few as hold the row in shares of 64 KB (two or three blocks of an SM then overlap one another's
- * phases), more while rows are too few to give every SM a block, as long as a share stays worth a block. */
+/* Blocks per row: as few as hold the row in shares of 68 KB, so that three blocks of an SM overlap one another's phases
+ * (fewer and larger, or more and smaller, were slower: rows of 256 KB by 3, 4, 5 blocks 597, 522, 593 us for a training
+ * step over 4096); more while rows are too few to give every SM two blocks, as long as a share stays worth a block. */
 static int cluster_for(long long rows, long long row_bytes, int sm_count) {
-    int size = 1;
-    while (size < kMaxCluster && row_bytes > kShareBytes * size) size *= 2;
-    while (size < kMaxCluster && rows * size < sm_count && row_bytes > (8 << 10) * size) size *= 2;
+    int size = (int)std::min<long long>(kMaxCluster, (row_bytes + kShareBytes - 1) / kShareBytes);
+    while (size < kMaxCluster && rows * (size + 1) <= 2 * sm_count && row_bytes > (8 << 10) * size) ++size;
     return size;
 }
 

@@ -62,6 +62,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
     __shared__ double scratch[kWarps];
     __shared__ float warp_top[kWarps];
     __shared__ alignas(16) u64 told[kMaxCluster * kWarps][4];
+    __shared__ float4 statistics;
     __shared__ int twice;
     Named *named = reinterpret_cast<Named *>(dynamic);
     unsigned *map = reinterpret_cast<unsigned *>(named + p.k);
@@ -214,7 +215,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
             }
             cross = warp_sum(cross);
         }
-        const double others = warp_sum((double)part_a + (double)part_b);
+        const double others = (double)warp_sum(part_a + part_b);
         if (size > 1) cluster_wait();
         if (lane < (int)size) {
             const unsigned to = peer_addr(shared_addr(&told[rank * kWarps + warp][0]), lane);
@@ -223,56 +224,58 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
         }
         cluster_sync(size);
         if (!grad && rank != 0) return;
-        /* every warp adds up what all warps of the row found */
-        const int n = (int)size * kWarps;
-        RowSums all{neg_inf(), neg_inf(), 0.0, 0.0, 0.0};
-        for (int i = lane; i < n; i += 32) {
-            all.others_top = fmaxf(all.others_top, __uint_as_float((unsigned)(told[i][3] >> 32)));
-            all.top = fmaxf(all.top, __uint_as_float((unsigned)told[i][3]));
-        }
-        all.others_top = warp_max(all.others_top), all.top = fmaxf(all.others_top, warp_max(all.top));
-        for (int i = lane; i < n; i += 32) {
-            /* a sum that is 0 belongs to no entry; one that is not, at a maximum of -inf, to entries that are NaN */
-            const double a = __longlong_as_double((long long)told[i][0]), b = __longlong_as_double((long long)told[i][1]);
-            const float at_a = __uint_as_float((unsigned)(told[i][3] >> 32)), at_b = __uint_as_float((unsigned)told[i][3]);
-            if (a != 0.0) all.others_sum += a * (double)fast_exp2((at_a - all.others_top) * c);
-            if (b != 0.0) all.sum += b * (double)fast_exp2((at_b - all.top) * c);
-            all.cross += __longlong_as_double((long long)told[i][2]);
-        }
-        all.others_sum = warp_sum(all.others_sum), all.sum = warp_sum(all.sum);
-        const float down = fast_exp2((all.others_top - all.top) * c); /* from one maximum to the other */
-        if (all.others_sum != 0.0) all.sum += all.others_sum * (double)down;
-        if (all.top == neg_inf() && all.sum == 0.0) { /* the student excludes every entry: the same in every block of the row */
-            nothing();
-            return;
-        }
-        top = all.top;
-        inverse = (float)(1.0 / all.sum);
-        double r = rest ? fmax(0.0, 1.0 - named_p) : 0.0;
-        if (!(all.others_top > neg_inf())) r = 0.0;
-        at_named = (float)(named_p + r);
-        /* r over the student's share of the others, which may be too small for its own exponential */
-        elsewhere = at_named;
-        if (r > 0.0) {
-            const double over = down > 0.0f ? all.sum / (all.others_sum * (double)down)
-                                            : all.sum / all.others_sum * exp_64(((double)all.top - (double)all.others_top) * inv);
-            elsewhere = (float)(named_p + r - r * over);
-        }
-        if (rank == 0 && warp == 0) {
-            all.cross = warp_sum(all.cross);
-            /* log of the teacher's sum: with teacher_lse the scores are relative to it, else to their maximum */
-            const double shifted = all.cross; /* sum of p (score - z) / tau */
-            const float loss = row_loss(RowSums{all.top, all.others_top, all.sum, all.others_sum, shifted - named_p * shift}, named_p,
-                                        rest ? 1.0 : total, r, inv);
-            if (lane == 0) {
-                p.loss[row] = weight * loss;
-                if (p.stats) {
-                    float *s = p.stats + row * 4;
-                    s[0] = top, s[1] = inverse, s[2] = at_named, s[3] = elsewhere;
+        /* one warp adds up what all warps of the row found, and says what the gradient needs */
+        if (warp == 0) {
+            const int n = (int)size * kWarps;
+            RowSums all{neg_inf(), neg_inf(), 0.0, 0.0, 0.0};
+            for (int i = lane; i < n; i += 32) {
+                all.others_top = fmaxf(all.others_top, __uint_as_float((unsigned)(told[i][3] >> 32)));
+                all.top = fmaxf(all.top, __uint_as_float((unsigned)told[i][3]));
+            }
+            all.others_top = warp_max(all.others_top);
+            all.top = rest ? fmaxf(all.others_top, warp_max(all.top)) : all.others_top;
+            for (int i = lane; i < n; i += 32) {
+                /* a sum that is 0 belongs to no entry; one that is not, at a maximum of -inf, to entries that are NaN */
+                const double a = __longlong_as_double((long long)told[i][0]), b = __longlong_as_double((long long)told[i][1]);
+                const float at_a = __uint_as_float((unsigned)(told[i][3] >> 32)), at_b = __uint_as_float((unsigned)told[i][3]);
+                if (a != 0.0) all.others_sum += a * (double)fast_exp2((at_a - all.others_top) * c);
+                if (b != 0.0) all.sum += b * (double)fast_exp2((at_b - all.top) * c);
+                all.cross += __longlong_as_double((long long)told[i][2]);
+            }
+            all.others_sum = warp_sum(all.others_sum);
+            if (rest) all.sum = warp_sum(all.sum);
+            const float down = rest ? fast_exp2((all.others_top - all.top) * c) : 1.0f; /* from one maximum to the other */
+            if (all.others_sum != 0.0) all.sum += all.others_sum * (double)down;
+            const bool excluded = all.top == neg_inf() && all.sum == 0.0; /* by the student, every entry */
+            double r = rest && all.others_top > neg_inf() ? fmax(0.0, 1.0 - named_p) : 0.0;
+            float4 said = make_float4(all.top, (float)(1.0 / all.sum), (float)(named_p + r), (float)(named_p + r));
+            if (r > 0.0) {
+                /* r over the student's share of the others, which may be too small for its own exponential */
+                double over = all.sum / all.others_sum;
+                over = down > 0.0f ? over / (double)down : over * exp_64(((double)all.top - (double)all.others_top) * inv);
+                said.w = (float)(named_p + r - r * over);
+            }
+            if (excluded) said = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (lane == 0) statistics = said;
+            if (rank == 0) {
+                all.cross = warp_sum(all.cross) - named_p * shift;
+                const float loss = excluded ? 0.0f : row_loss(all, named_p, rest ? 1.0 : total, r, inv);
+                if (lane == 0) {
+                    p.loss[row] = weight * loss;
+                    if (p.stats) {
+                        float *s = p.stats + row * 4;
+                        s[0] = said.x, s[1] = said.y, s[2] = said.z, s[3] = said.w;
+                    }
                 }
             }
         }
         if (!grad) return;
+        __syncthreads();
+        top = statistics.x, inverse = statistics.y, at_named = statistics.z, elsewhere = statistics.w;
+        if (inverse == 0.0f) { /* the same in every block of the row */
+            nothing();
+            return;
+        }
     }
 
     /* gradient: elsewhere * q everywhere, then the named entries once more with their own value */

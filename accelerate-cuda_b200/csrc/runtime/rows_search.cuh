@@ -451,8 +451,8 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
     coarse[0] = coarse[1] = 0;
     for (unsigned r = 0; r < size; ++r) coarse[0] += bins.shared[r][0], coarse[1] += bins.shared[r][1];
     /* every block adds up a slice of the bins of all */
-    const int slice = kFineBins / (int)size, per = (slice + kThreads - 1) / kThreads;
-    const int bin0 = (int)rank * slice + min(slice, t * per), bin1 = (int)rank * slice + min(slice, t * per + per);
+    const int slice = (kFineBins + (int)size - 1) / (int)size, per = (slice + kThreads - 1) / kThreads;
+    const int bin0 = min(kFineBins, (int)rank * slice + min(slice, t * per)), bin1 = min(kFineBins, (int)rank * slice + min(slice, t * per + per));
     const int middle = order.middle, last = order.last;
     auto counted = [&](int bin) -> u64 {
         const unsigned at = shared_addr(&bins.count[bin]);
