@@ -472,7 +472,8 @@ template <bool WIDE> struct Weigh {
     __device__ __forceinline__ u64 weight(float f) const { return f >= least ? of(f) : 0; }
     /* The weight of those of a vector's scores that are not below `from` (at least `least`): one after the other where
      * they are few; else, or where `most` are said to be, all of them side by side and without a branch, which hides the
-     * latency of the 64-bit operations.  Sums of up to 512 weights are exact in a double. */
+     * latency of the 64-bit operations.  Sums of up to 512 weights are exact in a double.  Unless `most`, all lanes of a
+     * warp call it together. */
     template <int E> __device__ __forceinline__ double some(const float (&f)[E], float from, bool most) const {
         unsigned found = 0;
         if (!most) {
@@ -480,7 +481,7 @@ template <bool WIDE> struct Weigh {
             for (int i = 0; i < E; ++i) found |= (unsigned)(f[i] >= from) << i;
         }
         double sum = 0.0;
-        if (most || __popc(found) > 2) {
+        if (most || __any_sync(~0u, __popc(found) > 2)) {
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const double w = above_2_52(f[i]) - 4503599627370496.0;

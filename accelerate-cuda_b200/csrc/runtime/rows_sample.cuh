@@ -209,17 +209,18 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
             const bool count = border.ties != 0;
             const float from = fmaxf(weigh.least, value_of(max(border.key, key_of(kLowest) - 1u) + 1u));
             ties = 0;
-            int v = share.first;
+            int v0 = start;
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
                 double sum = 0.0;
-                const int end = min(share.last, share.first + 32 * per_quarter * (q + 1));
+                const int end = min(share.last, start + 32 * per_quarter * (q + 1));
 #pragma unroll 1
-                for (; v < end; v += 32) {
-                    const uint4 w = share.raw(v);
+                for (; v0 < end; v0 += 32) { /* the same turns in all lanes */
+                    uint4 w = make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+                    if (v0 + lane < end) w = share.raw(v0 + lane);
                     typename Elem<T>::Max best;
                     best.add(w);
-                    if (!(count ? best.get() >= on : best.get() >= from)) continue;
+                    if (!__any_sync(~0u, count ? best.get() >= on : best.get() >= from)) continue;
                     float f[E];
                     Elem<T>::unpack(w, f);
                     if (count) {

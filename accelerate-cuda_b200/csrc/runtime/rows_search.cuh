@@ -349,6 +349,7 @@ __device__ __forceinline__ void count_bins(const Row<T, RESIDENT> &share, FineBi
     for (int i = 0; i < kFineBins / kThreads / 4; ++i) *reinterpret_cast<uint4 *>(&bins.count[4 * (t + i * kThreads)]) = make_uint4(0, 0, 0, 0);
     if (t < 2) bins.found[t][1] = ~0ull;
     if (t == 0) bins.n_near = 0;
+    const unsigned counts = shared_addr(bins.count);
     __syncthreads();
     for (int v = share.first; v < share.last; v += 32) {
         const uint4 w = share.raw(v);
@@ -357,18 +358,28 @@ __device__ __forceinline__ void count_bins(const Row<T, RESIDENT> &share, FineBi
         if (!(best.get() >= from)) continue;
         float f[E];
         Elem<T>::unpack(w, f);
-        unsigned near = 0;
+        unsigned near = 0, at[E], in[E];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const bool in = f[i] >= from;
-            if (in) atomicAdd(&bins.count[order.of(f[i])], 1u);
-            near |= (unsigned)(in && order.shared(f[i])) << i;
+            in[i] = f[i] >= from;
+            at[i] = counts + 4 * (unsigned)order.of(f[i]);
+            near |= (unsigned)(in[i] && order.shared(f[i])) << i;
         }
+#pragma unroll
+        for (int i = 0; i < E; ++i) /* no branch, which would wait for every address by itself */
+            asm volatile(
+                "{\n"
+                ".reg .pred p;\n"
+                "setp.ne.u32 p, %1, 0;\n"
+                "@p red.shared::cta.add.u32 [%0], 1;\n"
+                "}\n" ::"r"(at[i]),
+                "r"(in[i])
+                : "memory");
         if (near) {
-            unsigned at = atomicAdd(&bins.n_near, __popc(near));
+            unsigned place = atomicAdd(&bins.n_near, __popc(near));
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (((near >> i) & 1u) && at < kNear) bins.near[at++] = f[i];
+                if (((near >> i) & 1u) && place < kNear) bins.near[place++] = f[i];
         }
     }
     __syncthreads();
@@ -474,7 +485,7 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
     unsigned equals = 0;
     auto find = [&](int search, auto of, auto goal) {
         u64 mine = 0;
-#pragma unroll 1
+#pragma unroll 3
         for (int bin = bin0; bin < bin1; ++bin) mine += of(bin);
         u64 upto = warp_scan(mine), block = 0, all = 0;
         if (lane == 31) bins.warp[warp] = upto;
@@ -547,7 +558,7 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
             if (!(best.get() > above)) continue;
             float f[E];
             Elem<T>::unpack(w, f);
-            more += (u64)weigh.template some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), false);
+            more += (u64)weigh.template some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), true);
         }
         more = warp_sum(more);
         if (lane == 0) bins.warp[warp] = more;
