@@ -284,6 +284,20 @@ def _bytes_of(value, dtype=None):
 ROWS_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 
 
+_stream_of = None
+
+
+def _current_stream():
+    """The function that gives a device's current stream as a number: torch's own, without the object around it where
+    torch offers that."""
+    global _stream_of
+    if _stream_of is None:
+        import torch
+        _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _stream_of
+
+
 _element_types = {}  # names by dtype
 
 
@@ -603,10 +617,7 @@ class Context:
 
     def _own_stream(self, stream):
         """The given stream, or the current one of this context's device."""
-        if stream is None:
-            import torch
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return int(stream)
+        return _current_stream()(self.device) if stream is None else int(stream)
 
     def top_rows(self, x, values, index, lse=None, temperature: float = 1.0, stream=None):
         """The ``k`` largest scores of every row of ``x`` in falling order (equal ones by rising index) and where they
