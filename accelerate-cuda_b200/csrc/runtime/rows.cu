@@ -130,7 +130,7 @@ int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *
     while (room < 2 * k) room *= 2;
     const TopParams p{rows_in(x), values, index, lse, temperature, k, room};
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
-    const size_t fixed = room * sizeof(u64) + std::max(room / size * sizeof(u64), sizeof(Level));
+    const size_t fixed = (room + own_places(room, size)) * sizeof(u64);
 #define CALL(T) launch_rows(ctx, top_rows<T, true>, top_rows<T, false>, p, x, size, fixed, true, (cudaStream_t)stream, "top_rows")
     return BY_TYPE(x->type, CALL);
 #undef CALL

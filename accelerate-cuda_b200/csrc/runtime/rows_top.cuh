@@ -16,6 +16,13 @@ struct TopParams {
     int room; /* of the list of candidates, a power of two from 256 */
 };
 
+/* Places of a block's own candidates, or of a Level, which the same memory holds: an even number, since the share of the
+ * row comes behind them and starts with a whole vector. */
+static __host__ __device__ __forceinline__ int own_places(int room, int size) {
+    const int part = room / size, level = (int)(sizeof(Level) / sizeof(u64));
+    return ((part > level ? part : level) + 1) & ~1;
+}
+
 template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_rows(const __grid_constant__ TopParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 dynamic[];
@@ -26,14 +33,14 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
     __shared__ Extent extent;
     const unsigned size = cluster_size(), rank = cluster_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    u64 *list = reinterpret_cast<u64 *>(dynamic), *mine = list + p.room; /* `mine`: room / size places, or a Level */
+    u64 *list = reinterpret_cast<u64 *>(dynamic), *mine = list + p.room;
     Level &level = *reinterpret_cast<Level *>(mine);
     const T *x = static_cast<const T *>(p.in.x);
     const long long step = gridDim.x / size;
     if (size > 1) cluster_arrive(); /* every block of the cluster has started: waited for before the first message */
 
     Row<T, R> share;
-    share.init(x + (blockIdx.x / size) * p.in.pitch, p.in.cols, rank, size, dynamic + (p.room + max(p.room / (int)size, (int)sizeof(Level) / 8)) / 2);
+    share.init(x + (blockIdx.x / size) * p.in.pitch, p.in.cols, rank, size, dynamic + (p.room + own_places(p.room, (int)size)) / 2);
     share.fetch();
     if (size > 1) cluster_wait();
     int turn = 0;

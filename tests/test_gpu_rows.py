@@ -9,12 +9,17 @@ addition half a step) < 6e-6.  The result is rounded once, 2^-24 of itself.  A l
 times that.  A gradient entry is w / T times (sum p + r) q - p or (sum p + r - r / q_r) q: q and 1 / q_r are within the
 same 6e-6 of themselves plus 2^-22, the rest is computed in 64 bits and rounded once; so every part is off by at most
 twice 6e-6 of itself, and the whole is rounded to the element type."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 from rows_reference import clean, distill, sample, top
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 TYPES = ["float32", "float16", "bfloat16"]
 EPS = {"float32": 2.0**-24, "float16": 2.0**-11, "bfloat16": 2.0**-8}
@@ -55,9 +60,10 @@ def run_top(ctx, torch, x, k, temperature=1.0, lse=True):
     return numbers(values), index.cpu().numpy(), numbers(out) if lse else None
 
 
-def check_top(ctx, torch, x, k, temperature=1.0):
+def check_top(ctx, torch, x, k, temperature=1.0, every=1):
     values, index, lse = run_top(ctx, torch, x, k, temperature)
-    for r, row in enumerate(numbers(x)):
+    for r in range(0, x.shape[0], every):
+        row = numbers(x[r])
         v, i, s = top(row, k, temperature)
         assert np.array_equal(values[r], v), (r, values[r], v)
         assert np.array_equal(index[r], i), (r, index[r], i)
@@ -112,6 +118,27 @@ def test_top_of_rows_with_little_in_them(ctx, torch_cuda, rng, kind):
         if r != 5:  # an infinite score: inf - inf in the reference's formula
             assert lse[r] == s or abs(lse[r] - s) <= SUM_ERROR + 2.0**-24 * abs(s)
     assert lse[5] == np.inf
+
+
+@pytest.mark.parametrize("kind,cols", [("bfloat16", 150000), ("float16", 149993), ("float32", 75000)])
+@pytest.mark.parametrize("k", [600, 1000, 1024])
+def test_top_of_rows_held_by_five_blocks(ctx, torch_cuda, rng, kind, cols, k):
+    """A list in parts of odd length, and so many large entries at the row's start that they do not fit a part."""
+    x = rng.normal(0, 2, (60, cols)).astype(np.float32)
+    x[:, :1500] = rng.uniform(8, 12, (60, 1500))
+    x[:, :4] = rng.uniform(13, 14, (60, 4))
+    check_top(ctx, torch_cuda, place(torch_cuda, x, kind), k, every=29)
+
+
+@pytest.mark.parametrize("rows,cols,k", [(1500, 3001, 30), (1300, 1000, 200)])
+def test_top_many_rows(ctx, torch_cuda, rng, rows, cols, k):
+    """More rows than the GPU holds at a time, rows whose candidates fit a list and others side by side."""
+    x = rng.normal(0, 2, (rows, cols)).astype(np.float32)
+    x[::3] = np.round(x[::3])  # ties
+    x[5::7, :cols // 2] += 9.0
+    x[4] = -np.inf
+    x[9, 3:] = np.nan
+    check_top(ctx, torch_cuda, place(torch_cuda, x, "bfloat16", cols + 1, 1), k)
 
 
 # --------------------------------------------------------------- sampling
@@ -548,6 +575,36 @@ def test_teacher_to_student_to_answer_on_a_stream_and_as_a_graph(accb, ctx, torc
         t.cuda.synchronize()
         for a, b in zip((values, index, lse, loss, grad, token), eager):
             assert t.equal(a, b)
+
+
+def test_first_calls_are_captured():
+    """A program whose first call of each kind is made while its stream is captured."""
+    code = """
+import importlib, torch
+accb = importlib.import_module("accelerate-cuda_b200")
+ctx = accb.Context(0)
+x = torch.randn(40, 9000, device="cuda").bfloat16()
+u = torch.full((40,), 0.5, device="cuda")
+values, index, token = torch.empty_like(x[:, :8]), torch.empty(40, 8, dtype=torch.int32, device="cuda"), torch.empty(40, dtype=torch.int32, device="cuda")
+loss, grad, lse = torch.empty(40, device="cuda"), torch.empty_like(x), torch.empty(40, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def run():
+    ctx.top_rows(x, values, index, lse=lse)
+    ctx.sample_rows(x, u, token)
+    ctx.distill_rows(x, values, index, loss, grad=grad, teacher_lse=lse)
+with torch.cuda.graph(graph):
+    run()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (values, index, lse, token, loss, grad)]
+run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (values, index, lse, token, loss, grad)))
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
 
 
 def test_calls_on_two_streams_at_once(ctx, torch_cuda, rng):
