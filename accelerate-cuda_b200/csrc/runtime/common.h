@@ -174,7 +174,13 @@ struct accb_context {
     std::set<CUfunction> carveout_set; /* entries already told to prefer shared memory over L1 */
     const void *rows_ready[32] = {}; /* kernels of rows.cu whose shared memory this context has raised */
     int rows_ready_count = 0;
-    std::map<std::tuple<const void *, int, size_t>, int> rows_clusters; /* clusters of such a kernel that the GPU holds at a time */
+    struct RowsClusters {
+        const void *kernel;
+        int size;
+        size_t smem;
+        int most; /* clusters of `size` blocks that the GPU holds at a time */
+    } rows_clusters[64] = {}; /* of launches of late; the oldest makes room */
+    int rows_clusters_next = 0;
     std::map<std::tuple<CUfunction, int, size_t>, int> occupancy_cache; /* resident blocks per SM */
     size_t mem_hits = 0, disk_hits = 0, compiles = 0;
     bool trace_exec = false, trace_gc = false, trace_cc = false;

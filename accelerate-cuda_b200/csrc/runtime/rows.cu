@@ -7,6 +7,7 @@
  * is held on chip.
  */
 #include <algorithm>
+#include <iterator>
 
 #include "common.h"
 #include "rows_distill.cuh"
@@ -94,13 +95,18 @@ static int launch_rows(accb_context *ctx, void (*resident)(const P), void (*stre
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     if (persistent) { /* as many clusters as the GPU holds at a time, if there are more rows */
-        int &most = ctx->rows_clusters[std::make_tuple((const void *)kernel, size, smem)];
-        if (most == 0) {
+        auto known = std::find_if(std::begin(ctx->rows_clusters), std::end(ctx->rows_clusters), [&](const accb_context::RowsClusters &c) {
+            return c.kernel == (const void *)kernel && c.size == size && c.smem == smem;
+        });
+        if (known == std::end(ctx->rows_clusters)) {
+            int most = 0;
             const int st = check_cuda(ctx, cudaOccupancyMaxActiveClusters(&most, (const void *)kernel, &cfg), name);
             if (st != ACCB_OK) return st;
-            most = std::max(1, most);
+            known = ctx->rows_clusters + ctx->rows_clusters_next;
+            ctx->rows_clusters_next = (ctx->rows_clusters_next + 1) % (int)std::size(ctx->rows_clusters);
+            *known = {(const void *)kernel, size, smem, std::max(1, most)};
         }
-        clusters = std::min<long long>(clusters, most);
+        clusters = std::min<long long>(clusters, known->most);
         cfg.gridDim = dim3((unsigned)(clusters * size));
     }
     if (ctx->trace_exec)

@@ -607,6 +607,14 @@ print("captured")
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
 
 
+def test_rows_of_more_lengths_than_are_remembered(ctx, torch_cuda, rng):
+    """The context remembers how many clusters the GPU holds for the last 64 kinds of launch."""
+    lengths = list(range(40, 40 + 8 * 80, 8)) * 2
+    x = scores(torch_cuda, rng, 400, 700, "float32")
+    for n in lengths:
+        check_top(ctx, torch_cuda, x[:, :n], 3, every=133)
+
+
 def test_calls_on_two_streams_at_once(ctx, torch_cuda, rng):
     t = torch_cuda
     x = scores(t, rng, 300, 30011, "bfloat16")
