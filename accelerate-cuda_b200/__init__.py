@@ -283,18 +283,21 @@ def _bytes_of(value, dtype=None):
 
 ROWS_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 
-
 _stream_of = None
 
 
 def _current_stream():
     """The function that gives a device's current stream as a number: torch's own, without the object around it where
-    torch offers that."""
+    torch offers that; 0 without torch."""
     global _stream_of
     if _stream_of is None:
-        import torch
-        _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-            lambda device: torch.cuda.current_stream(device).cuda_stream)
+        try:
+            import torch
+        except ImportError:
+            _stream_of = lambda device: 0  # noqa: E731
+        else:
+            _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda device: torch.cuda.current_stream(device).cuda_stream)
     return _stream_of
 
 

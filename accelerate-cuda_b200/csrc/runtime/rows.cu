@@ -59,7 +59,25 @@ static int check_rows(accb_context *ctx, const accb_rows_array *a, const char *w
     return ACCB_OK;
 }
 
+/* an array of elements of `bytes` bytes, or null */
+static int check_aligned(accb_context *ctx, const void *ptr, size_t bytes, const char *what, const char *name) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes ? fail(ctx, ACCB_EINVAL, "%s: misaligned pointer to %s", what, name) : ACCB_OK;
+}
+
 static RowsIn rows_in(const accb_rows_array *a) { return RowsIn{a->ptr, a->rows, a->pitch, a->cols}; }
+
+/* Whether rows of two matrices of one shape and type share memory; the same memory row by row does not count, nor do
+ * matrices side by side in the rows of a larger one. */
+static bool overlap(const accb_rows_array *a, const accb_rows_array *b) {
+    const long long bytes = (long long)size_of(a->type), row = a->cols * bytes;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a->ptr), q = reinterpret_cast<uintptr_t>(b->ptr);
+    const long long p_step = a->rows > 1 ? a->pitch * bytes : row, q_step = a->rows > 1 ? b->pitch * bytes : row;
+    if (p + (a->rows - 1) * p_step + row <= q || q + (a->rows - 1) * q_step + row <= p) return false;
+    if (p_step != q_step) return true;
+    if (p == q) return false;
+    const long long apart = (long long)((p < q ? q - p : p - q) % (uintptr_t)p_step);
+    return apart < row || p_step - apart < row;
+}
 
 /* shared memory of a block's share of a row */
 static size_t share_bytes(const accb_rows_array *a, int size) {
@@ -132,6 +150,9 @@ int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *
     if (!(temperature > 1e-30) || temperature > 1e30) return fail(ctx, ACCB_EINVAL, "top_rows: bad temperature %g", temperature);
     if (x->rows == 0) return ACCB_OK;
     if (!values || !index) return fail(ctx, ACCB_EINVAL, "top_rows: null result");
+    TRY(check_aligned(ctx, values, size_of(x->type), "top_rows", "values"));
+    TRY(check_aligned(ctx, index, 4, "top_rows", "index"));
+    TRY(check_aligned(ctx, lse, 4, "top_rows", "lse"));
     int room = 256;
     while (room < 2 * k) room *= 2;
     const TopParams p{rows_in(x), values, index, lse, temperature, k, room};
@@ -147,10 +168,13 @@ int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_rows_arra
                      int32_t *token, float *logprob) {
     LOCK(ctx);
     TRY(check_rows(ctx, x, "sample_rows"));
-    if (allowed && allowed_pitch < (x->cols + 31) / 32)
+    if (allowed && (allowed_pitch < (x->cols + 31) / 32 || allowed_pitch > (1LL << 60) / std::max(1LL, x->rows)))
         return fail(ctx, ACCB_EINVAL, "sample_rows: %lld words of allowed bits for rows of %d entries", allowed_pitch, x->cols);
     if (x->rows == 0) return ACCB_OK;
     if (!uniform || !token) return fail(ctx, ACCB_EINVAL, "sample_rows: null random numbers or result");
+    const void *const arrays[] = {allowed, uniform, temperature, top_k, top_p, min_p, token, logprob};
+    const char *const names[] = {"allowed", "uniform", "temperature", "top_k", "top_p", "min_p", "token", "logprob"};
+    for (int i = 0; i < 8; ++i) TRY(check_aligned(ctx, arrays[i], 4, "sample_rows", names[i]));
     const SampleParams p{rows_in(x), allowed, allowed_pitch, uniform, temperature, top_p, min_p, top_k, token, logprob};
     const int size = cluster_for(x->rows, (long long)x->cols * size_of(x->type), ctx->sm_count);
 #define CALL(T)                                                                                                                            \
@@ -178,6 +202,11 @@ static int distill(accb_context *ctx, accb_stream stream, const accb_rows_array 
     if (student->rows == 0) return ACCB_OK;
     if (!p.teacher || !p.index) return fail(ctx, ACCB_EINVAL, "%s: null teacher", what);
     if (backward ? !p.stats || !grad : !p.loss) return fail(ctx, ACCB_EINVAL, "%s: null result or statistics", what);
+    const void *const arrays[] = {p.index, p.teacher_lse, p.weight, p.upstream, p.loss, p.stats};
+    const char *const names[] = {"index", "teacher_lse", "weight", "upstream", "loss", "stats"};
+    for (int i = 0; i < 6; ++i) TRY(check_aligned(ctx, arrays[i], 4, what, names[i]));
+    TRY(check_aligned(ctx, p.teacher, size_of(p.teacher_type), what, "teacher"));
+    if (grad && overlap(student, grad)) return fail(ctx, ACCB_EINVAL, "%s: the gradient overlaps the scores and is not in their place", what);
     p.in = rows_in(student);
     const int size = cluster_for(student->rows, (long long)student->cols * size_of(student->type), ctx->sm_count);
     const long long share = (long long)share_bytes(student, size) / size_of(student->type); /* entries of a block's share, at most */

@@ -270,10 +270,9 @@ ACCB_API int accb_top_rows(accb_context *ctx, accb_stream stream, const accb_row
  *   min_p   of those, the ones whose weight is at least min_p of the best one's (0 and below: off; above 1 as 1),
  * and the row's token is the first kept index, in index order, at which the running sum of the kept weights exceeds
  * uniform times their total.  A temperature that is not above 0 takes the best entry, one above 1e30 counts as 1e30.
- * `allowed` (or NULL) holds bits
- * for the entries, bit j % 32 of word j / 32 for entry j, rows every allowed_pitch words: the others are not there,
- * whatever their score; nor are -inf and NaN.  A row with no entry gives token -1.  logprob (or NULL): log of the
- * token's share of the kept weight; -inf with token -1.
+ * `allowed` (or NULL) holds bits for the entries, bit j % 32 of word j / 32 for entry j, rows every allowed_pitch
+ * words: the others are not there, whatever their score; nor are -inf and NaN.  A row with no entry gives token -1.
+ * logprob (or NULL): log of the token's share of the kept weight; -inf with token -1.
  * Weights are added as whole multiples of 2^-43 of the best entry's: sums are exact, and the token does not depend
  * on how a row is split over the GPU. */
 ACCB_API int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *x, const uint32_t *allowed,
@@ -299,7 +298,8 @@ ACCB_API int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_
  *          temperature), and the two factors of q in the gradient, at named entries (sum p + r) and elsewhere
  *          (sum p + r - r / q_r).  All 0 for rows that do not count.
  *   grad   NULL, or the gradient of sum(loss) in the student's shape and type, written in the same pass:
- *          weight / temperature * (factor * q - p).  It may be the student's own memory (same pointer and pitch). */
+ *          weight / temperature * (factor * q - p).  It may be the student's own memory (same pointer and pitch);
+ *          any other overlap of the two is refused. */
 ACCB_API int accb_distill_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const void *teacher,
                                int teacher_type, const int32_t *index, int k, const float *teacher_lse,
                                const float *weight, double temperature, float *loss, float *stats,

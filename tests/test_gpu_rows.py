@@ -662,6 +662,46 @@ def test_offsets_past_32_bits(ctx, torch_cuda, rng):
     check_gradient(numbers(x), host, tv, ti, None, np.ones(rows), np.ones(rows), 1.0, "bfloat16")
 
 
+def test_gradient_beside_the_scores(ctx, torch_cuda, rng):
+    """Scores and gradient side by side in the rows of one matrix; any other overlap is refused."""
+    t = torch_cuda
+    both = t.full((5, 2100), 7.0, dtype=t.bfloat16, device="cuda")
+    x, grad = both[:, :1000], both[:, 1003:2003]
+    x.copy_(scores(t, rng, 5, 1000, "bfloat16"))
+    tv, ti, _ = teacher_of(t, rng, x, 5, "float32", 1.0, False)
+    host, loss = x.clone(), t.empty(5, device="cuda")
+    ctx.distill_rows(x, tv, ti, loss, grad=grad)
+    ctx.sync()
+    check_gradient(numbers(grad), host, tv, ti, None, np.ones(5), np.ones(5), 1.0, "bfloat16")
+    assert t.equal(x, host) and (both[:, 1000:1003] == 7).all() and (both[:, 2003:] == 7).all()
+
+
+def test_overlaps_and_misaligned_pointers_are_refused(accb, ctx, torch_cuda):
+    t = torch_cuda
+    L = accb.lib()
+    import ctypes as C
+    m = t.zeros(4096, device="cuda")
+    p, off = C.c_void_p(m.data_ptr()), C.c_void_p(m.data_ptr() + 2)
+    rows = lambda at=0, pitch=10, rows=4: C.byref(accb.accb_rows_array(m.data_ptr() + 4 * at, 0, 8, rows, pitch))  # noqa: E731
+    for a, b in ((rows(), rows(1)), (rows(5), rows()), (rows(), rows(9)), (rows(), rows(12)), (rows(), rows(0, 11)), (rows(0, 10, 1), rows(7, 10, 1)),
+                 (rows(20, 8), rows(51, 8))):
+        assert L.accb_distill_rows(ctx.handle, None, a, p, 0, p, 2, None, None, 1.0, p, None, b) == accb.EINVAL
+        assert L.accb_distill_rows_backward(ctx.handle, None, a, p, 0, p, 2, None, None, 1.0, p, None, b) == accb.EINVAL
+    x = rows(1024)
+    for i in range(3):
+        v = [off if i == j else p for j in range(3)]
+        assert L.accb_top_rows(ctx.handle, None, x, 1.0, 2, *v) == accb.EINVAL
+    for i in range(8):
+        v = [off if i == j else p for j in range(8)]
+        assert L.accb_sample_rows(ctx.handle, None, x, v[0], 1, *v[1:]) == accb.EINVAL
+    assert L.accb_sample_rows(ctx.handle, None, x, p, 1 << 60, *([p] * 7)) == accb.EINVAL
+    for i in range(6):
+        v = [off if i == j else p for j in range(6)]
+        assert L.accb_distill_rows(ctx.handle, None, x, v[0], 0, v[1], 2, v[2], v[3], 1.0, v[4], v[5], None) == accb.EINVAL
+        assert L.accb_distill_rows_backward(ctx.handle, None, x, v[0], 0, v[1], 2, v[2], v[3], 1.0, v[4], v[5], rows(2048)) == accb.EINVAL
+    ctx.sync()
+
+
 # ------------------------------------------------------------ refusals
 def test_refusals_of_the_library(accb, ctx, torch_cuda):
     t = torch_cuda
