@@ -23,6 +23,17 @@ static __host__ __device__ __forceinline__ int own_places(int room, int size) {
     return ((part > level ? part : level) + 1) & ~1;
 }
 
+/* The k largest are found in one pass over the row's maximum, one over its exponentials (if asked for) and one over the
+ * few entries above a bound: ceil(k / size) of every block's 256 threads hold a maximum at or above the bound, so at
+ * least k entries do, and seldom many more.  They are listed in one block's memory, and sorted; the blocks of a cluster
+ * take the rows' lists in turns and sort side by side.  Only rows whose list overflows (ties, large entries side by
+ * side) search for the border with counting bins and list again.
+ * Clusters stay for row after row: the next row is fetched as soon as the listing has read this one, under the sort.
+ *
+ * 64 of 2048 x 131072 bf16 with log-sum-exp: 243 us, 2.2 TB/s, a third of the copy rate; 512 of 24 x 50257 floats: 23 us.
+ * A row takes its blocks 13 us, three an SM, most of it waiting for copies, barriers and instructions; the special function
+ * unit is busy for a third of the time.  The search by bins in place of lists took 947 us, one row per cluster without
+ * the turns 311. */
 template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_rows(const __grid_constant__ TopParams p) {
     constexpr int E = Elem<T>::E;
     extern __shared__ uint4 dynamic[];

@@ -19,7 +19,7 @@ module Data.Array.Accelerate.B200.FFI (
   AccbContext, AccbKernel, AccbProgram, Stream,
 
   -- * Records
-  AccbArray(..), AccbValueType(..), maxRank, maxComp,
+  AccbArray(..), AccbValueType(..), AccbRowsArray(..), maxRank, maxComp,
 
   -- * Status
   Status, statusOK, throwOnError,
@@ -31,6 +31,9 @@ module Data.Array.Accelerate.B200.FFI (
   -- * Single launches on device arrays
   c_map, c_foldAll, c_foldDim, c_foldSeg, c_scan, c_permuteDefaults, c_permute,
   c_stencil, c_stencil2, c_stencilIterate, c_stencilIterateFrom,
+
+  -- * Rows of scores
+  c_topRows, c_sampleRows, c_distillRows, c_distillRowsBackward, rowsF32, rowsF16, rowsBF16,
 
   -- * Memory table
   c_malloc, c_use, c_insertUnmanaged, c_withPtr, c_release, c_releaseAfter,
@@ -110,6 +113,35 @@ instance Storable AccbValueType where
     b <- forM [0 .. fromIntegral n - 1] $ \c -> (fromIntegral :: CInt -> Int) <$> peekByteOff p (8 + 4 * c)
     return (AccbValueType (fromIntegral r) b)
 
+-- | @struct accb_rows_array@: a matrix of scores, rows 'rowsPitch' elements apart.
+data AccbRowsArray = AccbRowsArray
+  { rowsPtr   :: Ptr ()
+  , rowsType  :: CInt          -- ^ 'rowsF32', 'rowsF16' or 'rowsBF16'
+  , rowsCols  :: Int
+  , rowsRows  :: Int
+  , rowsPitch :: Int
+  }
+
+instance Storable AccbRowsArray where
+  sizeOf    _ = 32             -- void *ptr; int type, cols; long long rows, pitch
+  alignment _ = 8
+  poke p AccbRowsArray{..} = do
+    pokeByteOff p 0  rowsPtr
+    pokeByteOff p 8  rowsType
+    pokeByteOff p 12 (fromIntegral rowsCols  :: CInt)
+    pokeByteOff p 16 (fromIntegral rowsRows  :: CLLong)
+    pokeByteOff p 24 (fromIntegral rowsPitch :: CLLong)
+  peek p = do
+    a <- peekByteOff p 0
+    t <- peekByteOff p 8
+    c <- peekByteOff p 12 :: IO CInt
+    r <- peekByteOff p 16 :: IO CLLong
+    w <- peekByteOff p 24 :: IO CLLong
+    return (AccbRowsArray a t (fromIntegral c) (fromIntegral r) (fromIntegral w))
+
+rowsF32, rowsF16, rowsBF16 :: CInt
+rowsF32 = 0; rowsF16 = 1; rowsBF16 = 2
+
 -- | Every entry point returns a status; the message lives in the context
 -- (the reference turns CUDA errors into exceptions, CUDA/State.hs:87-88).
 throwOnError :: Ptr AccbContext -> Status -> IO ()
@@ -172,6 +204,25 @@ foreign import ccall safe "accb_stencil_iterate"
 foreign import ccall safe "accb_stencil_iterate_from"
   c_stencilIterateFrom :: Ptr AccbContext -> Ptr AccbKernel -> Stream -> Ptr AccbArray -> Ptr AccbArray -> Ptr AccbArray
                        -> CInt -> CInt -> Ptr () -> CSize -> Ptr CInt -> IO Status
+
+-- rows of scores: best entries, one entry drawn per row, divergence from a teacher's best entries (no counterpart in the
+-- reference).  Null pointers where the header says "or NULL".
+foreign import ccall safe "accb_top_rows"
+  c_topRows :: Ptr AccbContext -> Stream -> Ptr AccbRowsArray -> CDouble {- temperature -} -> CInt {- k -}
+            -> Ptr () {- values -} -> Ptr CInt {- index -} -> Ptr CFloat {- lse -} -> IO Status
+foreign import ccall safe "accb_sample_rows"
+  c_sampleRows :: Ptr AccbContext -> Stream -> Ptr AccbRowsArray -> Ptr Word32 {- allowed -} -> CLLong {- its pitch -}
+               -> Ptr CFloat {- uniform -} -> Ptr CFloat {- temperature -} -> Ptr CInt {- top_k -} -> Ptr CFloat {- top_p -}
+               -> Ptr CFloat {- min_p -} -> Ptr CInt {- token -} -> Ptr CFloat {- logprob -} -> IO Status
+foreign import ccall safe "accb_distill_rows"
+  c_distillRows :: Ptr AccbContext -> Stream -> Ptr AccbRowsArray {- student -} -> Ptr () {- teacher -} -> CInt {- its type -}
+                -> Ptr CInt {- index -} -> CInt {- k -} -> Ptr CFloat {- teacher_lse -} -> Ptr CFloat {- weight -}
+                -> CDouble {- temperature -} -> Ptr CFloat {- loss -} -> Ptr CFloat {- stats -} -> Ptr AccbRowsArray {- grad -}
+                -> IO Status
+foreign import ccall safe "accb_distill_rows_backward"
+  c_distillRowsBackward :: Ptr AccbContext -> Stream -> Ptr AccbRowsArray -> Ptr () -> CInt -> Ptr CInt -> CInt
+                        -> Ptr CFloat -> Ptr CFloat -> CDouble -> Ptr CFloat {- stats -} -> Ptr CFloat {- upstream -}
+                        -> Ptr AccbRowsArray {- grad -} -> IO Status
 
 -- memory table: malloc / withRemote / insertUnmanaged / free / reclaim (CUDA/Array/Remote.hs:91-202),
 -- peek / poke (CUDA/Array/Prim.hs:189-391).  Keys are the hash of the host array's StableName.
