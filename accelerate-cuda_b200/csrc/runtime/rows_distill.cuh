@@ -36,6 +36,11 @@ struct Named {
     int first;   /* the first of its index that was met */
 };
 
+/* Where the best of the entries not named is less likely than this share of the row's best, the statistics hold the
+ * gradient of the others by their own maximum: q, and q times a factor that is a share of 1 / q_r, would leave the range
+ * of 32 bits.  Marked by a negative second number; top, -1 / sum, others_top, factor of exp((x - others_top) / tau). */
+constexpr float kApart = 2.328306437e-10f; /* 2^-32 */
+
 /* The row as all its blocks know it. */
 struct RowSums {
     float top, others_top;         /* maximum of the row, and of the entries not named (-inf: none) */
@@ -265,12 +270,10 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
             const bool excluded = all.top == neg_inf() && all.sum == 0.0; /* by the student, every entry */
             double r = rest && all.others_top > neg_inf() ? fmax(0.0, 1.0 - named_p) : 0.0;
             float4 said = make_float4(all.top, (float)(1.0 / all.sum), (float)(named_p + r), (float)(named_p + r));
-            if (r > 0.0) {
-                /* r over the student's share of the others, which may be too small for its own exponential */
-                double over = all.sum / all.others_sum;
-                over = down > 0.0f ? over / (double)down : over * exp_64(((double)all.top - (double)all.others_top) * inv);
-                said.w = (float)(named_p + r - r * over);
-            }
+            if (r > 0.0 && down >= kApart)
+                said.w = (float)(named_p + r - r * (all.sum / all.others_sum / (double)down));
+            else if (r > 0.0)
+                said = make_float4(all.top, -said.y, all.others_top, (float)((named_p + r) * (double)said.y * (double)down - r / all.others_sum));
             if (excluded) said = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (lane == 0) statistics = said;
             if (rank == 0) {
@@ -297,8 +300,9 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
     /* gradient: elsewhere * q everywhere, then the named entries once more with their own value */
     float g = (float)((double)weight * inv);
     if (BACKWARD && p.upstream) g *= p.upstream[row];
-    const float factor = g * elsewhere * inverse;
-    const Pair times(factor, factor), less(-top, -top), by(c, c);
+    const bool apart = inverse < 0.0f;
+    const float factor = apart ? g * elsewhere : g * elsewhere * inverse, base = apart ? at_named : top;
+    const Pair times(factor, factor), less(-base, -base), by(c, c);
 #pragma unroll 2
     for (int v = share.first; v < share.last; v += 32) {
         float f[E];
@@ -323,8 +327,8 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
                 }
             if (earlier) continue;
         }
-        const float q = inverse * fast_exp2((named[j].z - top) * c);
-        grad[at] = Elem<T>::down(g * (float)((double)at_named * q - sum));
+        const float q = fabsf(inverse) * fast_exp2((named[j].z - top) * c);
+        grad[at] = Elem<T>::down(g * (float)((apart ? fmax(named_p, 1.0) : (double)at_named) * q - sum));
     }
 }
 

@@ -291,12 +291,14 @@ ACCB_API int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_
  * teacher and index: rows x k, 1 <= k <= 1024.  An index outside the row, and a score of -inf or NaN, names nothing;
  * an index named twice has both probabilities.  weight: one per row, or NULL for 1.  A row with weight 0, one whose
  * teacher names nothing, and one of a student with only -inf has loss 0 and gradient 0, and the scores of a row with
- * weight 0 are not read.  r counts for nothing where the student leaves nothing to the others.  A NaN of the student
- * in a row that counts makes its loss and gradient NaN.
+ * weight 0 are not read.  r counts for nothing where the student leaves nothing to the others.  A NaN or +inf of the
+ * student, or +inf of the teacher, in a row that counts leaves its loss and gradient without a finite value.
  *   loss   rows
  *   stats  rows x 4, or NULL: what the backward pass needs -- the row's maximum, 1 / sum exp((x - maximum) /
  *          temperature), and the two factors of q in the gradient, at named entries (sum p + r) and elsewhere
  *          (sum p + r - r / q_r).  All 0 for rows that do not count.
+ *          Where the unnamed entries are less likely than 2^-32 of the best one, the second is negated, the
+ *          third is the maximum of the unnamed entries and the fourth the factor of exp((x - that) / temperature).
  *   grad   NULL, or the gradient of sum(loss) in the student's shape and type, written in the same pass:
  *          weight / temperature * (factor * q - p).  It may be the student's own memory (same pointer and pitch);
  *          any other overlap of the two is refused. */

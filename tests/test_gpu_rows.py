@@ -339,7 +339,7 @@ def check_gradient(got, x, teacher, index, lse, weight, upstream, temperature, k
         # (sum p + r) q - p, (sum p + r - r / q_r) q: every part is off by its own share, however small the difference
         parts = parts * abs(upstream[r])
         small = 2.0**-24 if kind == "float16" else 2.0**-126  # half a step of subnormal numbers
-        bad = np.abs(got[r] - d) > EPS[kind] * np.abs(d) + 2 * SUM_ERROR * parts + small
+        bad = ~(np.abs(got[r] - d) <= EPS[kind] * np.abs(d) + 2 * SUM_ERROR * parts + small)
         assert not bad.any(), (r, np.nonzero(bad)[0][:5], got[r][bad][:5], d[bad][:5])
 
 
@@ -459,6 +459,43 @@ def test_distill_the_rest_alone_far_below(ctx, torch_cuda, rng):
     ctx.sync()
     want = [distill(x[r], tv[r].cpu().numpy(), ti[r].cpu().numpy(), float(lse[r]), 1.0, 1.0)[0] for r in range(2)]
     assert np.abs(numbers(loss) - want).max() <= 2.0**-23 * max(want) + 2 * SUM_ERROR
+
+
+@pytest.mark.parametrize("kind,cols", [("float32", 2000), ("bfloat16", 40000), ("float16", 3001), ("float32", (1 << 20) - 7)])
+@pytest.mark.parametrize("temperature", [1.0, 0.05])
+def test_distill_gradient_of_the_rest_far_below(ctx, torch_cuda, rng, kind, cols, temperature):
+    """Entries that are not named and so unlikely that their probability has no 32-bit value: the share of the rest that
+    an entry has still moves it.  From nearly as likely as the named ones to e^-600."""
+    t = torch_cuda
+    apart = np.array([0.0, 10.0, 20.0, 24.0, 40.0, 70.0, 100.0, 200.0, 600.0], np.float32) * temperature
+    if cols > 1 << 19:
+        apart = apart[5:7]
+    rows = apart.size
+    x = rng.normal(0, 2 * temperature, (rows, cols)).astype(np.float32)
+    at = np.stack([rng.choice(cols, 4, replace=False) for _ in range(rows)]).astype(np.int32)
+    np.put_along_axis(x, at, rng.normal(0, temperature, (rows, 4)).astype(np.float32) + 9 * temperature + apart[:, None], 1)
+    tv = t.tensor([[1.0, 0.5, 0.2, 0.1]] * rows, device="cuda") * temperature
+    lse = t.full((rows,), 2.0, device="cuda")
+    lse[1::3] = 4.0
+    check_distill(ctx, t, rng, place(t, x, kind, cols + 1, 1), 4, temperature, teacher=(tv, t.from_numpy(at).cuda(), lse), in_place=True)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_infinities_in_a_row_that_counts(ctx, torch_cuda, rng, rest):
+    """+inf has no share of a softmax: loss and gradient are NaN, of that row alone."""
+    t = torch_cuda
+    x = scores(t, rng, 4, 1000, "bfloat16")
+    tv, ti, lse = teacher_of(t, rng, x, 3, "float32", 1.0, rest)
+    x[0, 999] = float("inf")
+    x[1, int(ti[1, 2])] = float("inf")
+    tv[2, 1] = float("inf")
+    loss, grad = t.zeros(4, device="cuda"), t.zeros_like(x)
+    ctx.distill_rows(x, tv, ti, loss, grad=grad, teacher_lse=lse)
+    ctx.sync()
+    if not rest:
+        assert loss.isnan().tolist() == [True, True, True, False]
+    assert not loss[:3].isfinite().any() and loss[3].isfinite()
+    assert not grad[3].isnan().any()
 
 
 def test_distill_nan_in_a_row_that_counts(ctx, torch_cuda, rng):
