@@ -425,7 +425,8 @@ template <class V> __device__ __forceinline__ V warp_scan(V v) { /* inclusive */
  * so that sums do not depend on their order -- on how a row is split over warps and blocks -- and a million entries
  * (kMaxCols) still fit into 64 bits.  Two indices are told apart by a sum: an error of 2^-24 of each of 10^5 like
  * entries would pick the wrong one every few thousand rows.  So 2^y is computed in 64 bits:
- *     64 y = K + r, K whole, |r| <= 1/2;  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r)
+ *     64 y = x c - N = K + r, c = 64 log2(e) / T, N the whole number next to top c, K whole, |r| <= 1/2;  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r)
+ * (the product x c is not rounded; N leaves all weights of a row a common factor of at most 2^(1/128)),
  * with the cubic Taylor polynomial of 2^(r / 64), wrong by less than (ln 2 / 128)^4 / 24 < 2^-34.6 of itself: eight
  * 64-bit operations where the library's function takes some twenty.  The table is in shared memory sixteen times, a
  * copy for every lane of a half warp, so that no two lanes meet in a bank; entry j is stored with j << 14 taken from its
@@ -440,29 +441,32 @@ static __device__ __noinline__ void fill_table(double *table) { /* kTable * kTab
     for (int i = threadIdx.x / kTable; i < kTableCopies; i += kThreads / kTable) table[(threadIdx.x % kTable) * kTableCopies + i] = v;
 }
 
-/* WIDE: scores of 24 bits, whose distance from the maximum takes 64 bits.  That of two 16-bit scores is exact in 32,
- * but for scores nearer to 0 than 2^-16 of the maximum, where it is off by 2^-25 of itself. */
-template <bool WIDE> struct Weigh {
+struct Weigh {
     static constexpr double kRound = 6755399441055744.0; /* 1.5 * 2^52: adding it rounds to a whole number */
     float top, least;    /* scores below `least` weigh less than half a unit, or are excluded */
     double c;            /* 64 log2(e) / T */
+    double start;        /* kRound less the whole number next to top * c: what that leaves is a factor of all weights */
     const double *table; /* this lane's copy */
 
     __device__ __forceinline__ Weigh(float maximum, double temperature, const double *shared_table) {
         top = maximum;
         table = shared_table + (threadIdx.x & (kTableCopies - 1));
         c = 64.0 * 1.4426950408889634 / temperature;
+        /* so cold that any other score weighs nothing, and would not be told apart: the maxima have one weight each */
+        if (!(fabs((double)top * c) < 1125899906842624.0)) c = 0.0;
+        start = kRound - rint((double)top * c);
         least = fmaxf(-3.402823466e+38f, (float)((double)top - (kUnitLog2 + 2) * 0.69314718055994531 * temperature));
     }
+    /* log of the weight of the maximum, in units */
+    __device__ __forceinline__ double log_of_top() const { return fma((double)top, c, start - kRound) * (0.69314718055994531 / kTable); }
     /* for f >= least; anything below */
     __device__ __forceinline__ u64 of(float f) const { return (u64)__double_as_longlong(above_2_52(f)) & 0xfffffffffffffull; }
     /* 2^52 + the weight */
     __device__ __forceinline__ double above_2_52(float f) const {
         constexpr double l = 0.69314718055994531 / kTable;
-        const double x = WIDE ? (double)f - (double)top : (double)(f - top);
-        const double t = fma(x, c, kRound);
+        const double x = (double)f, t = fma(x, c, start);
         const int k = __double2loint(t);
-        const double r = fma(x, c, kRound - t);
+        const double r = fma(x, c, start - t);
         double m = table[(k & (kTable - 1)) * kTableCopies];
         m = __hiloint2double(__double2hiint(m) + (k << 14), __double2loint(m));
         const double unit = (double)(1ull << kUnitLog2);

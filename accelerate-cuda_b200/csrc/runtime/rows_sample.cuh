@@ -35,17 +35,17 @@ __device__ __forceinline__ u64 drawn(float uniform, u64 total) {
     return want > 0.0 ? min((u64)want, total - 1) : 0;
 }
 
-__device__ __forceinline__ void put_token(const SampleParams &p, long long row, int index, float value, float most, double temperature, u64 total) {
+__device__ __forceinline__ void put_token(const SampleParams &p, long long row, int index, float value, const Weigh &weigh, double temperature, u64 total) {
     p.token[row] = index;
     if (p.logprob) {
-        const double below = value == most ? 0.0 : ((double)value - (double)most) / temperature;
-        p.logprob[row] = (float)(below - log_64((double)total * (1.0 / (double)(1ull << kUnitLog2))));
+        const double below = value == weigh.top ? 0.0 : ((double)value - (double)weigh.top) / temperature;
+        p.logprob[row] = (float)(below - (log_64((double)total * (1.0 / (double)(1ull << kUnitLog2))) - weigh.log_of_top()));
     }
 }
 
 /* Draws from the candidates in `list`, which hold every entry that top_k and top_p could keep; by one block. */
-template <class W> __device__ __noinline__ void draw_from_list(const SampleParams &p, const PendingDraw &d, u64 *list, u64 *scratch, unsigned size, const double *table) {
-    const W weigh(d.most, d.temperature, table);
+static __device__ __noinline__ void draw_from_list(const SampleParams &p, const PendingDraw &d, u64 *list, u64 *scratch, unsigned size, const double *table) {
+    const Weigh weigh(d.most, d.temperature, table);
     const int k = d.k;
     const float top_p = d.top_p, lowest = d.lowest;
     u64 total = d.total;
@@ -85,7 +85,7 @@ template <class W> __device__ __noinline__ void draw_from_list(const SampleParam
             const float x = value_of((unsigned)list[i]);
             if ((unsigned)list[i]) before += weigh.weight(x);
             if (target < before) {
-                put_token(p, d.row, index_of(list[i] >> 32), x, d.most, d.temperature, total);
+                put_token(p, d.row, index_of(list[i] >> 32), x, weigh, d.temperature, total);
                 return;
             }
         }
@@ -154,7 +154,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
         auto draw = [&] {
             if constexpr (CUTS) {
                 if (!waiting) return;
-                draw_from_list<Weigh<sizeof(T) == 4>>(p, sh.pending, sh.list, scratch, size, table);
+                draw_from_list(p, sh.pending, sh.list, scratch, size, table);
                 waiting = false;
                 __syncthreads(); /* the list is used again */
             }
@@ -236,7 +236,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
             const double low = (double)most + log_64(fmin((double)min_p, 1.0)) * temperature;
             if (low > -3.0e38) lowest = __double2float_ru(low);
         }
-        const Weigh<sizeof(T) == 4> weigh(most, temperature, table);
+        const Weigh weigh(most, temperature, table);
         if (k == 1) bound = most;
 
         /* weight above a border and number of entries on it, of this thread: the weight in quarters of the warp's
@@ -268,7 +268,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
 #pragma unroll
                         for (int i = 0; i < E; ++i) ties += f[i] == on;
                     }
-                    sum += weigh.template some<E>(f, from, most_count);
+                    sum += weigh.some<E>(f, from, most_count);
                 }
                 quarter[0] = quarter[1], quarter[1] = quarter[2], quarter[2] = quarter[3], quarter[3] = (u64)sum;
             }
@@ -292,7 +292,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
                         tell_all(told.block[1], block_total, 0, rank, size);
                         for (int i = 0; i < (int)size; ++i) total += told.block[1][i][0];
                         const double left = (1.0 - (double)top_p) * ((double)total * (1.0 / (double)(1ull << kUnitLog2)));
-                        const double low = (double)most + (log_64(left / (double)p.in.cols) - 0.01) * temperature;
+                        const double low = (double)most + (log_64(left / (double)p.in.cols) - weigh.log_of_top() - 0.01) * temperature;
                         if (left > 1e-5 && low > (double)least) least = __double2float_rd(low);
                         listed = true;
                     }
@@ -424,7 +424,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
                         c += w[i];
                         if (!done && target < c) at = share.entry(v) + i, value = f[i], done = true;
                     }
-                    put_token(p, row, at, value, most, temperature, total);
+                    put_token(p, row, at, value, weigh, temperature, total);
                 }
                 break;
             }

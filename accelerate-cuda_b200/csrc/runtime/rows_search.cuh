@@ -212,7 +212,7 @@ struct Level { /* one level of the border search */
  * arguments. */
 template <class T, bool RESIDENT, bool BY_MASS>
 __device__ __noinline__ Border find_border(const Row<T, RESIDENT> share, Level &lv, unsigned size, unsigned klo, unsigned khi,
-                              u64 target, const Weigh<sizeof(T) == 4> weigh, double fraction, unsigned spare) {
+                              u64 target, const Weigh weigh, double fraction, unsigned spare) {
     constexpr int E = Elem<T>::E, S0 = Elem<T>::kShift;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const unsigned bottom = klo;
@@ -341,7 +341,7 @@ struct BinOrder {
 /* Counts this block's entries that are not below `from`; returns its weights of the two shared bins.  All threads of the
  * block call it; barriers follow its writes. */
 template <class T, bool RESIDENT>
-__device__ __forceinline__ void count_bins(const Row<T, RESIDENT> &share, FineBins &bins, const BinOrder &order, const Weigh<sizeof(T) == 4> &weigh, float from,
+__device__ __forceinline__ void count_bins(const Row<T, RESIDENT> &share, FineBins &bins, const BinOrder &order, const Weigh &weigh, float from,
                            u64 (&coarse)[2]) {
     constexpr int E = Elem<T>::E;
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -418,7 +418,7 @@ template <bool EXACT> __device__ __forceinline__ unsigned key_of_bin(const BinOr
 }
 
 /* The weight of this block's counted entries in the bins before `end`, by all threads; two barriers. */
-template <bool WIDE> __device__ u64 weight_before(FineBins &bins, const BinOrder &order, const Weigh<WIDE> &weigh, const u64 (&coarse)[2], int end) {
+static __device__ u64 weight_before(FineBins &bins, const BinOrder &order, const Weigh &weigh, const u64 (&coarse)[2], int end) {
     u64 mine = 0;
 #pragma unroll 1
     for (int bin = threadIdx.x; bin < min(end, kFineBins); bin += kThreads) {
@@ -449,7 +449,7 @@ struct BlockPart {
  * caller's in memory.) */
 template <class T, bool RESIDENT>
 __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, FineBins &bins, Level &lv, unsigned size,
-                                              const Weigh<sizeof(T) == 4> weigh, float from, float most, u64 k, double top_p, u64 total, BlockPart &part) {
+                                              const Weigh weigh, float from, float most, u64 k, double top_p, u64 total, BlockPart &part) {
     constexpr int E = Elem<T>::E;
     constexpr bool EXACT = Elem<T>::kShift == 16; /* a bin that is not shared is one key */
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -558,7 +558,7 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
             if (!(best.get() > above)) continue;
             float f[E];
             Elem<T>::unpack(w, f);
-            more += (u64)weigh.template some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), true);
+            more += (u64)weigh.some<E>(f, fmaxf(weigh.least, value_of(khi + 1u)), true);
         }
         more = warp_sum(more);
         if (lane == 0) bins.warp[warp] = more;

@@ -119,7 +119,7 @@ template <class T, bool R> __global__ void __launch_bounds__(kThreads, 3) top_ro
         if (crowded) {
             /* too many (ties, or rows of few large entries side by side): find the border, then list what is above it and
              * the first of what is on it */
-            const Weigh<sizeof(T) == 4> none(0.0f, 1.0, nullptr);
+            const Weigh none(0.0f, 1.0, nullptr);
             const Border border = find_border<T, R, false>(share, level, size, key_of(bound), key_of(most), (u64)p.k, none, 0.0, 0);
             unsigned ties = 0;
             for (int v = share.first; v < share.last; v += 32) {

@@ -300,6 +300,28 @@ def test_sample_of_rows_too_long_for_shared_memory(ctx, torch_cuda, rng):
         check_sample(ctx, torch_cuda, x, allowed, uniform=rng.random(2), **cuts)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("near_zero", [False, True])
+def test_sample_close_to_the_borders(ctx, torch_cuda, rng, kind, near_zero):
+    """Random numbers next to the border between two tokens (as near as 32 bits come); also where the scores are so much
+    smaller than the largest that their difference from it takes more than 32 bits."""
+    t = torch_cuda
+    rows, cols = 120, 20011
+    x = scores(t, rng, rows, cols, kind)
+    temperature = np.full(rows, 0.9, np.float32)
+    if near_zero:
+        top = 2.0 ** rng.integers(4, 8, rows)
+        x.copy_(t.from_numpy((rng.uniform(0, 2.0**-25, (rows, cols)) * top[:, None]).astype(np.float32)))
+        x[t.arange(rows), t.from_numpy(rng.choice(cols, rows))] = t.from_numpy(top).to(x.dtype).cuda()
+        temperature = (top / rng.uniform(9, 11, rows)).astype(np.float32)
+    u = np.empty(rows, np.float32)
+    for r, row in enumerate(numbers(x)):
+        share = np.cumsum(np.exp((row - row.max()) / float(temperature[r])))
+        u[r] = (share / share[-1])[rng.integers(0, cols - 1)]
+    check_sample(ctx, t, x, uniform=u, temperature=temperature)
+    check_sample(ctx, t, x, uniform=u, temperature=temperature, top_p=0.99999)
+
+
 def test_sample_draws_by_the_shares(ctx, torch_cuda):
     """4096 evenly spaced random numbers over one row draw every index as often as its share says, give or take one."""
     t = torch_cuda
