@@ -425,9 +425,10 @@ template <class V> __device__ __forceinline__ V warp_scan(V v) { /* inclusive */
  * so that sums do not depend on their order -- on how a row is split over warps and blocks -- and a million entries
  * (kMaxCols) still fit into 64 bits.  Two indices are told apart by a sum: an error of 2^-24 of each of 10^5 like
  * entries would pick the wrong one every few thousand rows.  So 2^y is computed in 64 bits:
- *     64 y = x c - N = K + r, c = 64 log2(e) / T, N the whole number next to top c, K whole, |r| <= 1/2;  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r)
- * (the product x c is not rounded; N leaves all weights of a row a common factor of at most 2^(1/128)),
- * with the cubic Taylor polynomial of 2^(r / 64), wrong by less than (ln 2 / 128)^4 / 24 < 2^-34.6 of itself: eight
+ *     64 y = x c - N = K + r,  2^y = 2^(K >> 6) * table[K & 63] * polynomial(r),
+ * c = 64 log2(e) / T, N the whole number next to top c (which leaves all weights of a row a common factor of at most
+ * 2^(1/128)), K whole, |r| <= 1/2; x c is not rounded before N is taken off.  The polynomial is
+ * the cubic Taylor one of 2^(r / 64), wrong by less than (ln 2 / 128)^4 / 24 < 2^-34.6 of itself: eight
  * 64-bit operations where the library's function takes some twenty.  The table is in shared memory sixteen times, a
  * copy for every lane of a half warp, so that no two lanes meet in a bank; entry j is stored with j << 14 taken from its
  * upper half, so that adding K << 14 there adds K >> 6 to the exponent. */

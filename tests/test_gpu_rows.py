@@ -12,6 +12,7 @@ twice 6e-6 of itself, and the whole is rounded to the element type."""
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -164,12 +165,13 @@ def run_sample(ctx, torch, x, allowed=None, **s):
     return token.cpu().numpy(), numbers(logprob)
 
 
-def check_sample(ctx, torch, x, allowed=None, **values):
+def check_sample(ctx, torch, x, allowed=None, every=1, **values):
     rows = x.shape[0]
     s = settings(torch, rows, **values)
     host = {k: v.double().cpu().numpy() for k, v in s.items()}
     token, logprob = run_sample(ctx, torch, x, bits_of(torch, allowed) if allowed is not None else None, **s)
-    for r, row in enumerate(numbers(x)):
+    for r in range(0, rows, every):
+        row = numbers(x[r])
         want, log_share, distance = sample(row, allowed=None if allowed is None else allowed[r], **{k: v[r] for k, v in host.items()})
         # a weight is off by half a unit of 2^-43 (of a total of at least one) and by the cubic polynomial, less than
         # (ln 2 / 128)^4 / 24 < 2^-34.6 of itself; both of two sums may be, so a share is off by less than
@@ -664,6 +666,79 @@ print("captured")
 """
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+def test_rows_by_any_number_of_blocks(ctx, torch_cuda, rng, kind, blocks):
+    """Enough rows that a row gets as few blocks as hold it."""
+    t = torch_cuda
+    rows, cols = 300 if blocks == 1 else 150, (69632 * blocks - 300) // (2 if kind == "bfloat16" else 4)
+    x = scores(t, rng, rows, cols, kind)
+    few = (rows - 1) // 3
+    check_top(ctx, t, x, 50, every=few)
+    check_top(ctx, t, x, 900, 2.0, every=few)
+    for cuts in (dict(), dict(top_k=40), dict(top_p=0.8), dict(top_k=700, top_p=0.9), dict(min_p=0.02), dict(temperature=0.0)):
+        check_sample(ctx, t, x, uniform=rng.random(rows), every=few, **cuts)
+    some = t.arange(0, rows, few, device="cuda")
+    tv, ti, lse = t.randn(rows, 60, device="cuda"), t.randint(0, cols, (rows, 60), device="cuda", dtype=t.int32), t.full((rows,), 6.0, device="cuda")
+    for rest in (None, lse):
+        loss, grad, stats = t.empty(rows, device="cuda"), t.empty_like(x), t.empty(rows, 4, device="cuda")
+        ctx.distill_rows(x, tv, ti, loss, grad=grad, stats=stats, teacher_lse=rest)
+        ctx.sync()
+        one = np.ones(some.numel())
+        part = lambda a: None if a is None else a[some]  # noqa: E731
+        check_gradient(numbers(grad[some]), x[some], tv[some], ti[some], part(rest), one, one, 1.0, kind)
+        for r in some.tolist():
+            want = distill(numbers(x[r]), numbers(tv[r]), ti[r].cpu().numpy(), None if rest is None else 6.0, 1.0, 1.0)[0]
+            assert abs(float(loss[r]) - want) <= 2 * SUM_ERROR + 2.0**-23 * abs(want)
+        grad.fill_(7.0)
+        ctx.distill_rows_backward(x, tv, ti, stats, None, grad, teacher_lse=rest)
+        ctx.sync()
+        check_gradient(numbers(grad[some]), x[some], tv[some], ti[some], part(rest), one, one, 1.0, kind)
+
+
+def test_calls_from_several_threads_and_contexts(accb, ctx, torch_cuda, rng):
+    t = torch_cuda
+    x = scores(t, rng, 200, 20011, "bfloat16")
+    u = t.from_numpy(rng.random(200).astype(np.float32)).cuda()
+    other = accb.Context(0)
+
+    def call(c, stream, values, index, lse, token, loss, grad):
+        for _ in range(10):
+            c.top_rows(x, values, index, lse=lse, stream=stream)
+            c.sample_rows(x, u, token, stream=stream)
+            c.distill_rows(x, values, index, loss, grad=grad, teacher_lse=lse, stream=stream)
+
+    def results():
+        return (t.empty(200, 30, dtype=x.dtype, device="cuda"), t.empty(200, 30, dtype=t.int32, device="cuda"), t.empty(200, device="cuda"),
+                t.empty(200, dtype=t.int32, device="cuda"), t.empty(200, device="cuda"), t.empty_like(x))
+
+    want, out, streams = results(), [results() for _ in range(4)], [t.cuda.Stream() for _ in range(4)]
+    call(ctx, None, *want)
+    t.cuda.synchronize()
+    threads = [threading.Thread(target=call, args=((ctx, other)[i % 2], streams[i].cuda_stream, *out[i])) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    t.cuda.synchronize()
+    for got in out:
+        assert all(t.equal(a, b) for a, b in zip(got, want))
+
+
+def test_device_arrays(accb, ctx, torch_cuda, rng):
+    """Memory that is not torch's, and a stream by number."""
+    t = torch_cuda
+    x = scores(t, rng, 5, 3000, "float16")
+    raw = lambda a, dtype: accb.DeviceArray(a.data_ptr(), a.shape, dtype)  # noqa: E731
+    values, index = t.empty(5, 7, dtype=t.float16, device="cuda"), t.empty(5, 7, dtype=t.int32, device="cuda")
+    t.cuda.synchronize()
+    ctx.top_rows(raw(x, np.float16), raw(values, np.float16), raw(index, np.int32), stream=0)
+    t.cuda.synchronize()
+    for r, row in enumerate(numbers(x)):
+        v, i, _ = top(row, 7, 1.0)
+        assert np.array_equal(numbers(values)[r], v) and np.array_equal(index[r].cpu().numpy(), i)
 
 
 def test_rows_of_more_lengths_than_are_remembered(ctx, torch_cuda, rng):
