@@ -223,6 +223,14 @@ __device__ __forceinline__ void peer_store(unsigned addr, u64 a, u64 b) { /* 16-
 __device__ __forceinline__ void peer_store1(unsigned addr, u64 a) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(a) : "memory");
 }
+__device__ __forceinline__ uint4 peer_load(unsigned addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ u64 peer_load1(unsigned addr) {
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
@@ -300,6 +308,7 @@ template <class T, bool RESIDENT> struct Share {
         in = (unsigned)max(0, (lead + cols) / E - in0);
         stage = smem;
     }
+    __device__ __forceinline__ int vectors() const { return (lead + n + E - 1) / E; } /* of the whole row */
     __device__ __forceinline__ int entry(int v) const { return v * E - lead; } /* index of a vector's first entry */
     __device__ __forceinline__ bool whole(int v) const { return (unsigned)(v - in0) < in; }
 

@@ -102,6 +102,7 @@ struct CutSpace {
     u64 list[kSampleRoom];
     PendingDraw pending;
     Extent extent;
+    alignas(16) u64 parts[kMaxCluster * kWarps][2]; /* weight above the border and entries on it, by part of the share */
 };
 struct NoCutSpace {
     Extent extent;
@@ -351,12 +352,71 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
         /* the first entry whose running sum exceeds uniform * total */
         const u64 target = drawn(uniform, total);
         if (!more) draw();
-        if (!(before <= target && target < before + here)) { /* in another block */
+        const bool here_in_block = before <= target && target < before + here;
+        int v0 = start;
+        const bool shared_search = CUTS && R && part.known && size > 1;
+        if constexpr (CUTS && R) {
+            if (shared_search) {
+                /* Bins do not say where the weight lies.  The blocks of the cluster look for it side by side in the share of
+                 * the block that holds the token, each in one part of every warp's piece. */
+                unsigned holder = 0;
+                u64 upto = 0;
+                ties_seen = 0;
+                for (unsigned i = 0; i < size; ++i) {
+                    const unsigned n = (unsigned)told.block[3][i][1], kept = min(ties_seen + n, border.ties) - min(ties_seen, border.ties);
+                    upto += told.block[3][i][0] + kept * tie_weight, ties_seen += n;
+                    holder += upto <= target;
+                }
+                const int per = share.per_block(p.in.cols, (int)size), piece = ((per + kWarps - 1) / kWarps + 31) & ~31;
+                const int turns = (piece / 32 + (int)size - 1) / (int)size; /* of 32 vectors, a part */
+                const int from0 = warp * piece, end = min(min(per, share.vectors() - (int)holder * per), from0 + piece);
+                const unsigned staged = peer_addr(shared_addr(stage), holder);
+                const float on = value_of(border.key), from = fmaxf(weigh.least, value_of(max(border.key, key_of(kLowest) - 1u) + 1u));
+                double sum = 0.0;
+                ties = 0;
+#pragma unroll 1
+                for (int i = from0 + 32 * turns * (int)rank; i < min(end, from0 + 32 * turns * ((int)rank + 1)); i += 32) {
+                    uint4 w = make_uint4(Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest, Elem<T>::kLowest);
+                    if (i + lane < end) w = peer_load(staged + 16 * (i + lane));
+                    float f[E];
+                    Elem<T>::unpack(w, f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) ties += f[e] == on;
+                    sum += weigh.some<E>(f, from, false);
+                }
+                const u64 mass = warp_sum((u64)sum);
+                ties = warp_sum(ties);
+                if (lane == 0) peer_store(peer_addr(shared_addr(&sh.parts[warp * size + rank][0]), holder), mass, ties);
+                cluster_sync(size);
+                if (here_in_block) {
+                    /* the part: two a lane */
+                    const int n = kWarps * (int)size, i0 = 2 * lane;
+                    u64 m[2];
+                    unsigned q[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) m[i] = i0 + i < n ? sh.parts[i0 + i][0] : 0, q[i] = i0 + i < n ? (unsigned)sh.parts[i0 + i][1] : 0;
+                    const unsigned seen = warp_scan(q[0] + q[1]) - q[1] - q[0], block_quota = quota;
+                    const unsigned k0 = min(seen, block_quota), k1 = min(seen + q[0], block_quota), k2 = min(seen + q[0] + q[1], block_quota);
+                    const u64 w0 = m[0] + (k1 - k0) * tie_weight, w1 = m[1] + (k2 - k1) * tie_weight;
+                    const u64 after = before + warp_scan(w0 + w1), first = after - w1 - w0;
+                    const unsigned found = __ballot_sync(~0u, target < after);
+                    const int l = __ffs(found) - 1; /* one of them: the block holds the token */
+                    const bool second = target >= first + w0;
+                    const int at = __shfl_sync(~0u, i0 + (int)second, l);
+                    before = __shfl_sync(~0u, second ? first + w0 : first, l);
+                    here = __shfl_sync(~0u, second ? w1 : w0, l);
+                    quota = __shfl_sync(~0u, second ? k2 - k1 : k1 - k0, l);
+                    if (at / (int)size != warp) here = 0;
+                    v0 = start + 32 * turns * (at % (int)size);
+                }
+            }
+        }
+        if (!here_in_block) { /* in another block */
             next();
             continue;
         }
-        if (!passed) pass(border, false);
-        {
+        if (!shared_search) {
+            if (!passed) pass(border, false);
             const u64 mass = warp_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]));
             const unsigned n = warp_sum(ties);
             if (lane == 0) warp_part[warp][0] = mass, warp_part[warp][1] = n;
@@ -376,8 +436,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
             continue;
         }
 
-        int v0 = start;
-        if (quota == 0) { /* which quarter of the warp's piece */
+        if (!shared_search && quota == 0) { /* which quarter of the warp's piece */
 #pragma unroll
             for (int q = 0; q < 3; ++q) {
                 const u64 w = warp_sum(quarter[q]);
