@@ -528,8 +528,12 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
             return find_border<T, RESIDENT, true>(share, lv, size, key_of(from), key_of(most), 0, weigh, top_p, 0);
         }
         Border border{key_of_bin<EXACT>(order, bin, false), (unsigned)(k - before), equals};
-        if (!EXACT || bin == middle || bin == last)
+        if (!EXACT || bin == middle || bin == last) {
             border = find_border<T, RESIDENT, false>(share, lv, size, order.lowest(bin) << 16, order.highest(bin) << 16 | 0xffffu, k - before, weigh, 0.0, 0);
+        } else if (!(top_p < 1.0)) {
+            part.mass = weight_before(bins, order, weigh, own_coarse, bin), part.ties = bins.count[bin], part.known = true;
+            __syncthreads();
+        }
         if (!(top_p < 1.0)) return border;
         const Border b = find_border<T, RESIDENT, true>(share, lv, size, border.key, key_of(most), 0, weigh, top_p, border.equals - border.ties);
         return b.ties != 0xffffffffu ? b : border;
