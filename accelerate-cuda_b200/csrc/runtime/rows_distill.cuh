@@ -71,7 +71,7 @@ __device__ __noinline__ float row_loss(const RowSums &all, double named, double 
  * Loss and gradient of 4096 x 131072 bf16, 64 named, with the rest: 524 us, 4.0 TB/s, 61 % of the copy rate; the special
  * function unit, two exponentials an entry, is busy for 47 % and the row's chain of steps is the rest.  The loss alone of
  * 2048 x 50257 floats: 122 us, half of the copy rate.  The gradient from statistics needs no exchange and is bound by HBM
- * (1024 x 131072 bf16 at 96 % of the copy rate); where rows start anywhere, as 1500 x 100003 fp16 do, 105 us, 86 %.
+ * (1024 x 131072 bf16 at 96 % of the copy rate); where rows start anywhere, as 1500 x 100003 fp16 do, 107 us, 84 %.
  * One row per cluster: clusters that stay and fetch the next row in the place of this one, vector by vector behind
  * the gradient pass, took 560 us; 2 blocks an SM the same as 3, blocks of 128, 384, 512 and
  * 1024 threads more.

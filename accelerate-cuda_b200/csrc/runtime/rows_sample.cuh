@@ -114,11 +114,12 @@ struct NoCutSpace {
  *   top_k, or top_p with few candidates   a bound as in top_rows, or from the row's weight: what lies more than
  *                    log(cols / (1 - top_p)) below the maximum weighs less than what is cut off.  One block lists, sorts
  *                    and draws, the blocks of a cluster by turns
- *   others           the border by counting bins (border_by_bins), then as without cuts above it
+ *   others           the border by counting bins (border_by_bins), then as without cuts above it; where the bins also say
+ *                    what every block holds (bfloat16), only the share with the token is looked through, by all blocks
  * Clusters stay for row after row, as in top_rows.
  *
  * 1024 x 131072 bf16: without cuts 237 us (1.1 TB/s, 17 % of the copy rate), issue slots 57 % and the 64-bit
- * pipe 32 % busy: eight operations a weight; the best entry 70 us (58 %), top_k 50 146 us, top_p 0.9 of rows without a peak 704 us, min_p 0.05 136 us.
+ * pipe 32 % busy: eight operations a weight; the best entry 70 us (58 %), top_k 50 146 us, top_k 400 415 us, top_p 0.9 525 us, min_p 0.05 136 us.
  * Weights in 32 bits with a bound on their error, and again in 64 where the bound could not tell two indices apart, took
  * 343 us: with a hundred thousand like entries it seldom can.
  *
