@@ -389,8 +389,10 @@ template <class T, bool RESIDENT> struct Row : Share<T, RESIDENT> {
 #pragma unroll
         for (int i = 0; i < Elem<T>::E; ++i) f[i] = not_nan(f[i]);
     }
+    /* by all lanes of a warp, which see one another's vectors changed afterwards: gather() reads them */
     __device__ __forceinline__ void apply() const {
         for (int v = RESIDENT ? this->first : this->last; v < this->last; v += 32) this->stage[v - this->v0] = changed(v, this->get(v));
+        __syncwarp();
     }
 };
 

@@ -284,6 +284,25 @@ def test_sample_rows_with_little_in_them(ctx, torch_cuda, rng, kind):
         check_sample(ctx, t, place(t, x, kind), uniform=rng.random(8), **cuts)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols", [300, 9001, 100003])
+def test_sample_infinite_scores_among_others(ctx, torch_cuda, rng, kind, cols):
+    """Rows whose best scores are +inf, a few in one place or one in most threads' vectors: what the staged scores are
+    replaced by is listed by other lanes of the warp than the ones that replaced it."""
+    rows, every = 40, 1 if cols < 5000 else 3 if cols < 50000 else 7
+    x = rng.normal(0, 2, (rows, cols)).astype(np.float32)
+    for r in range(rows):
+        n = (1, 2, 3, 20, 150)[r % 5]
+        at = rng.choice(cols, n, replace=False) if r % 2 else rng.integers(0, cols - n + 1) + np.arange(n)
+        x[r, at] = np.inf
+    x = place(torch_cuda, x, kind, cols + 1, 1)
+    allowed = rng.random((rows, cols)) < 0.7
+    for cuts in (dict(top_k=1), dict(top_k=2), dict(top_k=30), dict(top_k=190), dict(top_k=400), dict(top_k=5, top_p=0.7), dict(top_p=0.5),
+                 dict(top_k=9, temperature=0.0), dict(top_k=50, min_p=0.5), dict(top_k=50, temperature=1e5)):
+        check_sample(ctx, torch_cuda, x, uniform=rng.random(rows), every=every, **cuts)
+        check_sample(ctx, torch_cuda, x, allowed, uniform=rng.random(rows), every=every, **cuts)
+
+
 def test_sample_random_numbers_at_the_ends(ctx, torch_cuda, rng):
     t = torch_cuda
     x = scores(t, rng, 6, 5000, "float32")
