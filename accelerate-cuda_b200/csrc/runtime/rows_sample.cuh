@@ -61,7 +61,7 @@ static __device__ __noinline__ void draw_from_list(const SampleParams &p, const 
     for (int i = from; i < to; ++i) mine += weigh.weight(score_of(list[i]));
     u64 upto = block_scan(mine, scratch);
     if (total == 0) total = block_sum(mine, scratch);
-    const u64 limit = top_p < 1.0f ? (u64)ceil((top_p > 0.0f ? (double)top_p : 0.0) * (double)total) : ~0ull;
+    const u64 limit = top_p < 1.0f ? (u64)ceil((double)top_p * (double)total) : ~0ull;
     u64 before = upto - mine, kept = 0;
     for (int i = from; i < to; ++i) {
         const float x = score_of(list[i]);
@@ -170,7 +170,8 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
         share.infinite = false;
         const float warmth = p.temperature ? p.temperature[row] : 1.0f;
         int k = CUTS && p.top_k ? p.top_k[row] : 0;
-        const float top_p = CUTS && p.top_p ? p.top_p[row] : 1.0f;
+        float top_p = CUTS && p.top_p ? p.top_p[row] : 1.0f;
+        if (top_p < 0.0f) top_p = 0.0f; /* the first entry, as 0; a NaN stays, and is off */
         const float min_p = p.min_p ? p.min_p[row] : 0.0f;
         const float uniform = p.uniform[row];
         if (!(warmth > 0.0f)) k = 1;
@@ -287,7 +288,8 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
                 if (k == 0) { /* top_p alone */
                     least = weigh.least;
                     /* counts by bin say what a row of bfloat16 weighs; else, or where min_p leaves few to list, a pass
-                     * does, and how far down entries lie that all of them together weigh less than what is cut off */
+                     * does, and how far down entries lie that all of them together weigh less than what is cut off: below
+                     * the maximum, since that is at most all of the weight, and the weight at most `cols` times the maximum's */
                     if (Elem<T>::kShift != 16 || min_p > 0.0f) {
                         pass(border, true);
                         const u64 block_total = block_sum((quarter[0] + quarter[1]) + (quarter[2] + quarter[3]), scratch);
@@ -326,7 +328,7 @@ template <class T, bool R, bool CUTS> __global__ void __launch_bounds__(kThreads
                 /* too many for a list */
                 border = k == 1 ? Border{key_of(most), 1, 1}
                                 : border_by_bins<T, R>(share, sh.bins, sh.level, size, weigh, k > 0 || Elem<T>::kShift != 16 ? least : weigh.least, most,
-                                                       (u64)k, top_p < 1.0f ? (top_p > 0.0f ? (double)top_p : 0.0) : 1.0, total, part);
+                                                       (u64)k, top_p < 1.0f ? (double)top_p : 1.0, total, part);
                 const unsigned below = key_of(lowest) - 1u;
                 if (below >= border.key) border = Border{below, 0, 0}, part.known = false;
             }

@@ -303,6 +303,20 @@ def test_sample_infinite_scores_among_others(ctx, torch_cuda, rng, kind, cols):
         check_sample(ctx, torch_cuda, x, allowed, uniform=rng.random(rows), every=every, **cuts)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("top_p", [-0.02, -1.0, -1e30, -np.inf, -0.0])
+def test_sample_a_negative_share_takes_the_first(ctx, torch_cuda, rng, kind, top_p):
+    """As 0 does, however negative: of rows of one entry, of equal ones, of any at a great temperature."""
+    t = torch_cuda
+    for cols in (1, 5, 4096, 100003):
+        x = rng.normal(0, 2, (6, cols)).astype(np.float32)
+        x[:2] = 1.5
+        x[2] = np.round(x[2])
+        for rest in (dict(), dict(temperature=np.inf), dict(temperature=0.01), dict(min_p=0.1), dict(min_p=1e-3, temperature=1e6), dict(top_k=3),
+                     dict(top_k=1000)):
+            check_sample(ctx, t, place(t, x, kind), uniform=rng.random(6), top_p=top_p, **rest)
+
+
 def test_sample_random_numbers_at_the_ends(ctx, torch_cuda, rng):
     t = torch_cuda
     x = scores(t, rng, 6, 5000, "float32")
