@@ -471,7 +471,7 @@ struct Weigh {
     }
     /* log of the weight of the maximum, in units */
     __device__ __forceinline__ double log_of_top() const { return fma((double)top, c, start - kRound) * (0.69314718055994531 / kTable); }
-    /* for f >= least; anything below */
+    /* for least <= f <= top; anything elsewhere */
     __device__ __forceinline__ u64 of(float f) const { return (u64)__double_as_longlong(above_2_52(f)) & 0xfffffffffffffull; }
     /* 2^52 + the weight */
     __device__ __forceinline__ double above_2_52(float f) const {

@@ -477,7 +477,8 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
         if (bin == middle) return coarse[0];
         if (bin == last) return coarse[1];
         const u64 n = counted(bin);
-        return n ? n * weigh.weight(value_of(key_of_bin<EXACT>(order, bin, high))) : 0;
+        /* the maximum's bin ends above the maximum, where scores have no weight */
+        return n ? n * weigh.weight(fminf(value_of(key_of_bin<EXACT>(order, bin, high)), weigh.top)) : 0;
     };
     /* the first bin up to which the sum of `of` reaches what `goal` makes of the whole sum, or -1; what precedes it.
      * Search 0 and 1 of a call. */

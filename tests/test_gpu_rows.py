@@ -317,6 +317,37 @@ def test_sample_a_negative_share_takes_the_first(ctx, torch_cuda, rng, kind, top
             check_sample(ctx, t, place(t, x, kind), uniform=rng.random(6), top_p=top_p, **rest)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("top", [1000.0, 30.0, 2.0, 1.0, -1.0, -20.0])
+@pytest.mark.parametrize("min_p", [0.0, 1e-6])
+def test_sample_shares_of_cold_rows_with_many_best(ctx, torch_cuda, rng, kind, top, min_p):
+    """Hundreds of entries with each of the few best values, so that no list holds them, and temperatures at which the
+    values next to one another weigh very differently: what a bin may weigh at most is not taken from scores above the
+    row's largest."""
+    t = torch_cuda
+    rows, cols = 48, 20011
+    step = abs(top) * {"float32": 1e-5, "float16": 2.0**-9, "bfloat16": 2.0**-6}[kind]
+    x = rng.normal(top - 40 * step, 5 * step, (rows, cols)).astype(np.float32)
+    x = np.minimum(x, np.float32(top - 20 * step))
+    for r in range(rows):
+        at = rng.permutation(cols)
+        for i, v in enumerate((top, top - step * rng.uniform(0.5, 3), top - step * rng.uniform(3, 6))):
+            x[r, at[700 * i:700 * i + 600]] = v
+    x = place(t, x, kind)
+    temperature = step * 10.0 ** rng.uniform(-1.5, 1.5, rows)
+    check_sample(ctx, t, x, uniform=rng.choice([0.0, 0.5, 0.999], rows), temperature=temperature, top_p=rng.uniform(0.05, 0.95, rows),
+                 min_p=np.full(rows, min_p))
+
+
+def test_sample_a_share_of_equal_scores_above_others(ctx, torch_cuda):
+    """600 scores of 1000 and 600 just below, cold: a share of 0.3 keeps 187 of the first."""
+    t = torch_cuda
+    x = np.zeros((1, 4096), np.float32)
+    x[0, :600], x[0, 600:1200] = 1000.0, 999.99
+    for u in (0.0, 0.5, 0.999):
+        check_sample(ctx, t, place(t, x, "float32"), uniform=u, temperature=0.003, top_p=0.3)
+
+
 def test_sample_random_numbers_at_the_ends(ctx, torch_cuda, rng):
     t = torch_cuda
     x = scores(t, rng, 6, 5000, "float32")
