@@ -593,9 +593,13 @@ class Context:
             raise AccbError(EINVAL, f"{name}: shape {tuple(t.shape)}, not {shape}")
         if isinstance(t, DeviceArray):
             return t.ptr
-        if not t.is_contiguous():
+        try:
+            contiguous, device = t.is_contiguous(), t.get_device()
+        except AttributeError:
+            raise TypeError(f"{name}: not a device array: {type(t)!r}") from None
+        if not contiguous:
             raise AccbError(EINVAL, f"{name}: not contiguous")
-        if t.get_device() != self.device:
+        if device != self.device:
             raise AccbError(EINVAL, f"{name}: on {t.device}, not on cuda:{self.device}")
         return t.data_ptr()
 
@@ -611,12 +615,26 @@ class Context:
             raise AccbError(EINVAL, f"{name}: rows of {cols} entries")
         if isinstance(t, DeviceArray):
             return accb_rows_array(t.ptr, ROWS_TYPES[kind], cols, rows, cols)
-        pitch, inner = t.stride()
+        try:
+            (pitch, inner), device = t.stride(), t.get_device()
+        except AttributeError:
+            raise TypeError(f"{name}: not a device array: {type(t)!r}") from None
         if cols > 1 and inner != 1:
             raise AccbError(EINVAL, f"{name}: the entries of a row are not contiguous")
-        if t.get_device() != self.device:
+        if device != self.device:
             raise AccbError(EINVAL, f"{name}: on {t.device}, not on cuda:{self.device}")
         return accb_rows_array(t.data_ptr(), ROWS_TYPES[kind], cols, rows, pitch if rows > 1 else cols)
+
+    @staticmethod
+    def _columns(name, t) -> int:
+        """Entries per row of an argument that must be a matrix."""
+        try:
+            shape = t.shape
+        except AttributeError:
+            raise TypeError(f"{name}: not a device array: {type(t)!r}") from None
+        if len(shape) != 2:
+            raise AccbError(EINVAL, f"{name}: rank {len(shape)}, not 2")
+        return int(shape[1])
 
     def _own_stream(self, stream):
         """The given stream, or the current one of this context's device."""
@@ -627,9 +645,7 @@ class Context:
         are: ``values`` and ``index`` have shape rows x k.  ``lse``: log-sum-exp of the whole row at ``temperature``.
         See ``accb_top_rows`` in ``include/accb200.h``."""
         a = self._rows("x", x)
-        if len(values.shape) != 2:
-            raise AccbError(EINVAL, f"values: rank {len(values.shape)}, not 2")
-        k = int(values.shape[1])
+        k = self._columns("values", values)
         v = self._address("values", values, (_element_type(x),), (a.rows, k))
         i = self._address("index", index, ("int32",), (a.rows, k))
         s = self._address("lse", lse, ("float32",), (a.rows,))
@@ -651,9 +667,7 @@ class Context:
         _check(lib().accb_sample_rows(self.handle, self._own_stream(stream), a, bits, words, *each), self.handle)
 
     def _teacher(self, a, teacher, index, teacher_lse, weight):
-        if len(teacher.shape) != 2:
-            raise AccbError(EINVAL, f"teacher: rank {len(teacher.shape)}, not 2")
-        k = int(teacher.shape[1])
+        k = self._columns("teacher", teacher)
         t = self._address("teacher", teacher, ROWS_TYPES, (a.rows, k))
         i = self._address("index", index, ("int32",), (a.rows, k))
         s = self._address("teacher_lse", teacher_lse, ("float32",), (a.rows,))

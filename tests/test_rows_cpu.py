@@ -63,6 +63,24 @@ def test_tensors_elsewhere_are_refused(accb, context):
     assert "contiguous" in refused(accb, context.sample_rows, torch.zeros(100, 3).T, torch.zeros(3), torch.zeros(3, dtype=torch.int32))
 
 
+def test_what_is_no_device_array_is_refused(accb, context):
+    """Host arrays and things that are no arrays at all, in every place: a refusal, not an error from within."""
+    a = lambda *shape, kind=np.float32: array(accb, *shape, kind=kind)  # noqa: E731
+    i32 = np.int32
+    calls = [(context.top_rows, dict(x=a(3, 100), values=a(3, 5), index=a(3, 5, kind=i32), lse=a(3))),
+             (context.sample_rows, dict(x=a(3, 100), uniform=a(3), token=a(3, kind=i32), logprob=a(3), temperature=a(3), top_k=a(3, kind=i32),
+                                        top_p=a(3), min_p=a(3), allowed=a(3, 4, kind=i32))),
+             (context.distill_rows, dict(student=a(3, 100), teacher=a(3, 5), index=a(3, 5, kind=i32), loss=a(3), grad=a(3, 100), stats=a(3, 4),
+                                         teacher_lse=a(3), weight=a(3))),
+             (context.distill_rows_backward, dict(student=a(3, 100), teacher=a(3, 5), index=a(3, 5, kind=i32), stats=a(3, 4), upstream=a(3),
+                                                  grad=a(3, 100), teacher_lse=a(3), weight=a(3)))]
+    for call, good in calls:
+        for name, value in good.items():
+            for other in (np.zeros(value.shape, value.dtype), [[1.0] * 5] * 3, 3.0):
+                with pytest.raises(TypeError, match="not a device array"):
+                    call(**{**good, name: other}, stream=0)
+
+
 def test_entry_points_refuse_a_null_context(accb):
     L = accb.lib()
     a = C.byref(accb.accb_rows_array(1 << 20, 0, 8, 1, 8))
