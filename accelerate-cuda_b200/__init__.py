@@ -288,16 +288,19 @@ _stream_of = None
 
 def _current_stream():
     """The function that gives a device's current stream as a number: torch's own, without the object around it where
-    torch offers that; 0 without torch."""
+    torch offers that; 0 without torch, or beside a torch that has no GPU."""
     global _stream_of
     if _stream_of is None:
         try:
             import torch
+            found = torch.cuda.is_available()
         except ImportError:
-            _stream_of = lambda device: 0  # noqa: E731
-        else:
+            found = False
+        if found:
             _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
                 lambda device: torch.cuda.current_stream(device).cuda_stream)
+        else:
+            _stream_of = lambda device: 0  # noqa: E731
     return _stream_of
 
 

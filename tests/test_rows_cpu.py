@@ -81,6 +81,16 @@ def test_what_is_no_device_array_is_refused(accb, context):
                     call(**{**good, name: other}, stream=0)
 
 
+def test_without_a_stream_where_torch_has_no_gpu(accb, context, monkeypatch):
+    """Memory that is not torch's, beside a torch that has no GPU: the default stream, as for every other launch."""
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    monkeypatch.setattr(accb, "_stream_of", None)
+    a = lambda *shape, kind=np.float32: array(accb, *shape, kind=kind)  # noqa: E731
+    assert context._own_stream(None) == 0
+    assert "null context" in refused(accb, context.top_rows, a(3, 100), a(3, 5), a(3, 5, kind=np.int32))
+
+
 def test_entry_points_refuse_a_null_context(accb):
     L = accb.lib()
     a = C.byref(accb.accb_rows_array(1 << 20, 0, 8, 1, 8))
