@@ -277,7 +277,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
             if (excluded) said = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (lane == 0) statistics = said;
             if (rank == 0) {
-                all.cross = warp_sum(all.cross) - named_p * shift;
+                all.cross = warp_sum(all.cross) - (named_p != 0.0 ? named_p * shift : 0.0); /* of an infinite shift nothing is named */
                 const float loss = excluded ? 0.0f : row_loss(all, named_p, rest ? 1.0 : total, r, inv);
                 if (lane == 0) {
                     p.loss[row] = weight * loss;

@@ -604,6 +604,15 @@ def test_distill_nan_in_a_row_that_counts(ctx, torch_cuda, rng):
         assert grad[:2].isnan().all() and not grad[2].isnan().any()
 
 
+def test_distill_a_teacher_whose_weight_is_all_elsewhere(ctx, torch_cuda, rng):
+    """teacher_lse of +inf, or far above the scores: the named entries have no probability and the rest has it all."""
+    t = torch_cuda
+    x = scores(t, rng, 3, 1000, "float32")
+    tv, ti, lse = teacher_of(t, rng, x, 5, "float32", 1.0, True)
+    lse[0], lse[1] = float("inf"), 1e30
+    check_distill(ctx, t, rng, x, 5, teacher=(tv, ti, lse), weight=np.ones(3, np.float32))
+
+
 @pytest.mark.parametrize("rest", [False, True])
 def test_distill_gradient_against_differences(ctx, torch_cuda, rng, rest):
     """Central differences of the loss, 32 bits: h = 2^-3, the third derivative of a log-sum-exp is below 1, so the
