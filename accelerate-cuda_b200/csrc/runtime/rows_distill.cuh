@@ -33,7 +33,7 @@ struct Named {
     float score; /* of the teacher */
     float z;     /* of the student, if the entry lies in this block's share */
     int at;      /* index, or -1 for an entry that names nothing or lies in another share */
-    int first;   /* the first of its index that was met */
+    int first;   /* the first of its index in the list */
 };
 
 /* Where the best of the entries not named is less likely than this share of the row's best, the statistics hold the
@@ -188,6 +188,16 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
         n.at = here ? at : -1;
     }
     __syncthreads();
+    if (!BACKWARD && twice) { /* not whichever thread came first: sums are taken in the order of the list */
+        most_named = neg_inf();
+        for (int j = threadIdx.x; j < p.k; j += kThreads) {
+            Named &n = named[j];
+            bool first = n.at >= 0;
+            for (int o = 0; o < j && first; ++o) first = named[o].at != n.at;
+            n.first = first;
+            if (first) most_named = fmaxf(most_named, n.z);
+        }
+    }
 
     if (!BACKWARD) {
         /* the rest of the row (all of it without teacher_lse) and the named entries, each as maximum and sum */

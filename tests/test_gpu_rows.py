@@ -613,6 +613,23 @@ def test_distill_a_teacher_whose_weight_is_all_elsewhere(ctx, torch_cuda, rng):
     check_distill(ctx, t, rng, x, 5, teacher=(tv, ti, lse), weight=np.ones(3, np.float32))
 
 
+@pytest.mark.parametrize("cols", [3000, 131072])
+def test_distill_of_entries_named_twice_is_the_same_every_time(ctx, torch_cuda, rng, cols):
+    """Whichever thread meets an index first, the sums are taken in one order."""
+    t = torch_cuda
+    rows, k = 600, 768
+    x = scores(t, rng, rows, cols, "float32" if cols < 5000 else "bfloat16")
+    ti = t.from_numpy(rng.integers(0, min(cols, 300), (rows, k)).astype(np.int32)).cuda()
+    x[:, :300] += t.from_numpy(rng.uniform(5, 30, (rows, 300)).astype(np.float32)).cuda()  # what is named has most of the weight
+    tv, lse = t.randn(rows, k, device="cuda"), t.full((rows,), 9.0, device="cuda")
+    new = lambda: (t.empty(rows, device="cuda"), t.empty_like(x), t.empty(rows, 4, device="cuda"))  # noqa: E731
+    want, got = new(), new()
+    for i in range(40):
+        loss, grad, stats = got if i else want
+        ctx.distill_rows(x, tv, ti, loss, grad=grad, stats=stats, teacher_lse=lse)
+        assert all(t.equal(a, b) for a, b in zip(got, want)) if i else True
+
+
 @pytest.mark.parametrize("rest", [False, True])
 def test_distill_gradient_against_differences(ctx, torch_cuda, rng, rest):
     """Central differences of the loss, 32 bits: h = 2^-3, the third derivative of a log-sum-exp is below 1, so the
