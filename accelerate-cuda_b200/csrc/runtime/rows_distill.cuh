@@ -41,11 +41,47 @@ struct Named {
  * of 32 bits.  Marked by a negative second number; top, -1 / sum, others_top, factor of exp((x - others_top) / tau). */
 constexpr float kApart = 2.328306437e-10f; /* 2^-32 */
 
+/* exp((a - b) / tau) for a <= b; inverse = 1 / tau, c = log2(e) / tau.  With k the whole number next to its exponent to
+ * base two, 2^k times the Taylor polynomial of degree 9 of x = (a - b) / tau - k ln 2, |x| < 0.347.  64-bit operations are
+ * what it waits for, so the terms from x^5 on, 5e-5 at most, are added up in 32 bits: wrong by less than 2^-32 of itself
+ * (ten roundings of 2^-24 of 5e-5, and 0.347^10 / 10! = 7e-12, over exp(x) >= 0.7).  For terms that are not one of many:
+ * the special function unit's error of 2^-22 of a named entry, which may have most of the row's weight, would be the
+ * loss's (1024 x 131072 bf16, loss 0.06: off by 6e-8 root mean square, with these 2e-9, at 531 us a step over 4096 such
+ * rows in place of 525). */
+__device__ __forceinline__ double exp_below(float a, float b, double inverse, float c) {
+    const float y = (a - b) * c;
+    const int k = __float2int_rn(y);
+    const double x = fma((double)a - (double)b, inverse, (double)k * -0.69314718055994531), x2 = x * x;
+    const float s = (float)x, s2 = s * s;
+    float rest = fmaf(1.0f / 362880.0f, s, 1.0f / 40320.0f);
+    rest = fmaf(rest, s, 1.0f / 5040.0f);
+    rest = fmaf(rest, s, 1.0f / 720.0f);
+    rest = fmaf(rest, s, 1.0f / 120.0f);
+    rest *= s2 * s2 * s;
+    const double e = fma(fma(1.0 / 24.0, x2, fma(1.0 / 6.0, x, 0.5)), x2, 1.0 + x) + (double)rest;
+    /* a NaN stays one, at k = 0 */
+    return y < -1000.0f ? 0.0 : __hiloint2double(__double2hiint(e) + (k << 20), __double2loint(e));
+}
+
 /* The row as all its blocks know it. */
 struct RowSums {
     float top, others_top;         /* maximum of the row, and of the entries not named (-inf: none) */
     double sum, others_sum, cross; /* sums of exponentials below those maxima; sum of p (teacher's - student's score) / tau */
 };
+
+/* Where an index is named twice: not whichever thread came first but the first in the list counts, so that sums are taken
+ * in one order.  Returns the largest of the student's scores of this thread's. */
+static __device__ __noinline__ float settle_firsts(Named *named, int k) {
+    float most = neg_inf();
+    for (int j = threadIdx.x; j < k; j += kThreads) {
+        Named &n = named[j];
+        bool first = n.at >= 0;
+        for (int o = 0; o < j && first; ++o) first = named[o].at != n.at;
+        n.first = first;
+        if (first) most = fmaxf(most, n.z);
+    }
+    return most;
+}
 
 /* What the loss is computed from, by one warp of the row: its logarithms are taken by four lanes at once. */
 __device__ __noinline__ float row_loss(const RowSums &all, double named, double teacher_sum, double rest, double inv) {
@@ -188,16 +224,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
         n.at = here ? at : -1;
     }
     __syncthreads();
-    if (!BACKWARD && twice) { /* not whichever thread came first: sums are taken in the order of the list */
-        most_named = neg_inf();
-        for (int j = threadIdx.x; j < p.k; j += kThreads) {
-            Named &n = named[j];
-            bool first = n.at >= 0;
-            for (int o = 0; o < j && first; ++o) first = named[o].at != n.at;
-            n.first = first;
-            if (first) most_named = fmaxf(most_named, n.z);
-        }
-    }
+    if (!BACKWARD && twice) most_named = settle_firsts(named, p.k);
 
     if (!BACKWARD) {
         /* the rest of the row (all of it without teacher_lse) and the named entries, each as maximum and sum */
@@ -223,6 +250,8 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
         typename Elem<T>::Max largest;
 #pragma unroll 4
         for (int v = share.first; v < share.last; v += 32) largest.add(get(v));
+        /* exponents and exponentials of the many in 32 bits, added up by thread and warp in 32 and from there in 64: their
+         * errors, 2^-22 of a term, average out (c in two parts brought the loss no closer: 8e-8 off, with one 6e-8, 1.3 large) */
         const float most = warp_max(largest.get()), base = most > neg_inf() ? most : 0.0f;
         const Pair less(-base, -base), by(c, c);
         Pair part[2] = {Pair(0.0f, 0.0f), Pair(0.0f, 0.0f)};
@@ -241,7 +270,7 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
                 most_named = warp_max(most_named);
                 const float named_base = most_named > neg_inf() ? most_named : 0.0f;
                 for (int j = threadIdx.x; j < p.k; j += kThreads)
-                    if (named[j].first) named_sum += (double)fast_exp2((named[j].z - named_base) * c);
+                    if (named[j].first) named_sum += exp_below(named[j].z, named_base, inv, c);
                 named_sum = warp_sum(named_sum);
             }
             cross = warp_sum(cross);
@@ -269,21 +298,22 @@ template <class T, bool R, bool BACKWARD> __global__ void __launch_bounds__(kThr
                 /* a sum that is 0 belongs to no entry; one that is not, at a maximum of -inf, to entries that are NaN */
                 const double a = __longlong_as_double((long long)told[i][0]), b = __longlong_as_double((long long)told[i][1]);
                 const float at_a = __uint_as_float((unsigned)(told[i][3] >> 32)), at_b = __uint_as_float((unsigned)told[i][3]);
-                if (a != 0.0) all.others_sum += a * (double)fast_exp2((at_a - all.others_top) * c);
-                if (b != 0.0) all.sum += b * (double)fast_exp2((at_b - all.top) * c);
+                const double of_a = exp_below(at_a, all.others_top, inv, c), of_b = exp_below(at_b, all.top, inv, c);
+                if (a != 0.0) all.others_sum += a * of_a;
+                if (b != 0.0) all.sum += b * of_b;
                 all.cross += __longlong_as_double((long long)told[i][2]);
             }
             all.others_sum = warp_sum(all.others_sum);
             if (rest) all.sum = warp_sum(all.sum);
-            const float down = rest ? fast_exp2((all.others_top - all.top) * c) : 1.0f; /* from one maximum to the other */
-            if (all.others_sum != 0.0) all.sum += all.others_sum * (double)down;
+            const double down = rest ? exp_below(all.others_top, all.top, inv, c) : 1.0; /* from one maximum to the other */
+            if (all.others_sum != 0.0) all.sum += all.others_sum * down;
             const bool excluded = all.top == neg_inf() && all.sum == 0.0; /* by the student, every entry */
             double r = rest && all.others_top > neg_inf() ? fmax(0.0, 1.0 - named_p) : 0.0;
             float4 said = make_float4(all.top, (float)(1.0 / all.sum), (float)(named_p + r), (float)(named_p + r));
             if (r > 0.0 && down >= kApart)
-                said.w = (float)(named_p + r - r * (all.sum / all.others_sum / (double)down));
+                said.w = (float)(named_p + r - r * (all.sum / all.others_sum / down));
             else if (r > 0.0)
-                said = make_float4(all.top, -said.y, all.others_top, (float)((named_p + r) * (double)said.y * (double)down - r / all.others_sum));
+                said = make_float4(all.top, -said.y, all.others_top, (float)((named_p + r) * (double)said.y * down - r / all.others_sum));
             if (excluded) said = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (lane == 0) statistics = said;
             if (rank == 0) {

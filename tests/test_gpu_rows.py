@@ -630,6 +630,39 @@ def test_distill_of_entries_named_twice_is_the_same_every_time(ctx, torch_cuda, 
         assert all(t.equal(a, b) for a, b in zip(got, want)) if i else True
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("cols,temperature", [(3001, 1.0), (32768, 0.7), (131072, 1.0)])
+def test_distill_a_loss_near_agreement(ctx, torch_cuda, rng, kind, cols, temperature):
+    """A student that is nearly its teacher, so that the loss is the difference of like numbers: log q of the named entries
+    and of the rest, near 0 both.  What is named has at least 0.9 of the weight.  Its exponentials and those that join the
+    sums are off by less than 2^-31 each, a sum of the others, x of the weight, by 2^-22 of a term plus 128 additions of a thread, half a
+    step each, 2^-17 at most, and scale^-1 in 32 bits (2^-24 of an exponent of at most 30): x (2^-22 + 2^-17 + 2^-19) at
+    most.  The loss is r log r - r log q_r + sum p (log p - log q): an error d of the others' sum moves log q by x d and log
+    q_r by d (1 - x), so the loss by about |x - r| d, and r and x are alike within a tenth of 0.1; and it is rounded once."""
+    t = torch_cuda
+    rows, k = 24, 40
+    x = rng.normal(0, 1, (rows, cols)).astype(np.float32)
+    at = np.stack([rng.choice(cols, k, replace=False) for _ in range(rows)]).astype(np.int32)
+    np.put_along_axis(x, at, rng.uniform(14, 18, (rows, k)).astype(np.float32) * temperature, 1)
+    x = place(t, x, kind)
+    z = numbers(x)
+    teacher = z + rng.normal(0, 0.01, z.shape)
+    tv = t.from_numpy(np.take_along_axis(teacher, at, 1)).float().cuda()
+    lse = t.from_numpy(np.array([np.log(np.exp(row / temperature).sum()) for row in teacher])).float().cuda()
+    ti, loss = t.from_numpy(at).cuda(), t.empty(rows, device="cuda")
+    ctx.distill_rows(x, tv, ti, loss, teacher_lse=lse, temperature=temperature)
+    ctx.sync()
+    for r in range(rows):
+        want = distill(z[r], numbers(tv)[r], at[r], float(lse[r]), 1.0, temperature)[0]
+        named = np.exp(z[r][at[r]] / temperature).sum()
+        share = 1 - named / np.exp(z[r] / temperature).sum()
+        rest = max(0.0, 1 - np.exp(numbers(tv)[r] / temperature - float(lse[r])).sum())
+        assert share < 0.1
+        d = 2.0**-22 + 2.0**-17 + 2.0**-19
+        allowance = abs(share - rest) * d + 2.0**-30 + 2.0**-24 * abs(want)
+        assert abs(float(loss[r]) - want) <= allowance, (r, float(loss[r]), want, allowance)
+
+
 @pytest.mark.parametrize("rest", [False, True])
 def test_distill_gradient_against_differences(ctx, torch_cuda, rng, rest):
     """Central differences of the loss, 32 bits: h = 2^-3, the third derivative of a log-sum-exp is below 1, so the
