@@ -39,7 +39,9 @@ __device__ __forceinline__ void put_token(const SampleParams &p, long long row, 
     p.token[row] = index;
     if (p.logprob) {
         const double below = value == weigh.top ? 0.0 : ((double)value - (double)weigh.top) / temperature;
-        p.logprob[row] = (float)(below - (log_64((double)total * (1.0 / (double)(1ull << kUnitLog2))) - weigh.log_of_top()));
+        /* the total as a multiple of the maximum's weight as it was added up, which is among what is kept: 0 for the only
+         * entry, and never above */
+        p.logprob[row] = (float)(below - log_64((double)total / (double)weigh.of(weigh.top)));
     }
 }
 

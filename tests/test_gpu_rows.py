@@ -348,6 +348,28 @@ def test_sample_a_share_of_equal_scores_above_others(ctx, torch_cuda):
         check_sample(ctx, t, place(t, x, "float32"), uniform=u, temperature=0.003, top_p=0.3)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_the_only_entry_has_log_probability_zero(ctx, torch_cuda, rng, kind):
+    """Exactly, whatever its score and the temperature, and no token's is above zero."""
+    t = torch_cuda
+    rows, cols = 64, 3001
+    x = rng.normal(0, 3, (rows, cols)).astype(np.float32)
+    x[::4] *= 1e-3
+    x[np.arange(rows), rng.integers(0, cols, rows)] = x.max(axis=1) * rng.uniform(1.1, 1.5, rows)
+    x = place(t, x, kind)
+    one = np.zeros((rows, cols), bool)
+    one[np.arange(rows), rng.integers(0, cols, rows)] = True
+    temperature = (10.0 ** rng.uniform(-2, 2, rows)).astype(np.float32)
+    for allowed, cuts in ((None, dict(top_k=1)), (None, dict(top_p=0.0)), (None, dict(min_p=1.0)), (one, dict()), (one, dict(top_k=40)),
+                          (one, dict(top_p=0.9)), (one, dict(min_p=0.1)), (None, dict(top_k=1, top_p=0.5, min_p=0.5))):
+        _, logprob = run_sample(ctx, t, x, None if allowed is None else bits_of(t, allowed),
+                                **settings(t, rows, uniform=rng.random(rows), temperature=temperature, **cuts))
+        assert (logprob == 0).all(), (cuts, logprob[logprob != 0])
+    for cuts in (dict(), dict(top_k=2), dict(top_p=0.9), dict(top_k=400), dict(min_p=0.5)):
+        _, logprob = run_sample(ctx, t, x, **settings(t, rows, uniform=rng.random(rows), temperature=temperature / 50, **cuts))
+        assert (logprob <= 0).all(), (cuts, logprob[logprob > 0])
+
+
 def test_sample_random_numbers_at_the_ends(ctx, torch_cuda, rng):
     t = torch_cuda
     x = scores(t, rng, 6, 5000, "float32")
