@@ -9,9 +9,10 @@
  * So a row belongs to a cluster of 1 to 8 blocks.  Every block copies its
  * share of the row to shared memory once (cp.async, 16 bytes a thread), all
  * passes read that copy, and the blocks tell one another what they found
- * through distributed shared memory.  HBM sees the row once.  No scratch
- * memory is used at all: launches on different streams or in captured graphs
- * share nothing.
+ * through distributed shared memory.  HBM sees the row once, up to eight
+ * blocks' 192 KB; longer rows are read again by every pass (draws from 128
+ * rows of 2^20 bf16 338 us, with top_p 0.9 1117).  No scratch memory is used
+ * at all: launches on different streams or in captured graphs share nothing.
  *
  * Inside a block every warp owns a contiguous piece of the share, so that
  * sums over warps in order are sums over the row in order; a thread reads the
@@ -397,7 +398,8 @@ template <class T, bool RESIDENT> struct Row : Share<T, RESIDENT> {
 };
 
 /* a vector of a result row laid out like the share's row; 16-byte stores where both start at the same place of a
- * 16-byte word */
+ * 16-byte word, else entry by entry: the gradient from statistics of 1500 x 100003 fp16 takes 108 us with rows every
+ * 100003 in scores and gradient, 101 with every 100032 in both, 365 to 377 with one of each */
 template <class T, bool R> __device__ __forceinline__ void put(const Share<T, R> &share, T *row, bool same, int v, const uint4 &w) {
     if (same && share.whole(v))
         *reinterpret_cast<uint4 *>(row + share.entry(v)) = w;

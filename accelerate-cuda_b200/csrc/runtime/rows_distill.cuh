@@ -104,10 +104,10 @@ __device__ __noinline__ float row_loss(const RowSums &all, double named, double 
  * Maximum and sum are taken per warp, each by itself, and joined once per row by one warp of every block; the gradient is
  * written from the staged copy everywhere as if no entry were named, then the named ones once more.
  *
- * Loss and gradient of 4096 x 131072 bf16, 64 named, with the rest: 524 us, 4.0 TB/s, 61 % of the copy rate; the special
+ * Loss and gradient of 4096 x 131072 bf16, 64 named, with the rest: 531 us, 3.9 TB/s, 60 % of the copy rate; the special
  * function unit, two exponentials an entry, is busy for 47 % and the row's chain of steps is the rest.  The loss alone of
- * 2048 x 50257 floats: 122 us, half of the copy rate.  The gradient from statistics needs no exchange and is bound by HBM
- * (1024 x 131072 bf16 at 96 % of the copy rate); where rows start anywhere, as 1500 x 100003 fp16 do, 107 us, 84 %.
+ * 2048 x 50257 floats: 124 us, half of the copy rate.  The gradient from statistics needs no exchange and is bound by HBM
+ * (1024 x 131072 bf16 89 us, 92 % of the copy rate); where rows start anywhere, as 1500 x 100003 fp16 do, 107 us, 84 %.
  * One row per cluster: clusters that stay and fetch the next row in the place of this one, vector by vector behind
  * the gradient pass, took 560 us; 2 blocks an SM the same as 3, blocks of 128, 384, 512 and
  * 1024 threads more.

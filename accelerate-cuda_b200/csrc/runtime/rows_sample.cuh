@@ -120,8 +120,8 @@ struct NoCutSpace {
  *                    what every block holds (bfloat16), only the share with the token is looked through, by all blocks
  * Clusters stay for row after row, as in top_rows.
  *
- * 1024 x 131072 bf16: without cuts 237 us (1.1 TB/s, 17 % of the copy rate), issue slots 57 % and the 64-bit
- * pipe 32 % busy: eight operations a weight; the best entry 70 us (58 %), top_k 50 146 us, top_k 400 415 us, top_p 0.9 525 us, min_p 0.05 136 us.
+ * 1024 x 131072 bf16: without cuts 238 us (1.1 TB/s, 17 % of the copy rate), issue slots 57 % and the 64-bit
+ * pipe 32 % busy: eight operations a weight; the best entry 70 us (58 %), top_k 50 146 us, top_k 400 416 us, top_p 0.9 533 us, min_p 0.05 138 us.
  * Weights in 32 bits with a bound on their error, and again in 64 where the bound could not tell two indices apart, took
  * 343 us: with a hundred thousand like entries it seldom can.
  *

@@ -524,7 +524,6 @@ __device__ __noinline__ Border border_by_bins(const Row<T, RESIDENT> share, Fine
     if (k > 0) {
         const int bin = find(0, counted, [&](u64) { return k; });
         if (bin < 0) { /* fewer than k */
-            k = 0;
             if (!(top_p < 1.0)) return Border{key_of(neg_inf()), 0, 0};
             return find_border<T, RESIDENT, true>(share, lv, size, key_of(from), key_of(most), 0, weigh, top_p, 0);
         }

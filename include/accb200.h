@@ -301,7 +301,9 @@ ACCB_API int accb_sample_rows(accb_context *ctx, accb_stream stream, const accb_
  *          third is the maximum of the unnamed entries and the fourth the factor of exp((x - that) / temperature).
  *   grad   NULL, or the gradient of sum(loss) in the student's shape and type, written in the same pass:
  *          weight / temperature * (factor * q - p).  It may be the student's own memory (same pointer and pitch);
- *          any other overlap of the two is refused. */
+ *          any other overlap of the two is refused.  Its rows are written whole vectors at a time where they start at
+ *          the same place of a 16-byte word as the student's -- give both one pitch -- and several times slower
+ *          elsewhere. */
 ACCB_API int accb_distill_rows(accb_context *ctx, accb_stream stream, const accb_rows_array *student, const void *teacher,
                                int teacher_type, const int32_t *index, int k, const float *teacher_lse,
                                const float *weight, double temperature, float *loss, float *stats,
